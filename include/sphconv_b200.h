@@ -313,6 +313,59 @@ int sph_voxelize_fill(const float* d_points, int32_t point_stride, const float* 
                       int64_t nnz, float* d_feature, int32_t* d_z_idx, int32_t* d_coordinates, int32_t* d_num_points,
                       void* stream);
 
+/* ---- a head on the encoder's rows, and its training step --------------------------------------------------------------
+ * No counterparts in the reference, whose path ends with the convolution.
+ *
+ * Norms before and after a block, fused with its gate and residual scale:
+ *   inner  = norm(block) * weight + bias                 (inner = block where param[0] is null)
+ *   out    = residual + scale[c] * sigmoid(gate) * inner
+ *   normed = norm(out) * next_weight + next_bias         (of the sum before it is rounded)
+ *   norm(x) = x / sqrt(mean(x^2) + eps); with center != 0 (x - mean(x)) / sqrt(var(x) + eps)
+ * Without a block the norm alone: normed = norm(residual) * next_weight + next_bias, and no out.
+ *   param        weight, bias, scale, next_weight, next_bias: [c] of param_dtype each (SPH_F32, SPH_F16, SPH_BF16), or null;
+ *                a bias needs its weight
+ *   gate         [n,c], or [n] with gate_per_row != 0, in `dtype`; null: none
+ *   d_stats      float [n,4], 16-byte aligned: what the backward pass needs of the forward one; null: not kept
+ * Backward: d_dout and d_dnormed are the gradients of out and normed (either may be null: zeros); every result may be null (not
+ * wanted).  d_dparam[i] is of param_dtype[i].  The scratch is left free to be used again when the launches have run.
+ * Rows are contiguous, of SPH_F32, SPH_F16 or SPH_BF16; statistics and sums are fp32.  Results do not depend on the run. */
+#define SPH_NORM_MAX_CHANNELS 8192
+typedef struct sph_norm {
+  int64_t n;
+  int32_t c;
+  int32_t dtype;
+  int32_t center;
+  int32_t gate_per_row;
+  float eps;
+  const void *block, *residual, *gate;
+  const void* param[5];
+  int32_t param_dtype[5];
+} sph_norm;
+int sph_residual_norm(const sph_norm* args, void* d_out, void* d_normed, float* d_stats, void* stream);
+int64_t sph_residual_norm_scratch_bytes(int64_t n, int32_t c);
+int sph_residual_norm_backward(const sph_norm* args, const void* d_dout, const void* d_dnormed, const float* d_stats,
+                               void* d_scratch, void* d_dblock, void* d_dresidual, void* d_dgate, void* const d_dparam[5],
+                               void* stream);
+
+/* The global norm of `count` gradients, and clipping by it:  *d_norm = sqrt(sum g^2) (SPH_NORM_2; sums in 64 bits) or max |g|
+ * (SPH_NORM_MAX; NaN if any is), and  dst = src * min(1, max_norm / (*d_norm + 1e-6)).
+ *   tensors      host array; n values of src_dtype at src, and of dst_dtype at dst (SPH_F32, SPH_F16, SPH_BF16).  dst may be src
+ *                (of one dtype); no dst may overlap anything else in the list
+ *   d_scratch    sph_grad_norm_scratch_bytes(count) bytes, 8-byte aligned
+ * The array is copied into the launches: it may be freed at once, and a captured graph keeps its own. */
+#define SPH_NORM_2 0
+#define SPH_NORM_MAX 1
+typedef struct sph_clip_tensor {
+  const void* src;
+  void* dst;
+  int64_t n;
+  int32_t src_dtype, dst_dtype;
+} sph_clip_tensor;
+int64_t sph_grad_norm_scratch_bytes(int32_t count);
+int sph_grad_norm(const sph_clip_tensor* tensors, int32_t count, int norm_kind, void* d_scratch, float* d_norm, void* stream);
+int sph_grad_clip(const sph_clip_tensor* tensors, int32_t count, int norm_kind, float max_norm, void* d_scratch, float* d_norm,
+                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

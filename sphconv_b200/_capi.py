@@ -39,6 +39,17 @@ class VoxelGrid(ctypes.Structure):
                 ("max_voxels", i32), ("append_mode", i32)]
 
 
+class Norm(ctypes.Structure):
+    """struct sph_norm"""
+    _fields_ = [("n", i64), ("c", i32), ("dtype", i32), ("center", i32), ("gate_per_row", i32), ("eps", ctypes.c_float),
+                ("block", vp), ("residual", vp), ("gate", vp), ("param", vp * 5), ("param_dtype", i32 * 5)]
+
+
+class ClipTensor(ctypes.Structure):
+    """struct sph_clip_tensor"""
+    _fields_ = [("src", vp), ("dst", vp), ("n", i64), ("src_dtype", i32), ("dst_dtype", i32)]
+
+
 # name -> (restype, argtypes); exactly the symbols include/sphconv_b200.h declares
 SIGNATURES = {
     "sph_last_error": (ctypes.c_char_p, []),
@@ -77,6 +88,12 @@ SIGNATURES = {
     "sph_voxel_feature_count": (cint, [i32, cint]),
     "sph_voxelize_scratch_bytes": (i64, [ctypes.POINTER(VoxelGrid), i64]),
     "sph_voxelize_count": (cint, [vp, vp, i64, ctypes.POINTER(VoxelGrid), vp, vp, c_i32p, vp]),
+    "sph_residual_norm": (cint, [ctypes.POINTER(Norm), vp, vp, vp, vp]),
+    "sph_residual_norm_scratch_bytes": (i64, [i64, i32]),
+    "sph_residual_norm_backward": (cint, [ctypes.POINTER(Norm), vp, vp, vp, vp, vp, vp, vp, ctypes.POINTER(vp), vp]),
+    "sph_grad_norm_scratch_bytes": (i64, [i32]),
+    "sph_grad_norm": (cint, [ctypes.POINTER(ClipTensor), i32, cint, vp, vp, vp]),
+    "sph_grad_clip": (cint, [ctypes.POINTER(ClipTensor), i32, cint, ctypes.c_float, vp, vp, vp]),
     "sph_voxelize_fill": (cint, [vp, i32, vp, vp, i64, ctypes.POINTER(VoxelGrid), vp, i64, vp, vp, vp, vp, vp]),
 }
 

@@ -33,7 +33,8 @@ using Ints = std::vector<int64_t>;
   X(sph_rules_to_nbr) X(sph_packed_weight_bytes) X(sph_pack_weight) X(sph_conv_gather) X(sph_conv_wgrad)             \
   X(sph_init_tensor_scratch_bytes) X(sph_init_tensor) X(sph_permute_rows) X(sph_dense_channels_first)                \
   X(sph_epilogue_backward) X(sph_voxel_transform) X(sph_voxel_feature_count) X(sph_voxelize_scratch_bytes)           \
-  X(sph_voxelize_count) X(sph_voxelize_fill)
+  X(sph_voxelize_count) X(sph_voxelize_fill) X(sph_residual_norm) X(sph_residual_norm_scratch_bytes)                  \
+  X(sph_residual_norm_backward) X(sph_grad_norm_scratch_bytes) X(sph_grad_norm) X(sph_grad_clip)
 
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
@@ -552,6 +553,213 @@ Tensor conv_layer(const Tensor& feature, const Tensor& weight, const optional<Te
   return ConvLayer::apply(feature, weight, bias, nbr, nbr_t, n_out, relu);
 }
 
+// ---- a head on the encoder's rows ------------------------------------------------------------------------------------
+// No gradient of these operators' gradients: refused, where autograd would take them for constants.
+void once_differentiable(const char* who) {
+  if (at::GradMode::is_enabled()) fail(std::string(who) + ": not differentiable twice (create_graph)");
+}
+
+struct NormInputs {
+  optional<Tensor> block;
+  Tensor residual;
+  optional<Tensor> gate;
+  std::array<optional<Tensor>, 5> param;      // weight, bias, scale, next_weight, next_bias
+  double eps;
+  bool center;
+
+  sph_norm args() const {
+    sph_norm a = {};
+    a.c = (int32_t)residual.size(-1);
+    a.n = a.c ? residual.numel() / a.c : 0;
+    a.dtype = dtype_code(residual, "row");
+    a.center = center;
+    a.gate_per_row = gate && gate->size(-1) == 1 && a.c != 1;
+    a.eps = (float)eps;
+    a.block = ptr(block);
+    a.residual = ptr(residual);
+    a.gate = ptr(gate);
+    for (int i = 0; i < 5; ++i) {
+      a.param[i] = ptr(param[i]);
+      a.param_dtype[i] = param[i] ? dtype_code(*param[i], "parameter") : SPH_F32;
+    }
+    return a;
+  }
+};
+
+// Checks and brings parameters to consecutive memory.
+NormInputs norm_inputs(const optional<Tensor>& block, const Tensor& residual, const optional<Tensor>& gate,
+                       const std::array<optional<Tensor>, 5>& param, double eps, bool center) {
+  require_cuda(residual);
+  require_cuda(block);
+  require_cuda(gate);
+  if (residual.dim() < 1 || residual.size(-1) < 1 || residual.size(-1) > SPH_NORM_MAX_CHANNELS)
+    fail("rows of 1 to " + std::to_string(SPH_NORM_MAX_CHANNELS) + " channels are needed");
+  if (dtype_code(residual, "row") == SPH_I8) fail("rows are float32, float16 or bfloat16");
+  auto same = [&](const optional<Tensor>& t, const char* what) {
+    if (t && (t->scalar_type() != residual.scalar_type() || t->device() != residual.device()))
+      fail(std::string(what) + " must have the residual's dtype and device");
+  };
+  same(block, "block");
+  same(gate, "gate");
+  if (block && block->sizes() != residual.sizes()) fail("block and residual must have one shape");
+  if (gate) {
+    auto rows = residual.sizes().vec();
+    rows.back() = 1;
+    if (gate->sizes() != residual.sizes() && gate->sizes() != at::IntArrayRef(rows)) fail("the gate has the residual's shape, or one value a row");
+  }
+  NormInputs in{block, residual, gate, param, eps, center};
+  for (auto& p : in.param) {
+    if (!p) continue;
+    if (p->dim() != 1 || p->size(0) != residual.size(-1) || p->device() != residual.device())
+      fail("weights, biases and the scale have one value a channel, on the rows' device");
+    if (dtype_code(*p, "parameter") == SPH_I8) fail("parameters are float32, float16 or bfloat16");
+    p = p->contiguous();
+  }
+  if (!block && (gate || param[0] || param[1] || param[2])) fail("a gate, a scale or a norm of no block");
+  if ((param[1] && !param[0]) || (param[4] && !param[3])) fail("a bias needs its weight");
+  if (!block && !param[3]) fail("nothing to compute");
+  if (!(eps >= 0)) fail("eps must not be negative");
+  return in;
+}
+
+struct NormOutputs {
+  Tensor out, normed, stats;                  // out without a block, normed without a next_weight, stats without training: undefined
+};
+NormOutputs norm_forward(const NormInputs& in, bool train) {
+  const c10::cuda::CUDAGuard guard(in.residual.device());
+  const sph_norm a = in.args();
+  NormOutputs r;
+  if (in.block) r.out = at::empty_like(in.residual);
+  if (in.param[3]) r.normed = at::empty_like(in.residual);
+  if (train) r.stats = empty({a.n, 4}, at::kFloat, in.residual);
+  if (a.n)
+    check(abi.sph_residual_norm(&a, in.block ? ptr(r.out) : nullptr, in.param[3] ? ptr(r.normed) : nullptr,
+                                train ? static_cast<float*>(ptr(r.stats)) : nullptr, stream_of(in.residual)));
+  return r;
+}
+
+struct NormLayer : public torch::autograd::Function<NormLayer> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const optional<Tensor>& block,
+                                                const Tensor& residual, const optional<Tensor>& gate, const optional<Tensor>& weight,
+                                                const optional<Tensor>& bias, const optional<Tensor>& scale,
+                                                const optional<Tensor>& next_weight, const optional<Tensor>& next_bias, double eps,
+                                                bool center) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const NormInputs in = norm_inputs(block, residual, gate, {weight, bias, scale, next_weight, next_bias}, eps, center);
+    const NormOutputs r = norm_forward(in, true);
+    auto or_undefined = [](const optional<Tensor>& t) { return t.value_or(Tensor()); };
+    ctx->save_for_backward({or_undefined(block), residual, or_undefined(gate), or_undefined(weight), or_undefined(bias),
+                            or_undefined(scale), or_undefined(next_weight), or_undefined(next_bias), r.stats});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["center"] = center;
+    ctx->set_materialize_grads(false);
+    torch::autograd::variable_list outs;
+    if (r.out.defined()) outs.push_back(r.out);
+    if (r.normed.defined()) outs.push_back(r.normed);
+    return outs;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    once_differentiable("residual_norm");
+    const auto saved = ctx->get_saved_variables();
+    auto given = [&](int i) { return saved[i].defined() ? optional<Tensor>(saved[i]) : std::nullopt; };
+    const NormInputs in = norm_inputs(given(0), saved[1], given(2), {given(3), given(4), given(5), given(6), given(7)},
+                                      ctx->saved_data["eps"].toDouble(), ctx->saved_data["center"].toBool());
+    const Tensor& stats = saved[8];
+    const c10::cuda::CUDAGuard guard(in.residual.device());
+    Tensor d_out, d_normed;
+    size_t at = 0;
+    if (in.block) d_out = grads[at++];
+    if (in.param[3]) d_normed = grads[at];
+    auto ready = [&](Tensor& g) { if (g.defined()) g = g.to(in.residual.scalar_type()).contiguous(); };
+    ready(d_out);
+    ready(d_normed);
+    // inputs: block, residual, gate, weight, bias, scale, next_weight, next_bias
+    std::array<Tensor, 8> d;
+    size_t edge = 0;                          // autograd numbers the tensors that were given
+    auto make = [&](int i, const optional<Tensor>& like) {
+      if (like && ctx->needs_input_grad(edge++)) d[i] = at::empty_like(*like, at::MemoryFormat::Contiguous);
+    };
+    make(0, in.block);
+    make(1, in.residual);
+    make(2, in.gate);
+    for (int i = 0; i < 5; ++i) make(3 + i, in.param[i]);
+    const sph_norm a = in.args();
+    const Tensor scratch = empty({check(abi.sph_residual_norm_scratch_bytes(a.n, a.c))}, at::kByte, in.residual);
+    auto at_or_null = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    void* d_param[5];
+    for (int i = 0; i < 5; ++i) d_param[i] = at_or_null(d[3 + i]);
+    check(abi.sph_residual_norm_backward(&a, at_or_null(d_out), at_or_null(d_normed), static_cast<const float*>(at_or_null(stats)),
+                                         ptr(scratch), at_or_null(d[0]), at_or_null(d[1]), at_or_null(d[2]), d_param,
+                                         stream_of(in.residual)));
+    return {d[0], d[1], d[2], d[3], d[4], d[5], d[6], d[7], Tensor(), Tensor()};
+  }
+};
+
+// -> (out or None, normed or None)
+py::tuple residual_norm(const optional<Tensor>& block, const Tensor& residual, const optional<Tensor>& gate,
+                        const optional<Tensor>& weight, const optional<Tensor>& bias, const optional<Tensor>& scale,
+                        const optional<Tensor>& next_weight, const optional<Tensor>& next_bias, double eps, bool center) {
+  bool train = residual.requires_grad();
+  for (const auto* t : {&block, &gate, &weight, &bias, &scale, &next_weight, &next_bias}) train |= *t && (*t)->requires_grad();
+  Tensor out, normed;
+  if (train && at::GradMode::is_enabled()) {
+    const auto r = NormLayer::apply(block, residual, gate, weight, bias, scale, next_weight, next_bias, eps, center);
+    if (block) out = r.front();
+    if (next_weight) normed = r.back();
+  } else {
+    const NormOutputs r = norm_forward(norm_inputs(block, residual, gate, {weight, bias, scale, next_weight, next_bias}, eps, center), false);
+    out = r.out;
+    normed = r.normed;
+  }
+  return py::make_tuple(or_none(out), or_none(normed));
+}
+
+// Norm of many gradients (max_norm absent), or the norm with every gradient scaled into `out` (or where it is).
+Tensor grad_clip(const std::vector<Tensor>& grads, const optional<std::vector<Tensor>>& out, optional<double> max_norm, bool largest) {
+  if (grads.empty()) fail("no gradients");
+  if (out && out->size() != grads.size()) fail("as many destinations as gradients are needed");
+  if (max_norm && !(*max_norm >= 0)) fail("max_norm must not be negative");
+  std::vector<sph_clip_tensor> list(grads.size());
+  struct Span { uintptr_t begin, end; size_t of; bool written; };
+  std::vector<Span> spans;
+  const auto device = grads[0].device();
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor &g = grads[i], &o = out ? (*out)[i] : g;
+    for (const Tensor* t : {&g, &o}) {
+      if (!t->is_cuda()) require_cuda(*t);
+      if (t->device() != device) fail("gradients on several devices: take their norms apart");
+      if (!t->is_non_overlapping_and_dense()) fail("sphconv_b200 ops need contiguous tensors");
+      if (dtype_code(*t, "gradient") == SPH_I8) fail("gradients are float32, float16 or bfloat16");
+    }
+    if (g.sizes() != o.sizes() || (g.strides() != o.strides() && !(g.is_contiguous() && o.is_contiguous())))
+      fail("a destination must have its gradient's shape and layout");
+    list[i] = {ptr(g), ptr(o), g.numel(), dtype_code(g, "gradient"), dtype_code(o, "gradient")};
+    if (!max_norm || g.numel() == 0) continue;
+    const uintptr_t src = (uintptr_t)list[i].src, dst = (uintptr_t)list[i].dst;
+    spans.push_back({dst, dst + o.nbytes(), i, true});
+    if (src != dst || list[i].src_dtype != list[i].dst_dtype) spans.push_back({src, src + g.nbytes(), i, false});
+  }
+  // every value is read and written by one thread, and in any order: nothing that is written may be anything else's memory
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  uintptr_t written = 0, read = 0;
+  for (const Span& s : spans) {
+    if (s.begin < written || (s.written && s.begin < read)) fail("a gradient is in the list twice, or overlaps another one or a destination");
+    (s.written ? written : read) = std::max(s.written ? written : read, s.end);
+  }
+  const c10::cuda::CUDAGuard guard(device);
+  const int32_t count = (int32_t)list.size();
+  const int kind = largest ? SPH_NORM_MAX : SPH_NORM_2;
+  Tensor norm = empty({}, at::kFloat, grads[0]);
+  Tensor scratch = empty({check(abi.sph_grad_norm_scratch_bytes(count))}, at::kByte, grads[0]);
+  float* to = static_cast<float*>(ptr(norm));
+  if (max_norm) check(abi.sph_grad_clip(list.data(), count, kind, (float)*max_norm, ptr(scratch), to, stream_of(norm)));
+  else check(abi.sph_grad_norm(list.data(), count, kind, ptr(scratch), to, stream_of(norm)));
+  if (max_norm)                               // the values were written behind autograd's back
+    for (const Tensor& t : out ? *out : grads) if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
 // ---- tensor operations ---------------------------------------------------------------------------------------------
 // COO rows -> (rows in range-voxel order, z_idx, z_ptr, permutation)
 py::tuple init_tensor(const Tensor& feature_in, const Tensor& indices, int64_t B, const Ints& shape) {
@@ -686,6 +894,8 @@ PYBIND11_MODULE(sph_host, m) {
   m.def("conv_wgrad", &conv_wgrad);
   m.def("epilogue_backward", &epilogue_backward);
   m.def("conv_layer", &conv_layer);
+  m.def("residual_norm", &residual_norm);
+  m.def("grad_clip", &grad_clip);
   m.def("init_tensor", &init_tensor);
   m.def("gather_rows", &gather_rows);
   m.def("dense_channels_first", &dense_channels_first);

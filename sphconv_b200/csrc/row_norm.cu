@@ -1,0 +1,597 @@
+// Norms before and after a block, fused with the block's gate and residual scale, and the gradients of all of it.
+//
+//   inner  = norm(block) * weight + bias            (inner = block without a weight)
+//   out    = residual + scale[c] * sigmoid(gate) * inner
+//   normed = norm(out) * next_weight + next_bias    (from the sum before it is rounded)
+//   norm(x) = x / sqrt(mean(x^2) + eps), or (x - mean(x)) / sqrt(var(x) + eps) with CENTER
+//
+// One pass: a row is read once into registers, by 1 to 512 threads that hold E values each, reduced among them (shuffles, or shared
+// memory where they are more than a warp) and written.  Statistics and sums are float32; rows are rounded once.  Bound by HBM.
+// The variance is the mean of squared deviations, which the values in registers make as cheap as the mean of squares.
+//
+// Backward reads the block, the residual, the gate and the two gradients, makes `out` again in float32 (the rounded one would shift
+// the gradient of a 16-bit row's norm) and takes mean and 1/deviation of both norms from the forward pass (16 bytes a row).  The
+// threads of a persistent grid own columns, so the sums over rows - gradients of weights, biases and the scale - stay in registers
+// until the end; each block leaves its sums in the scratch, and a second launch adds those up in a fixed order: no atomics, the same
+// bits every time.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace sph {
+
+namespace {
+
+constexpr int kBlock = 256;                   // threads of a block where a row takes a warp or less
+constexpr int kMaxWarps = 16;                 // of a row
+constexpr int kSums = 5;                      // sums over rows: weight, bias, scale, next_weight, next_bias
+
+struct Params {
+  const void *block, *residual, *gate;        // [n, c], [n, c], [n, c] or [n]; block and gate may be null
+  const void* param[kSums];                   // weight, bias, scale, next_weight, next_bias [c]: any may be null
+  int param_dtype[kSums];
+  const void *d_out, *d_normed;               // backward: either may be null
+  void *out, *normed;                         // forward: either may be null
+  void *d_block, *d_residual, *d_gate;        // backward: any may be null
+  float* stats;                               // [n][4]: mean and 1/deviation of block and of out; null: not wanted
+  float* partial;                             // backward: [blocks][kSums][c]
+  int64_t n;
+  int c, lanes, gate_row;                     // lanes: threads of a row, a power of two
+  float eps;
+};
+
+template <typename T> struct Row;
+template <> struct Row<float> {
+  static constexpr int kVec = 4;
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ float put(float v) { return v; }
+};
+template <> struct Row<__half> {
+  static constexpr int kVec = 8;
+  static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
+};
+template <> struct Row<__nv_bfloat16> {
+  static constexpr int kVec = 8;
+  static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
+};
+
+// A thread's values of a row: NV pieces of VEC consecutive ones, piece j at (j * lanes + t) * VEC.
+template <typename T, int VEC, int NV>
+struct Tile {
+  static constexpr int E = VEC * NV;
+  struct __align__(VEC * sizeof(T)) Piece { T v[VEC]; };
+
+  static __device__ __forceinline__ int column(int j, int t, int lanes) { return (j * lanes + t) * VEC; }
+
+  static __device__ __forceinline__ void load(float (&x)[E], const void* base, int64_t row, int c, int t, int lanes, bool active) {
+    const T* p = (const T*)base + row * c;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int at = column(j, t, lanes);
+      Piece q;
+      if (active && at < c) {
+        q = *(const Piece*)(p + at);          // c is a multiple of VEC
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) q.v[i] = Row<T>::put(0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[j * VEC + i] = Row<T>::get(q.v[i]);
+    }
+  }
+  static __device__ __forceinline__ void store(const float (&x)[E], void* base, int64_t row, int c, int t, int lanes, bool active) {
+    T* p = (T*)base + row * c;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int at = column(j, t, lanes);
+      if (active && at < c) {
+        Piece q;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) q.v[i] = Row<T>::put(x[j * VEC + i]);
+        *(Piece*)(p + at) = q;
+      }
+    }
+  }
+  // a parameter [c] of float32 or of 16 bits, or `other` where there is none; 16-byte aligned where rows come in pieces
+  static __device__ __forceinline__ void param(float (&x)[E], const void* p, int dtype, float other, int c, int t, int lanes) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int at = column(j, t, lanes);
+      if constexpr (VEC > 1) {
+        if (p == nullptr || at >= c) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) x[j * VEC + i] = other;
+        } else if (dtype == SPH_F32) {
+#pragma unroll
+          for (int i = 0; i < VEC / 4; ++i) {
+            const float4 f = __ldg((const float4*)((const float*)p + at) + i);
+            x[j * VEC + 4 * i] = f.x; x[j * VEC + 4 * i + 1] = f.y;
+            x[j * VEC + 4 * i + 2] = f.z; x[j * VEC + 4 * i + 3] = f.w;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC / 4; ++i) {
+            const uint2 h = __ldg((const uint2*)((const unsigned short*)p + at) + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const unsigned short bits = (unsigned short)((k < 2 ? h.x : h.y) >> (16 * (k & 1)));
+              x[j * VEC + 4 * i + k] =
+                  dtype == SPH_F16 ? __half2float(__ushort_as_half(bits)) : __uint_as_float((unsigned)bits << 16);
+            }
+          }
+        }
+      } else {
+        float v = other;
+        if (p && at < c) {
+          if (dtype == SPH_F32) {
+            v = __ldg((const float*)p + at);
+          } else {
+            const unsigned short bits = __ldg((const unsigned short*)p + at);
+            v = dtype == SPH_F16 ? __half2float(__ushort_as_half(bits)) : __uint_as_float((unsigned)bits << 16);
+          }
+        }
+        x[j] = v;
+      }
+    }
+  }
+};
+
+// Sums over the threads of a row, in every one of them.  More than a warp: the block is one row, and calls alternate between two
+// places in shared memory, so that one barrier a call is enough.
+struct Reducer {
+  float (*slots)[kMaxWarps][4];               // [2][warps][4]
+  int lanes, turn;
+  template <int N>
+  __device__ __forceinline__ void sum(float (&v)[N]) {
+    for (int o = min(lanes, 32) >> 1; o > 0; o >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
+    if (lanes > 32) {
+      const int warp = threadIdx.x >> 5, warps = lanes >> 5;
+      if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) slots[turn][warp][i] = v[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = 0.f;
+      for (int w = 0; w < warps; ++w) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += slots[turn][w][i];
+      }
+      turn ^= 1;
+    }
+  }
+};
+
+// mean and 1/deviation of a row
+template <bool CENTER, int VEC, int NV>
+__device__ __forceinline__ void statistics(const float (&x)[VEC * NV], Reducer& red, int c, int t, float eps, float& mean, float& inv) {
+  constexpr int E = VEC * NV;
+  mean = 0.f;
+  float s[1];
+  if (CENTER) {
+    s[0] = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[0] += x[e];
+    red.sum(s);
+    mean = s[0] / (float)c;
+  }
+  s[0] = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float d = x[j * VEC + i] - mean;
+      if (!CENTER || (j * red.lanes + t) * VEC + i < c) s[0] = fmaf(d, d, s[0]);       // behind the row are zeros
+    }
+  red.sum(s);
+  inv = 1.f / sqrtf(s[0] / (float)c + eps);
+}
+
+__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
+
+template <typename T>
+__device__ __forceinline__ float row_gate(const Params& p, int64_t row, bool active) {
+  return active ? sigmoid(Row<T>::get(((const T*)p.gate)[row])) : 0.f;
+}
+
+template <typename T, int VEC, int NV, bool CENTER>
+__global__ void __launch_bounds__(512) forward_kernel(const __grid_constant__ Params p) {
+  using X = Tile<T, VEC, NV>;
+  constexpr int E = X::E;
+  __shared__ float slots[2][kMaxWarps][4];
+  after_previous();
+  const int lanes = p.lanes, c = p.c, t = threadIdx.x & (lanes - 1), rows = blockDim.x / lanes;
+  Reducer red{slots, lanes, 0};
+  for (int64_t base = (int64_t)blockIdx.x * rows; base < p.n; base += (int64_t)gridDim.x * rows) {
+    const int64_t row = base + threadIdx.x / lanes;
+    const bool active = row < p.n;
+    float out[E], b[E], g[E], w[E];
+    float mean = 0.f, inv = 1.f;
+    X::load(out, p.residual, row, c, t, lanes, active);
+    if (p.block) {
+      X::load(b, p.block, row, c, t, lanes, active);
+      const bool gated = p.gate && !p.gate_row;
+      if (gated) X::load(g, p.gate, row, c, t, lanes, active);
+      const float rg = p.gate && p.gate_row ? row_gate<T>(p, row, active) : 1.f;
+      if (p.param[0]) {
+        statistics<CENTER, VEC, NV>(b, red, c, t, p.eps, mean, inv);
+        X::param(w, p.param[0], p.param_dtype[0], 1.f, c, t, lanes);
+#pragma unroll
+        for (int e = 0; e < E; ++e) b[e] = (b[e] - mean) * inv * w[e];
+        if (p.param[1]) {
+          X::param(w, p.param[1], p.param_dtype[1], 0.f, c, t, lanes);
+#pragma unroll
+          for (int e = 0; e < E; ++e) b[e] += w[e];
+        }
+      }
+      if (p.stats && t == 0 && active) *(float2*)(p.stats + row * 4) = make_float2(mean, inv);
+      X::param(w, p.param[2], p.param_dtype[2], 1.f, c, t, lanes);
+#pragma unroll
+      for (int e = 0; e < E; ++e) out[e] = fmaf(w[e] * (gated ? sigmoid(g[e]) : rg), b[e], out[e]);
+      if (p.out) X::store(out, p.out, row, c, t, lanes, active);
+    }
+    if (p.normed) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)                                  // what a bias added behind the row's end
+        if (X::column(j, t, lanes) >= c) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) out[j * VEC + i] = 0.f;
+        }
+      statistics<CENTER, VEC, NV>(out, red, c, t, p.eps, mean, inv);
+      if (p.stats && t == 0 && active) *(float2*)(p.stats + row * 4 + 2) = make_float2(mean, inv);
+      X::param(w, p.param[3], p.param_dtype[3], 1.f, c, t, lanes);
+      X::param(b, p.param[4], p.param_dtype[4], 0.f, c, t, lanes);
+#pragma unroll
+      for (int e = 0; e < E; ++e) out[e] = fmaf((out[e] - mean) * inv, w[e], b[e]);
+      X::store(out, p.normed, row, c, t, lanes, active);
+    }
+  }
+}
+
+template <typename T, int VEC, int NV, bool CENTER>
+__global__ void __launch_bounds__(512) backward_kernel(const __grid_constant__ Params p) {
+  using X = Tile<T, VEC, NV>;
+  constexpr int E = X::E;
+  __shared__ float slots[2][kMaxWarps][4];
+  extern __shared__ float columns[];                                // rows of a block > 1: [kBlock][E]
+  after_previous();
+  const int lanes = p.lanes, c = p.c, t = threadIdx.x & (lanes - 1), rows = blockDim.x / lanes;
+  const float per_c = 1.f / (float)c;
+  Reducer red{slots, lanes, 0};
+  float sums[kSums][E];
+#pragma unroll
+  for (int s = 0; s < kSums; ++s)
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[s][e] = 0.f;
+  for (int64_t base = (int64_t)blockIdx.x * rows; base < p.n; base += (int64_t)gridDim.x * rows) {
+    const int64_t row = base + threadIdx.x / lanes;
+    const bool active = row < p.n;
+    const bool gated = p.gate && !p.gate_row;
+    float x[E], b[E], g[E], w[E], total[E], dn[E];
+    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (active) st = *(const float4*)(p.stats + row * 4);
+    const float mb = p.param[0] ? st.x : 0.f, ib = p.param[0] ? st.y : 1.f;
+    X::load(x, p.residual, row, c, t, lanes, active);
+    float rg = 1.f;
+    if (p.block) {
+      X::load(b, p.block, row, c, t, lanes, active);
+      if (gated) X::load(g, p.gate, row, c, t, lanes, active);
+      else if (p.gate) rg = row_gate<T>(p, row, active);
+    }
+    if (p.d_out) {
+      X::load(total, p.d_out, row, c, t, lanes, active);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) total[e] = 0.f;
+    }
+    if (p.d_normed) X::load(dn, p.d_normed, row, c, t, lanes, active);
+    if (p.block) {                                                  // b: the normalised block; x: out
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        b[e] = (b[e] - mb) * ib;
+        g[e] = gated ? sigmoid(g[e]) : rg;
+      }
+    }
+    if (p.d_normed) {
+      if (p.block) {
+        float w2[E];
+        X::param(w, p.param[0], p.param_dtype[0], 1.f, c, t, lanes);
+        X::param(w2, p.param[1], p.param_dtype[1], 0.f, c, t, lanes);
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[e] = fmaf(b[e], w[e], w2[e]);
+        X::param(w2, p.param[2], p.param_dtype[2], 1.f, c, t, lanes);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = fmaf(w2[e] * g[e], w[e], x[e]);
+      }
+      X::param(w, p.param[3], p.param_dtype[3], 1.f, c, t, lanes);
+      float s[2] = {0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        x[e] = (x[e] - st.z) * st.w;                                // the normalised out; dn is zero behind the row's end
+        sums[3][e] = fmaf(dn[e], x[e], sums[3][e]);
+        sums[4][e] += dn[e];
+        dn[e] *= w[e];
+        s[0] = fmaf(dn[e], x[e], s[0]);
+        s[1] += dn[e];
+      }
+      red.sum(s);
+      s[0] *= per_c;
+      s[1] = CENTER ? s[1] * per_c : 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) total[e] = fmaf(st.w, dn[e] - s[1] - x[e] * s[0], total[e]);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (X::column(j, t, lanes) >= c) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) total[j * VEC + i] = 0.f;
+        }
+    }
+    if (p.d_residual) X::store(total, p.d_residual, row, c, t, lanes, active);
+    if (p.block) {
+      float s[3] = {0.f, 0.f, 0.f};
+      X::param(w, p.param[0], p.param_dtype[0], 1.f, c, t, lanes);
+      X::param(x, p.param[1], p.param_dtype[1], 0.f, c, t, lanes);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = fmaf(b[e], w[e], x[e]);    // inner
+      X::param(dn, p.param[2], p.param_dtype[2], 1.f, c, t, lanes);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float tg = total[e] * g[e];                           // gradient of scale * inner
+        const float d_inner = tg * dn[e];
+        sums[2][e] = fmaf(tg, x[e], sums[2][e]);
+        sums[0][e] = fmaf(d_inner, b[e], sums[0][e]);
+        sums[1][e] += d_inner;
+        x[e] = d_inner * x[e] * (1.f - g[e]);                       // gradient of the gate's logit
+        s[2] += x[e];
+        dn[e] = d_inner * w[e];
+        s[0] = fmaf(dn[e], b[e], s[0]);
+        s[1] += dn[e];
+      }
+      if (gated && p.d_gate) X::store(x, p.d_gate, row, c, t, lanes, active);
+      if (p.param[0] || p.gate_row) {
+        red.sum(s);
+        if (p.gate_row && p.d_gate && t == 0 && active) ((T*)p.d_gate)[row] = Row<T>::put(s[2]);
+      }
+      if (p.param[0]) {
+        s[0] *= per_c;
+        s[1] = CENTER ? s[1] * per_c : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) dn[e] = ib * (dn[e] - s[1] - b[e] * s[0]);
+      }
+      if (p.d_block) X::store(dn, p.d_block, row, c, t, lanes, active);
+    }
+  }
+  // the block's sums over its rows
+  if (p.partial == nullptr) return;
+#pragma unroll
+  for (int s = 0; s < kSums; ++s) {
+    if (p.param[s] == nullptr) continue;
+    float* to = p.partial + ((int64_t)blockIdx.x * kSums + s) * c;
+    if (rows > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; ++e) columns[e * kBlock + threadIdx.x] = sums[s][e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < lanes * E; i += blockDim.x) {
+        const int e = i / lanes, tt = i - e * lanes;
+        const int at = X::column(e / VEC, tt, lanes) + e % VEC;
+        if (at < c) {
+          float v = 0.f;
+          for (int r = 0; r < rows; ++r) v += columns[e * kBlock + r * lanes + tt];
+          to[at] = v;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int at = X::column(e / VEC, t, lanes) + e % VEC;
+        if (at < c) to[at] = sums[s][e];
+      }
+    }
+  }
+}
+
+// d_param[s][c] = sum over blocks of partial[block][s][c], in the order of the blocks
+struct SumParams {
+  const float* partial;
+  void* to[kSums];
+  int dtype[kSums];
+  int blocks, c;
+};
+__global__ void __launch_bounds__(256) sums_kernel(const __grid_constant__ SumParams p) {
+  __shared__ double part[8][32];
+  after_previous();
+  const int s = blockIdx.y, lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  if (p.to[s] == nullptr) return;
+  double v = 0.0;
+  if (col < p.c)
+    for (int b = w; b < p.blocks; b += 8) v += (double)p.partial[((int64_t)b * kSums + s) * p.c + col];
+  part[w][lane] = v;
+  __syncthreads();
+  if (w == 0 && col < p.c) {
+    for (int i = 1; i < 8; ++i) v += part[i][lane];
+    const float f = (float)v;
+    if (p.dtype[s] == SPH_F32) ((float*)p.to[s])[col] = f;
+    else if (p.dtype[s] == SPH_F16) ((__half*)p.to[s])[col] = __float2half_rn(f);
+    else ((__nv_bfloat16*)p.to[s])[col] = __float2bfloat16_rn(f);
+  }
+}
+
+struct Shape {
+  int vec, nv, lanes, threads;
+};
+
+// Threads of a row and pieces a thread holds.  whole: rows are a multiple of 16 bytes, and 16-byte aligned.
+bool shape_of(int c, int esize, bool whole, Shape* s) {
+  const int full = 16 / esize;
+  s->vec = whole ? full : 1;
+  // 8 values a thread; 16 where more than 512 threads would be needed
+  for (const int e : {8, 16}) {
+    s->nv = e / s->vec;
+    s->lanes = 1;
+    while (s->lanes < 512 && s->lanes * e < c) s->lanes *= 2;
+    if (s->lanes * e >= c) {
+      s->threads = s->lanes > 32 ? s->lanes : kBlock;
+      return true;
+    }
+  }
+  return false;
+}
+
+int grid_of(const Shape& s, int64_t n, int sms, int per_sm) {
+  const int64_t blocks = div_up64(n, s.threads / s.lanes);
+  return (int)std::min<int64_t>(blocks, (int64_t)sms * per_sm);
+}
+int backward_blocks_per_sm(const Shape& s) { return std::max(1, 512 / s.threads); }
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool params_aligned(const Params& p) {
+  for (int s = 0; s < kSums; ++s)
+    if (!aligned16(p.param[s])) return false;
+  return true;
+}
+
+int fill(const sph_norm* a, const char* who, Params* p) {
+#define SPH_CHECK_ARG_IN(cond, msg)                                             \
+  do {                                                                          \
+    if (!(cond)) { set_error("%s: %s", who, msg); return SPH_ERR_INVALID; }     \
+  } while (0)
+  SPH_CHECK_ARG_IN(a && a->n >= 0 && a->c > 0, "bad sizes");
+  SPH_CHECK_ARG_IN(a->dtype == SPH_F32 || a->dtype == SPH_F16 || a->dtype == SPH_BF16, "rows are fp32, fp16 or bf16");
+  SPH_CHECK_ARG_IN(a->n == 0 || a->residual, "null pointer");
+  SPH_CHECK_ARG_IN(a->block || (!a->gate && !a->param[0] && !a->param[1] && !a->param[2]), "a gate, a scale or a norm of no block");
+  SPH_CHECK_ARG_IN(a->param[0] || !a->param[1], "a bias without its weight");
+  SPH_CHECK_ARG_IN(a->param[3] || !a->param[4], "a bias without its weight");
+  SPH_CHECK_ARG_IN(a->eps >= 0.f, "eps must not be negative or NaN");
+  if (a->c > SPH_NORM_MAX_CHANNELS) {
+    set_error("%s: %d channels, at most %d are supported", who, a->c, SPH_NORM_MAX_CHANNELS);
+    return SPH_ERR_LIMIT;
+  }
+  for (int s = 0; s < kSums; ++s) {
+    SPH_CHECK_ARG_IN(!a->param[s] || a->param_dtype[s] == SPH_F32 || a->param_dtype[s] == SPH_F16 || a->param_dtype[s] == SPH_BF16,
+                     "parameters are fp32, fp16 or bf16");
+    p->param[s] = a->param[s];
+    p->param_dtype[s] = a->param_dtype[s];
+  }
+#undef SPH_CHECK_ARG_IN
+  p->block = a->block; p->residual = a->residual; p->gate = a->gate;
+  p->gate_row = a->gate && a->gate_per_row;
+  p->n = a->n; p->c = a->c; p->eps = a->eps;
+  return SPH_OK;
+}
+
+template <typename T, int VEC, int NV>
+void start(bool backward, bool center, int grid, const Shape& s, cudaStream_t st, const Params& p) {
+  const size_t smem = backward && s.threads > s.lanes ? (size_t)kBlock * VEC * NV * sizeof(float) : 0;
+  if (backward) {
+    if (center) launch(backward_kernel<T, VEC, NV, true>, grid, s.threads, smem, st, p);
+    else launch(backward_kernel<T, VEC, NV, false>, grid, s.threads, smem, st, p);
+  } else {
+    if (center) launch(forward_kernel<T, VEC, NV, true>, grid, s.threads, 0, st, p);
+    else launch(forward_kernel<T, VEC, NV, false>, grid, s.threads, 0, st, p);
+  }
+}
+template <typename T>
+void start(bool backward, bool center, int grid, const Shape& s, cudaStream_t st, const Params& p) {
+  constexpr int V = Row<T>::kVec;
+  const bool wide = s.vec * s.nv == 16;
+  if (s.vec == 1) {
+    if (wide) start<T, 1, 16>(backward, center, grid, s, st, p);
+    else start<T, 1, 8>(backward, center, grid, s, st, p);
+  } else {
+    if (wide) start<T, V, 16 / V>(backward, center, grid, s, st, p);
+    else start<T, V, 8 / V>(backward, center, grid, s, st, p);
+  }
+}
+int start(int dtype, bool backward, bool center, int grid, const Shape& s, cudaStream_t st, Params& p) {
+  p.lanes = s.lanes;
+  if (dtype == SPH_F32) start<float>(backward, center, grid, s, st, p);
+  else if (dtype == SPH_F16) start<__half>(backward, center, grid, s, st, p);
+  else start<__nv_bfloat16>(backward, center, grid, s, st, p);
+  SPH_LAUNCH_CHECK();
+  return SPH_OK;
+}
+
+}  // namespace
+
+}  // namespace sph
+
+using namespace sph;
+
+extern "C" int sph_residual_norm(const sph_norm* a, void* d_out, void* d_normed, float* d_stats, void* stream) {
+  Params p = {};
+  const int rc = fill(a, __func__, &p);
+  if (rc != SPH_OK) return rc;
+  if (a->n == 0) return SPH_OK;
+  SPH_CHECK_ARG(!!d_out == !!a->block, "out belongs to a block");
+  SPH_CHECK_ARG(!!d_normed == !!a->param[3], "normed belongs to a next_weight");
+  SPH_CHECK_ARG(aligned16(d_stats), "the statistics must be 16-byte aligned");
+  p.out = d_out; p.normed = d_normed; p.stats = d_stats;
+  const int sms = current_sm_count();
+  if (sms <= 0) return SPH_ERR_CUDA;
+  const int e = dtype_bytes(a->dtype);
+  const bool whole = (int64_t)a->c * e % 16 == 0 && aligned16(a->block) && aligned16(a->residual) &&
+                     (p.gate_row || aligned16(a->gate)) && aligned16(d_out) && aligned16(d_normed) && params_aligned(p);
+  Shape s;
+  if (!shape_of(a->c, e, whole, &s)) { set_error("%s: too many channels", __func__); return SPH_ERR_LIMIT; }
+  return start(a->dtype, false, a->center != 0, grid_of(s, a->n, sms, 2048 / s.threads), s, (cudaStream_t)stream, p);
+}
+
+extern "C" int64_t sph_residual_norm_scratch_bytes(int64_t n, int32_t c) {
+  if (n < 0 || c <= 0) { set_error("%s: bad sizes", __func__); return SPH_ERR_INVALID; }
+  const int sms = current_sm_count();
+  if (sms <= 0) return SPH_ERR_CUDA;
+  Shape s;                                    // how many threads a row has goes by its channels alone
+  if (!shape_of(c, 4, false, &s)) { set_error("%s: %d channels, at most %d are supported", __func__, c, SPH_NORM_MAX_CHANNELS); return SPH_ERR_LIMIT; }
+  return std::max<int64_t>(1, grid_of(s, n, sms, backward_blocks_per_sm(s))) * kSums * c * (int64_t)sizeof(float);
+}
+
+extern "C" int sph_residual_norm_backward(const sph_norm* a, const void* d_dout, const void* d_dnormed, const float* d_stats,
+                                          void* d_scratch, void* d_dblock, void* d_dresidual, void* d_dgate, void* const d_dparam[5],
+                                          void* stream) {
+  Params p = {};
+  const int rc = fill(a, __func__, &p);
+  if (rc != SPH_OK) return rc;
+  SPH_CHECK_ARG(d_dparam, "null pointer");
+  SPH_CHECK_ARG(!d_dnormed || a->param[3], "a gradient of normed without a next_weight");
+  SPH_CHECK_ARG(!d_dout || a->block, "a gradient of out without a block");
+  SPH_CHECK_ARG(a->n == 0 || (d_stats && aligned16(d_stats)), "the statistics must be given, 16-byte aligned");
+  SPH_CHECK_ARG(d_scratch, "null scratch");
+  for (int s = 0; s < kSums; ++s) SPH_CHECK_ARG(a->param[s] || !d_dparam[s], "a gradient of a parameter that there is not");
+  p.d_out = d_dout; p.d_normed = d_dnormed;
+  p.d_block = d_dblock; p.d_residual = d_dresidual; p.d_gate = d_dgate;
+  p.stats = const_cast<float*>(d_stats);
+  p.partial = (float*)d_scratch;
+  const int sms = current_sm_count();
+  if (sms <= 0) return SPH_ERR_CUDA;
+  const int e = dtype_bytes(a->dtype);
+  const bool whole = (int64_t)a->c * e % 16 == 0 && aligned16(a->block) && aligned16(a->residual) &&
+                     (p.gate_row || (aligned16(a->gate) && aligned16(d_dgate))) && aligned16(d_dout) && aligned16(d_dnormed) &&
+                     aligned16(d_dblock) && aligned16(d_dresidual) && params_aligned(p);
+  Shape s;
+  if (!shape_of(a->c, e, whole, &s)) { set_error("%s: too many channels", __func__); return SPH_ERR_LIMIT; }
+  SumParams q = {};
+  q.partial = p.partial;
+  q.c = a->c;
+  if (a->n > 0) {
+    q.blocks = grid_of(s, a->n, sms, backward_blocks_per_sm(s));
+    const int done = start(a->dtype, true, a->center != 0, q.blocks, s, (cudaStream_t)stream, p);
+    if (done != SPH_OK) return done;
+  }
+  bool any = false;
+  for (int i = 0; i < kSums; ++i) {
+    q.to[i] = d_dparam[i];
+    q.dtype[i] = a->param_dtype[i];
+    any |= d_dparam[i] != nullptr;
+  }
+  if (any) {
+    launch(sums_kernel, dim3(div_up(a->c, 32), kSums), 256, 0, (cudaStream_t)stream, q);
+    SPH_LAUNCH_CHECK();
+  }
+  return SPH_OK;
+}

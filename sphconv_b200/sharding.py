@@ -3,7 +3,8 @@ shared across the batch only as a list index, row ids and z_ptr are per-tensor p
 src/sphconv/rules.cu:72-80,204-227), so rank r of R takes a contiguous slice of the batch, builds its own
 SparseConvTensor (its z_ptr starts at 0) and runs the path locally.  Forward needs no collective; training
 adds ONE all-reduce over a flat fp32 buffer holding every layer's weight gradient."""
-from typing import Iterable, List, Tuple
+import math
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -75,13 +76,25 @@ class GradBuffer:
                 v.add_(p.grad.float())
                 p.grad = None
 
-    def to_grads(self) -> None:
-        """`.grad` of every parameter = its slice, rounded once to the parameter's dtype."""
+    def to_grads(self, max_norm: Optional[float] = None, norm_type: float = 2.0) -> Optional[torch.Tensor]:
+        """`.grad` of every parameter = its slice, rounded once to the parameter's dtype.  With `max_norm` the gradients are
+        clipped on the way (the buffer itself stays as it is), and their norm before that is returned: after all_reduce it is the
+        norm over all ranks, the same on each."""
+        if max_norm is not None:
+            with torch.no_grad():
+                for p in self.params:
+                    if p.grad is None or p.grad.dtype != p.dtype or not p.grad.is_contiguous():
+                        p.grad = torch.empty_like(p, memory_format=torch.contiguous_format)
+                return clip_gradients(self.views, max_norm, out=[p.grad for p in self.params], norm_type=norm_type)
         for p, v in zip(self.params, self.views):
             if p.grad is None or p.grad.dtype != p.dtype:
                 p.grad = v.to(p.dtype)
             else:
                 p.grad.copy_(v)
+
+    def norm(self, norm_type: float = 2.0) -> torch.Tensor:
+        """Norm over all gradients in the buffer (a float32 scalar on its device)."""
+        return grad_norm([self.flat], norm_type)
 
     def detach(self) -> None:
         for p in self.params:
@@ -125,3 +138,58 @@ def allreduce_gradients(params: Iterable[torch.nn.Parameter], group=None, averag
             flat /= dist.get_world_size(group)
     unflatten_grads(flat, plist)
     return int(flat.numel())
+
+
+def _largest(norm_type: float) -> bool:
+    if norm_type not in (2.0, math.inf):
+        raise ValueError("the norm is 2 or inf, got %r" % (norm_type,))
+    return norm_type == math.inf
+
+
+@torch.no_grad()
+def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
+    """sqrt(sum g^2) over every value of every tensor (norm_type 2), or max |g| (inf; NaN if any is): a float32 scalar on their
+    device, nothing is read back.  float32, float16 and bfloat16 tensors, mixed; sums are held in 64 bits, in a fixed order."""
+    largest, grads = _largest(norm_type), list(grads)
+    if grads and grads[0].is_cuda:
+        from . import _capi
+        return _capi.host().grad_clip(grads, None, None, largest)
+    if not grads:
+        return torch.zeros(())
+    if largest:
+        return torch.stack([g.abs().max().float() if g.numel() else torch.zeros(()) for g in grads]).max()
+    return torch.stack([g.double().square().sum() for g in grads]).sum().sqrt().float()
+
+
+@torch.no_grad()
+def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None,
+                   norm_type: float = 2.0) -> torch.Tensor:
+    """Every gradient times min(1, max_norm / (norm + 1e-6)), in place or into `out` (tensors of the same shapes, of any of the
+    dtypes: rounded once); returns the norm before clipping.  A norm that is not finite makes the gradients so, as in
+    torch.nn.utils.clip_grad_norm_.  A tensor that is listed twice, or that overlaps another one or a destination, is refused."""
+    largest, grads = _largest(norm_type), list(grads)
+    if not max_norm >= 0:
+        raise ValueError("max_norm must not be negative")
+    out = None if out is None else list(out)
+    if out is not None and len(out) != len(grads):
+        raise ValueError("as many destinations as gradients are needed")
+    if grads and grads[0].is_cuda:
+        from . import _capi
+        return _capi.host().grad_clip(grads, out, float(max_norm), largest)
+    if len({g.data_ptr() for g in grads if g.numel()}) < sum(g.numel() > 0 for g in grads):
+        raise RuntimeError("a gradient is in the list twice")
+    norm = grad_norm(grads, norm_type)
+    by = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
+    for g, o in zip(grads, grads if out is None else out):
+        o.copy_(g.float() * by)
+    return norm
+
+
+def clip_grad_norm_(params: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
+    """Clips the `.grad`s of `params` in place by their global norm, and returns it; parameters without a gradient are passed
+    over, one given twice counts once.  For a model whose gradients are in a GradBuffer: `GradBuffer.to_grads(max_norm)`."""
+    params = [params] if isinstance(params, torch.Tensor) else params
+    grads = {id(p): p.grad for p in params if p.grad is not None}
+    if not grads:
+        return torch.zeros(())
+    return clip_gradients(list(grads.values()), max_norm, norm_type=norm_type)
