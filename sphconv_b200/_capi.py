@@ -45,6 +45,13 @@ class Norm(ctypes.Structure):
                 ("block", vp), ("residual", vp), ("gate", vp), ("param", vp * 5), ("param_dtype", i32 * 5)]
 
 
+class Attention(ctypes.Structure):
+    """struct sph_attention"""
+    _fields_ = [("B", i32), ("q_heads", i32), ("k_heads", i32), ("channels", i32), ("dtype", i32), ("scale", ctypes.c_float),
+                ("n_q", i64), ("n_k", i64), ("q", vp), ("k", vp), ("v", vp), ("q_row", i64), ("q_head", i64), ("k_row", i64),
+                ("k_head", i64), ("v_row", i64), ("v_head", i64), ("q_ptr", vp), ("k_ptr", vp), ("key_mask", vp)]
+
+
 class ClipTensor(ctypes.Structure):
     """struct sph_clip_tensor"""
     _fields_ = [("src", vp), ("dst", vp), ("n", i64), ("src_dtype", i32), ("dst_dtype", i32)]
@@ -91,6 +98,9 @@ SIGNATURES = {
     "sph_residual_norm": (cint, [ctypes.POINTER(Norm), vp, vp, vp, vp]),
     "sph_residual_norm_scratch_bytes": (i64, [i64, i32]),
     "sph_residual_norm_backward": (cint, [ctypes.POINTER(Norm), vp, vp, vp, vp, vp, vp, vp, ctypes.POINTER(vp), vp]),
+    "sph_attention_scratch_bytes": (i64, [ctypes.POINTER(Attention), cint]),
+    "sph_attention_forward": (cint, [ctypes.POINTER(Attention), vp, vp, vp, vp, vp]),
+    "sph_attention_backward": (cint, [ctypes.POINTER(Attention), vp, vp, vp, vp, vp, vp, vp, vp]),
     "sph_grad_norm_scratch_bytes": (i64, [i32]),
     "sph_grad_norm": (cint, [ctypes.POINTER(ClipTensor), i32, cint, vp, vp, vp]),
     "sph_grad_clip": (cint, [ctypes.POINTER(ClipTensor), i32, cint, ctypes.c_float, vp, vp, vp]),

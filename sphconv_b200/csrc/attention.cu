@@ -1,0 +1,639 @@
+// Cross attention of queries to the rows of their scan: the kernels on the CUDA cores, for float32 and for rows that the tensor-core
+// kernels do not take, the sums over parts that both kinds leave, and the entry points.
+//
+//   S = scale Q K^T, masked keys -inf;  P = softmax of its rows;  O = P V
+//   delta = rowsum(dO O);  dP = dO V^T;  dS = P (dP - delta);  dQ = scale dS K;  dK = scale dS^T Q;  dV = P^T dO
+//
+// A block has a tile of 64 rows and walks the other side in tiles of 64: forward with the running maximum and sum of a softmax, backward
+// with the logarithm of the sum from the forward pass, once for queries (dQ) and once for keys (dK and dV), so that nothing is added
+// atomically and results are the same every time.  256 threads hold 4 x 4 scores each.  The longer side is split over blocks where
+// the tiles do not fill the GPU; each leaves its part in float32, and a launch more joins them in their order.
+//
+// Rows that are no keys are read as zeros: what they hold does not matter, NaN included.  A query without keys has zeros.
+#include <algorithm>
+
+#include "attention.cuh"
+
+namespace sph {
+
+namespace attn {
+
+constexpr int kTile = 64;
+constexpr int kThreads = 256;
+constexpr int kScorePitch = kTile + 4;
+
+template <typename T> __device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float(float v) { return v; }
+template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+
+// 64 rows of d elements to shared memory as float32, zeros where there is no row (row(r) is null) and behind d.
+template <typename T, int DP, typename Row>
+__device__ __forceinline__ void load_tile(float* to, int d, int vec, Row row) {
+  constexpr int PITCH = DP + 4;
+  constexpr int E = 16 / sizeof(T);
+  if (vec) {
+    for (int i = threadIdx.x; i < kTile * (DP / E); i += kThreads) {
+      const int r = i / (DP / E), c = i % (DP / E) * E;
+      const T* src = row(r);
+      struct __align__(16) Piece { T v[E]; } piece;
+      const bool some = src != nullptr && c < d;
+      if (some) piece = *(const Piece*)(src + c);
+#pragma unroll
+      for (int j = 0; j < E; j += 4)
+        *(float4*)(to + r * PITCH + c + j) = some ? make_float4(to_float(piece.v[j]), to_float(piece.v[j + 1]), to_float(piece.v[j + 2]),
+                                                                to_float(piece.v[j + 3]))
+                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  } else {
+    for (int i = threadIdx.x; i < kTile * DP; i += kThreads) {
+      const int r = i / DP, c = i % DP;
+      const T* src = row(r);
+      to[r * PITCH + c] = src != nullptr && c < d ? to_float(src[c]) : 0.f;
+    }
+  }
+}
+
+// s[i][j] = a[4 ty + i] . b[tx + 16 j]
+template <int DP>
+__device__ __forceinline__ void scores(float (&s)[4][4], const float* a, const float* b, int d, int tx, int ty) {
+  constexpr int PITCH = DP + 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < d; c += 4) {            // zeros up to a multiple of 4
+    float4 x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *(const float4*)(a + (4 * ty + i) * PITCH + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = *(const float4*)(b + (tx + 16 * j) * PITCH + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        s[i][j] = fmaf(x[i].x, y[j].x, fmaf(x[i].y, y[j].y, fmaf(x[i].z, y[j].z, fmaf(x[i].w, y[j].w, s[i][j]))));
+  }
+}
+
+// A thread's channels of a row: pieces of W consecutive ones, piece j at 16 W j + W tx.
+template <int DP>
+struct Columns {
+  static constexpr int W = DP >= 64 ? 4 : 2, N = DP / 16 / W;
+};
+
+// acc[i] += sum over n of p[4 ty + i][n] * v[n]
+template <int DP>
+__device__ __forceinline__ void accumulate(float (&acc)[4][DP / 16], const float* p, const float* v, int tx, int ty) {
+  constexpr int PITCH = DP + 4, W = Columns<DP>::W, N = Columns<DP>::N;
+#pragma unroll 2
+  for (int n = 0; n < kTile; n += 4) {
+    float x[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 f = *(const float4*)(p + (4 * ty + i) * kScorePitch + n);
+      x[i][0] = f.x; x[i][1] = f.y; x[i][2] = f.z; x[i][3] = f.w;
+    }
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        float y[W];
+        const float* from = v + (n + m) * PITCH + 16 * W * j + W * tx;
+        if (W == 4) {
+          const float4 f = *(const float4*)from;
+          y[0] = f.x; y[1] = f.y; y[2 % W] = f.z; y[3 % W] = f.w;
+        } else {
+          const float2 f = *(const float2*)from;
+          y[0] = f.x; y[1] = f.y;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int w = 0; w < W; ++w) acc[i][j * W + w] = fmaf(x[i][m], y[w], acc[i][j * W + w]);
+      }
+  }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(const float (&acc)[DP / 16], float by, T* to, int d, int tx) {
+  constexpr int W = Columns<DP>::W, N = Columns<DP>::N;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const int c = 16 * W * j + W * tx + w;
+      if (c < d) to[c] = from_float<T>(acc[j * W + w] * by);
+    }
+}
+
+// Work of a block: items of tiles, key heads, parts.
+struct Place {
+  int item, head, split;
+};
+__device__ __forceinline__ Place place_of(const Params& p) {
+  Place r;
+  r.split = blockIdx.x % p.splits;
+  const int i = blockIdx.x / p.splits;
+  r.head = i % p.hkv;
+  r.item = i / p.hkv;
+  return r;
+}
+
+template <bool QUERIES>
+__device__ __forceinline__ Work block_work(const Params& p, int item) {
+  __shared__ Work s_work;
+  if (threadIdx.x < 32) {
+    const Work w = find_work<QUERIES>(p, item, kTile);
+    if (threadIdx.x == 0) s_work = w;
+  }
+  __syncthreads();
+  return s_work;
+}
+
+// Scans that are not in order, or not within the rows, are reported.
+__device__ __forceinline__ void check_scans(const Params& p) {
+  if (blockIdx.x != 0 || p.status == nullptr) return;
+  bool bad = false;
+  for (int b = threadIdx.x; b <= p.B; b += blockDim.x) {
+    const int q = __ldg(p.q_ptr + b), k = __ldg(p.k_ptr + b);
+    bad |= q < 0 || q > p.n_q || k < 0 || k > p.n_k;
+    if (b < p.B) bad |= q > __ldg(p.q_ptr + b + 1) || k > __ldg(p.k_ptr + b + 1);
+  }
+  if (bad) atomicOr(p.status, SPH_STATUS_BAD_INDEX);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Params p) {
+  constexpr int PITCH = DP + 4;
+  extern __shared__ __align__(16) float smem[];
+  float *s_q = smem, *s_k = s_q + kTile * PITCH, *s_v = s_k + kTile * PITCH, *s_p = s_v + kTile * PITCH;
+  __shared__ uint8_t s_key[kTile];
+  after_previous();
+  check_scans(p);
+  const Place at = place_of(p);
+  const Work w = block_work<true>(p, at.item);
+  if (w.scan < 0) return;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int rows = min(kTile, w.nq * p.group - w.tile * kTile);       // of the tile
+  auto query = [&](int r, int* head) {
+    const int i = w.tile * kTile + r;
+    *head = at.head * p.group + i % p.group;
+    return w.q0 + i / p.group;
+  };
+  load_tile<T, DP>(s_q, p.d, p.vec, [&](int r) -> const T* {
+    int h;
+    const int64_t q = query(min(r, rows - 1), &h);
+    return r < rows ? (const T*)p.q + q * p.q_row + h * p.q_head : nullptr;
+  });
+  const int2 keys = split_rows(w.nk, at.split, p.splits, kTile);
+  float o[4][DP / 16], top[4], sum[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    top[i] = -INFINITY;
+    sum[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < DP / 16; ++j) o[i][j] = 0.f;
+  }
+  for (int k0 = keys.x; k0 < keys.y; k0 += kTile) {
+    __syncthreads();
+    if (threadIdx.x < kTile) {
+      const int k = k0 + threadIdx.x;
+      s_key[threadIdx.x] = k < keys.y && (p.mask == nullptr || p.mask[w.k0 + k] != 0);
+    }
+    __syncthreads();
+    load_tile<T, DP>(s_k, p.d, p.vec, [&](int r) -> const T* {
+      return s_key[r] ? (const T*)p.k + (int64_t)(w.k0 + k0 + r) * p.k_row + at.head * p.k_head : nullptr;
+    });
+    load_tile<T, DP>(s_v, p.d, p.vec, [&](int r) -> const T* {
+      return s_key[r] ? (const T*)p.v + (int64_t)(w.k0 + k0 + r) * p.v_row + at.head * p.v_head : nullptr;
+    });
+    __syncthreads();
+    float s[4][4];
+    scores<DP>(s, s_q, s_k, p.d, tx, ty);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float most = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = s_key[tx + 16 * j] ? s[i][j] * p.scale_log2 : -INFINITY;
+        most = fmaxf(most, s[i][j]);
+      }
+#pragma unroll
+      for (int of = 8; of > 0; of >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, of));
+      const float now = fmaxf(top[i], most);
+      const float base = now == -INFINITY ? 0.f : now;                // nothing yet: every 2^(-inf - 0) is zero
+      const float by = exp2f(top[i] - base);
+      top[i] = now;
+      float add = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = exp2f(s[i][j] - base);
+        add += s[i][j];
+        s_p[(4 * ty + i) * kScorePitch + tx + 16 * j] = s[i][j];
+      }
+      sum[i] = sum[i] * by + add;                                     // of this thread's columns; joined at the end
+#pragma unroll
+      for (int j = 0; j < DP / 16; ++j) o[i][j] *= by;
+    }
+    __syncwarp();                                                     // a row of P belongs to half a warp
+    accumulate<DP>(o, s_p, s_v, tx, ty);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int of = 8; of > 0; of >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], of);
+    const int r = 4 * ty + i;
+    if (r >= rows) continue;
+    int h;
+    const int64_t q = query(r, &h);
+    const bool none = sum[i] == 0.f;
+    const float by = none ? 0.f : 1.f / sum[i], lse = none ? INFINITY : top[i] + log2f(sum[i]);
+    if (p.splits > 1) {
+      store_row<float, DP>(o[i], by, p.part + (((int64_t)at.split * p.n_q + q) * p.hq + h) * p.d, p.d, tx);
+      if (tx == 0) p.part_lse[((int64_t)at.split * p.n_q + q) * p.hq + h] = lse;
+    } else {
+      store_row<T, DP>(o[i], by, (T*)p.out + (q * p.hq + h) * p.d, p.d, tx);
+      if (tx == 0 && p.lse) p.lse[q * p.hq + h] = lse;
+    }
+  }
+}
+
+// KEYS: a tile of keys against all queries of the scan (dK, dV); else a tile of queries against its keys (dQ).
+template <typename T, int DP, bool KEYS>
+__global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constant__ Params p) {
+  constexpr int PITCH = DP + 4;
+  extern __shared__ __align__(16) float smem[];
+  float *s_r1 = smem, *s_r2 = s_r1 + kTile * PITCH;                   // rows: K and V, or Q and dO
+  float *s_c1 = s_r2 + kTile * PITCH, *s_c2 = s_c1 + kTile * PITCH;   // columns: Q and dO, or K and V
+  float *s_ds = s_c2 + kTile * PITCH, *s_p = s_ds + kTile * kScorePitch;
+  __shared__ float s_lse[kTile], s_delta[kTile];
+  __shared__ uint8_t s_key[kTile];
+  after_previous();
+  const Place at = place_of(p);
+  const Work w = block_work<!KEYS>(p, at.item);
+  if (w.scan < 0) return;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int all = w.nq * p.group;
+  auto query = [&](int i, int* head) {                                // row i of the scan's queries
+    *head = at.head * p.group + i % p.group;
+    return (int64_t)w.q0 + i / p.group;
+  };
+  auto load_queries = [&](float* q_to, float* d_to, int first, int n) {
+    load_tile<T, DP>(q_to, p.d, p.vec, [&](int r) -> const T* {
+      if (r >= n) return nullptr;
+      int h;
+      const int64_t q = query(first + r, &h);
+      return (const T*)p.q + q * p.q_row + h * p.q_head;
+    });
+    load_tile<T, DP>(d_to, p.d, p.vec, [&](int r) -> const T* {
+      if (r >= n) return nullptr;
+      int h;
+      const int64_t q = query(first + r, &h);
+      return (const T*)p.d_out + (q * p.hq + h) * p.d;
+    });
+    if (threadIdx.x < kTile) {
+      float lse = INFINITY, delta = 0.f;
+      if ((int)threadIdx.x < n) {
+        int h;
+        const int64_t q = query(first + threadIdx.x, &h);
+        lse = p.lse[q * p.hq + h];
+        delta = p.delta[q * p.hq + h];
+      }
+      s_lse[threadIdx.x] = lse;
+      s_delta[threadIdx.x] = delta;
+    }
+  };
+  auto load_keys = [&](float* k_to, float* v_to, int first, int n) {  // between two barriers of their own
+    if (threadIdx.x < kTile)
+      s_key[threadIdx.x] = (int)threadIdx.x < n && (p.mask == nullptr || p.mask[w.k0 + first + threadIdx.x] != 0);
+    __syncthreads();
+    load_tile<T, DP>(k_to, p.d, p.vec, [&](int r) -> const T* {
+      return s_key[r] ? (const T*)p.k + (int64_t)(w.k0 + first + r) * p.k_row + at.head * p.k_head : nullptr;
+    });
+    load_tile<T, DP>(v_to, p.d, p.vec, [&](int r) -> const T* {
+      return s_key[r] ? (const T*)p.v + (int64_t)(w.k0 + first + r) * p.v_row + at.head * p.v_head : nullptr;
+    });
+  };
+  const int row0 = w.tile * kTile, rows = min(kTile, (KEYS ? w.nk : all) - row0);
+  if (KEYS) load_keys(s_r1, s_r2, row0, rows);
+  else load_queries(s_r1, s_r2, row0, rows);
+  const int2 span = split_rows(KEYS ? all : w.nk, at.split, p.splits, kTile);
+  float a1[4][DP / 16], a2[4][DP / 16];                               // dV ; dK or dQ
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < DP / 16; ++j) a1[i][j] = a2[i][j] = 0.f;
+  for (int c0 = span.x; c0 < span.y; c0 += kTile) {
+    __syncthreads();
+    if (KEYS) load_queries(s_c1, s_c2, c0, min(kTile, span.y - c0));
+    else load_keys(s_c1, s_c2, c0, min(kTile, span.y - c0));
+    __syncthreads();
+    float s[4][4], t[4][4];
+    scores<DP>(s, s_r1, s_c1, p.d, tx, ty);
+    scores<DP>(t, s_r2, s_c2, p.d, tx, ty);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * ty + i, c = tx + 16 * j, q = KEYS ? c : r, k = KEYS ? r : c;
+        const float x = s_key[k] ? exp2f(fmaf(s[i][j], p.scale_log2, -s_lse[q])) : 0.f;
+        if (KEYS) s_p[r * kScorePitch + c] = x;
+        s_ds[r * kScorePitch + c] = x * (t[i][j] - s_delta[q]);
+      }
+    __syncwarp();
+    if (KEYS) accumulate<DP>(a1, s_p, s_c2, tx, ty);
+    accumulate<DP>(a2, s_ds, s_c1, tx, ty);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 4 * ty + i;
+    if (r >= rows) continue;
+    int64_t at_row;                                                   // of [rows][heads]
+    if (KEYS) {
+      at_row = (int64_t)(w.k0 + row0 + r) * p.hkv + at.head;
+    } else {
+      int h;
+      const int64_t q = query(row0 + r, &h);
+      at_row = q * p.hq + h;
+    }
+    if (p.splits > 1) {
+      at_row += (int64_t)at.split * (KEYS ? (int64_t)p.n_k * p.hkv : (int64_t)p.n_q * p.hq);
+      store_row<float, DP>(a2[i], p.scale, p.part + at_row * p.d, p.d, tx);
+      if (KEYS) store_row<float, DP>(a1[i], 1.f, p.part2 + at_row * p.d, p.d, tx);
+    } else {
+      store_row<T, DP>(a2[i], p.scale, (T*)(KEYS ? p.dk : p.dq) + at_row * p.d, p.d, tx);
+      if (KEYS) store_row<T, DP>(a1[i], 1.f, (T*)p.dv + at_row * p.d, p.d, tx);
+    }
+  }
+}
+
+// delta of every row of every query head: a warp each
+template <typename T>
+__global__ void __launch_bounds__(kThreads) delta_kernel(const T* d_out, const T* out, float* delta, int64_t rows, int d) {
+  after_previous();
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * (kThreads / 32)) {
+    float s = 0.f;
+    for (int c = lane; c < d; c += 32) s = fmaf(to_float(d_out[r * d + c]), to_float(out[r * d + c]), s);
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) delta[r] = s;
+  }
+}
+
+// Parts of the forward pass: out = sum of 2^(lse_i - lse) part_i with lse = log2 of the sum of 2^lse_i; a warp a row.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_forward_kernel(const float* part, const float* part_lse, int splits, int64_t rows, int d,
+                                                                T* out, float* lse) {
+  after_previous();
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * (kThreads / 32)) {
+    float top = -INFINITY;
+    bool some = false;
+    for (int s = 0; s < splits; ++s) {
+      const float l = part_lse[(int64_t)s * rows + r];
+      if (l == INFINITY) continue;                                    // +inf: a part without keys
+      some = true;
+      top = l != l ? l : fmaxf(top, l);
+    }
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (int s = 0; s < splits; ++s) {
+      const float l = part_lse[(int64_t)s * rows + r];
+      if (l != INFINITY) sum += exp2f(l - base);
+    }
+    const float inv = some ? 1.f / sum : 0.f;
+    for (int c = lane; c < d; c += 32) {
+      float v = 0.f;
+      for (int s = 0; s < splits; ++s) {
+        const float l = part_lse[(int64_t)s * rows + r];
+        if (l != INFINITY) v = fmaf(exp2f(l - base) * inv, part[((int64_t)s * rows + r) * d + c], v);
+      }
+      out[r * d + c] = from_float<T>(v);
+    }
+    if (lane == 0 && lse) lse[r] = some ? base + log2f(sum) : INFINITY;
+  }
+}
+
+// Parts of a gradient, added in their order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_sum_kernel(const float* part, int splits, int64_t n, T* to) {
+  after_previous();
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+    float v = 0.f;
+    for (int s = 0; s < splits; ++s) v += part[(int64_t)s * n + i];
+    to[i] = from_float<T>(v);
+  }
+}
+
+namespace {
+
+int padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+int forward_smem(int dp) { return (3 * kTile * (dp + 4) + kTile * kScorePitch) * 4; }
+int backward_smem(int dp, bool keys) { return (4 * kTile * (dp + 4) + (keys ? 2 : 1) * kTile * kScorePitch) * 4; }
+
+// Parts that fill the GPU: as many as blocks are missing, none shorter than `least` rows on average.
+int splits_for(int64_t blocks, int64_t room, int64_t rows, int B, int64_t least) {
+  const int64_t mean = rows / std::max(B, 1);
+  const int64_t most = std::max<int64_t>(1, mean / least);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({room / std::max<int64_t>(blocks, 1), most, 64}));
+}
+
+struct Plan {
+  int fwd_splits, dq_splits, dkv_splits;
+  int fwd_blocks, dq_blocks, dkv_blocks;     // without the splits
+};
+Plan plan_of(const sph_attention& a, int sms) {
+  const int group = a.q_heads / a.k_heads, dp = padded(a.channels);
+  const int64_t room = 227 * 1024;
+  auto per_sm = [&](int smem) { return std::min<int64_t>(room / (smem + 1024), 4); };
+  Plan p;
+  const int64_t q_tiles = most_tiles(a.n_q * group, kTile, a.B), k_tiles = most_tiles(a.n_k, kTile, a.B);
+  p.fwd_blocks = p.dq_blocks = (int)(q_tiles * a.k_heads);
+  p.dkv_blocks = (int)(k_tiles * a.k_heads);
+  // tiles that there really are, if scans are of like length
+  const int64_t q_real = std::max<int64_t>(1, div_up64(a.n_q * group, (int64_t)kTile * a.B)) * a.B * a.k_heads;
+  const int64_t k_real = std::max<int64_t>(1, div_up64(a.n_k, (int64_t)kTile * a.B)) * a.B * a.k_heads;
+  p.fwd_splits = splits_for(q_real, sms * per_sm(forward_smem(dp)), a.n_k, a.B, 2 * kTile);
+  p.dq_splits = splits_for(q_real, sms * per_sm(backward_smem(dp, false)), a.n_k, a.B, 2 * kTile);
+  p.dkv_splits = splits_for(k_real, sms * per_sm(backward_smem(dp, true)), a.n_q * group, a.B, 2 * kTile);
+  return p;
+}
+
+template <typename K>
+int run_kernel(K* kernel, int blocks, int smem, cudaStream_t st, const Params& p) {
+  SPH_CUDA(allow_smem(kernel, 227 * 1024 - 2048));
+  launch(kernel, blocks, kThreads, smem, st, p);
+  SPH_LAUNCH_CHECK();
+  return SPH_OK;
+}
+
+template <typename T>
+int forward(const Params& p, int blocks, cudaStream_t st) {
+  const int dp = padded(p.d), smem = forward_smem(dp);
+  if (dp == 32) return run_kernel(forward_kernel<T, 32>, blocks, smem, st, p);
+  if (dp == 64) return run_kernel(forward_kernel<T, 64>, blocks, smem, st, p);
+  return run_kernel(forward_kernel<T, 128>, blocks, smem, st, p);
+}
+template <typename T, bool KEYS>
+int backward(const Params& p, int blocks, cudaStream_t st) {
+  const int dp = padded(p.d), smem = backward_smem(dp, KEYS);
+  if (dp == 32) return run_kernel(backward_kernel<T, 32, KEYS>, blocks, smem, st, p);
+  if (dp == 64) return run_kernel(backward_kernel<T, 64, KEYS>, blocks, smem, st, p);
+  return run_kernel(backward_kernel<T, 128, KEYS>, blocks, smem, st, p);
+}
+
+unsigned grid_for(int64_t items, int64_t per_block) { return (unsigned)std::min<int64_t>(div_up64(items, per_block), 148 * 16); }
+
+template <typename T>
+int run_forward(Params p, const Plan& plan, void* scratch, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.n_q * p.hq;
+  p.splits = plan.fwd_splits;
+  if (p.splits > 1) {
+    p.part = (float*)scratch;
+    p.part_lse = p.part + rows * p.d * p.splits;
+  }
+  const int rc = forward<T>(p, plan.fwd_blocks * p.splits, st);
+  if (rc != SPH_OK || p.splits == 1) return rc;
+  launch(join_forward_kernel<T>, grid_for(rows, kThreads / 32), kThreads, 0, st, p.part, p.part_lse, p.splits, rows, p.d, (T*)p.out, p.lse);
+  SPH_LAUNCH_CHECK();
+  return SPH_OK;
+}
+
+template <typename T>
+int run_backward(Params p, const Plan& plan, const void* out, void* scratch, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.n_q * p.hq, k_values = (int64_t)p.n_k * p.hkv * p.d;
+  float* delta = (float*)scratch;
+  float* part = delta + (rows + 3) / 4 * 4;
+  p.delta = delta;
+  if (rows) {
+    launch(delta_kernel<T>, grid_for(rows, kThreads / 32), kThreads, 0, st, (const T*)p.d_out, (const T*)out, delta, rows, p.d);
+    SPH_LAUNCH_CHECK();
+  }
+  if (p.dq && rows) {
+    p.splits = plan.dq_splits;
+    p.part = part;
+    int rc = backward<T, false>(p, plan.dq_blocks * p.splits, st);
+    if (rc != SPH_OK) return rc;
+    if (p.splits > 1) {
+      launch(join_sum_kernel<T>, grid_for(rows * p.d, kThreads), kThreads, 0, st, part, p.splits, rows * p.d, (T*)p.dq);
+      SPH_LAUNCH_CHECK();
+    }
+  }
+  if ((p.dk || p.dv) && k_values) {
+    p.splits = plan.dkv_splits;
+    p.part = part;
+    p.part2 = part + k_values * p.splits;
+    int rc = backward<T, true>(p, plan.dkv_blocks * p.splits, st);
+    if (rc != SPH_OK) return rc;
+    if (p.splits > 1) {
+      launch(join_sum_kernel<T>, grid_for(k_values, kThreads), kThreads, 0, st, p.part, p.splits, k_values, (T*)p.dk);
+      SPH_LAUNCH_CHECK();
+      launch(join_sum_kernel<T>, grid_for(k_values, kThreads), kThreads, 0, st, p.part2, p.splits, k_values, (T*)p.dv);
+      SPH_LAUNCH_CHECK();
+    }
+  }
+  return SPH_OK;
+}
+
+bool aligned(const void* p, int64_t row, int64_t head, int esize) {
+  return ((uintptr_t)p & 15) == 0 && row * esize % 16 == 0 && head * esize % 16 == 0;
+}
+
+int fill(const sph_attention* a, const char* who, Params* p) {
+  auto bad = [&](const char* what) { set_error("%s: %s", who, what); return SPH_ERR_INVALID; };
+  if (!a || a->B < 0 || a->n_q < 0 || a->n_k < 0 || a->q_heads < 1 || a->k_heads < 1 || a->channels < 1) return bad("bad sizes");
+  if (a->q_heads % a->k_heads != 0) return bad("query heads must be a multiple of key heads");
+  if (a->dtype != SPH_F32 && a->dtype != SPH_F16 && a->dtype != SPH_BF16) return bad("rows are fp32, fp16 or bf16");
+  if ((a->n_q > 0 && !a->q) || (a->n_k > 0 && (!a->k || !a->v)) || !a->q_ptr || !a->k_ptr) return bad("null pointer");
+  if (!(a->scale == a->scale)) return bad("the scale is NaN");
+  if (a->channels > SPH_ATTENTION_MAX_CHANNELS) {
+    set_error("%s: %d channels a head, at most %d are supported", who, a->channels, SPH_ATTENTION_MAX_CHANNELS);
+    return SPH_ERR_LIMIT;
+  }
+  // tiles and the rows of a scan (queries times heads) are numbered in 31 bits
+  const int64_t most = (int64_t)1 << 30;
+  if (a->n_k > most || a->n_q * (a->q_heads / a->k_heads) > most || (a->n_q * a->q_heads / kTile + (a->B + 2ll) * a->k_heads) * 64 > most ||
+      (a->n_k * a->k_heads / kTile + (a->B + 2ll) * a->k_heads) * 64 > most) {
+    set_error("%s: too many rows", who);
+    return SPH_ERR_LIMIT;
+  }
+  *p = Params{};
+  p->q = a->q; p->k = a->k; p->v = a->v;
+  p->q_row = a->q_row; p->q_head = a->q_head; p->k_row = a->k_row; p->k_head = a->k_head; p->v_row = a->v_row; p->v_head = a->v_head;
+  p->q_ptr = a->q_ptr; p->k_ptr = a->k_ptr; p->mask = a->key_mask;
+  p->n_q = (int)a->n_q; p->n_k = (int)a->n_k; p->B = a->B; p->hq = a->q_heads; p->hkv = a->k_heads; p->group = a->q_heads / a->k_heads;
+  p->d = a->channels;
+  p->scale = a->scale;
+  p->scale_log2 = a->scale * kLog2e;
+  const int e = dtype_bytes(a->dtype);
+  p->vec = (int64_t)p->d * e % 16 == 0 && aligned(p->q, p->q_row, p->q_head, e) && aligned(p->k, p->k_row, p->k_head, e) &&
+           aligned(p->v, p->v_row, p->v_head, e);
+  return SPH_OK;
+}
+
+}  // namespace
+}  // namespace attn
+
+}  // namespace sph
+
+using namespace sph;
+using namespace sph::attn;
+
+extern "C" int64_t sph_attention_scratch_bytes(const sph_attention* a, int backward) {
+  Params p;
+  const int rc = fill(a, __func__, &p);
+  if (rc != SPH_OK) return rc;
+  const int sms = current_sm_count();
+  if (sms <= 0) return SPH_ERR_CUDA;
+  const Plan plan = plan_of(*a, sms);
+  const int64_t rows = (int64_t)p.n_q * p.hq, k_values = (int64_t)p.n_k * p.hkv * p.d;
+  if (!backward) return plan.fwd_splits > 1 ? plan.fwd_splits * rows * (p.d + 1) * 4 : 0;
+  return ((rows + 3) / 4 * 4 + std::max(plan.dq_splits > 1 ? plan.dq_splits * rows * p.d : 0,
+                                         plan.dkv_splits > 1 ? 2 * plan.dkv_splits * k_values : 0)) * 4;
+}
+
+extern "C" int sph_attention_forward(const sph_attention* a, void* d_out, float* d_lse, void* d_scratch, int32_t* d_status, void* stream) {
+  Params p;
+  const int rc = fill(a, __func__, &p);
+  if (rc != SPH_OK) return rc;
+  if (a->n_q == 0) return SPH_OK;
+  SPH_CHECK_ARG(d_out, "null pointer");
+  const int sms = current_sm_count();
+  if (sms <= 0) return SPH_ERR_CUDA;
+  const Plan plan = plan_of(*a, sms);
+  SPH_CHECK_ARG(plan.fwd_splits == 1 || (d_scratch && (uintptr_t)d_scratch % 16 == 0), "the scratch must be 16-byte aligned");
+  p.out = d_out;
+  p.lse = d_lse;
+  p.status = d_status;
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (a->dtype == SPH_F32) return run_forward<float>(p, plan, d_scratch, st);
+  if (a->dtype == SPH_F16) return run_forward<__half>(p, plan, d_scratch, st);
+  return run_forward<__nv_bfloat16>(p, plan, d_scratch, st);
+}
+
+extern "C" int sph_attention_backward(const sph_attention* a, const void* d_dout, const void* d_out, const float* d_lse, void* d_scratch,
+                                      void* d_dq, void* d_dk, void* d_dv, void* stream) {
+  Params p;
+  const int rc = fill(a, __func__, &p);
+  if (rc != SPH_OK) return rc;
+  SPH_CHECK_ARG(a->n_q == 0 || (d_dout && d_out && d_lse), "null pointer");
+  SPH_CHECK_ARG(!!d_dk == !!d_dv, "the gradients of keys and values come together");
+  SPH_CHECK_ARG(d_scratch && (uintptr_t)d_scratch % 16 == 0, "the scratch must be 16-byte aligned");
+  const int sms = current_sm_count();
+  if (sms <= 0) return SPH_ERR_CUDA;
+  const Plan plan = plan_of(*a, sms);
+  p.d_out = d_dout;
+  p.lse = const_cast<float*>(d_lse);
+  p.dq = d_dq; p.dk = d_dk; p.dv = d_dv;
+  p.vec = p.vec && ((uintptr_t)d_dout & 15) == 0;
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (a->dtype == SPH_F32) return run_backward<float>(p, plan, d_out, d_scratch, st);
+  if (a->dtype == SPH_F16) return run_backward<__half>(p, plan, d_out, d_scratch, st);
+  return run_backward<__nv_bfloat16>(p, plan, d_out, d_scratch, st);
+}

@@ -34,7 +34,8 @@ using Ints = std::vector<int64_t>;
   X(sph_init_tensor_scratch_bytes) X(sph_init_tensor) X(sph_permute_rows) X(sph_dense_channels_first)                \
   X(sph_epilogue_backward) X(sph_voxel_transform) X(sph_voxel_feature_count) X(sph_voxelize_scratch_bytes)           \
   X(sph_voxelize_count) X(sph_voxelize_fill) X(sph_residual_norm) X(sph_residual_norm_scratch_bytes)                  \
-  X(sph_residual_norm_backward) X(sph_grad_norm_scratch_bytes) X(sph_grad_norm) X(sph_grad_clip)
+  X(sph_residual_norm_backward) X(sph_grad_norm_scratch_bytes) X(sph_grad_norm) X(sph_grad_clip)                    \
+  X(sph_attention_scratch_bytes) X(sph_attention_forward) X(sph_attention_backward)
 
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
@@ -715,6 +716,112 @@ py::tuple residual_norm(const optional<Tensor>& block, const Tensor& residual, c
   return py::make_tuple(or_none(out), or_none(normed));
 }
 
+struct AttentionInputs {
+  Tensor q, k, v, q_ptr, k_ptr;
+  optional<Tensor> mask;
+  double scale;
+
+  sph_attention args() const {
+    sph_attention a = {};
+    a.B = (int32_t)q_ptr.size(0) - 1;
+    a.q_heads = (int32_t)q.size(1);
+    a.k_heads = (int32_t)k.size(1);
+    a.channels = (int32_t)q.size(2);
+    a.dtype = dtype_code(q, "query");
+    a.scale = (float)scale;
+    a.n_q = q.size(0);
+    a.n_k = k.size(0);
+    a.q = ptr(q); a.k = ptr(k); a.v = ptr(v);
+    a.q_row = q.stride(0); a.q_head = q.stride(1);
+    a.k_row = k.stride(0); a.k_head = k.stride(1);
+    a.v_row = v.stride(0); a.v_head = v.stride(1);
+    a.q_ptr = ints(q_ptr); a.k_ptr = ints(k_ptr);
+    a.key_mask = static_cast<const uint8_t*>(ptr(mask));
+    return a;
+  }
+};
+
+AttentionInputs attention_inputs(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_ptr, const Tensor& k_ptr,
+                                 const optional<Tensor>& mask, double scale) {
+  for (const Tensor* t : {&q, &k, &v}) {
+    if (!t->is_cuda()) require_cuda(*t);
+    if (t->dim() != 3) fail("queries are [n, heads, channels], keys and values [m, key heads, channels]");
+    if (t->scalar_type() != q.scalar_type() || t->device() != q.device()) fail("queries, keys and values must have one dtype and device");
+  }
+  if (dtype_code(q, "query") == SPH_I8) fail("queries are float32, float16 or bfloat16");
+  if (k.sizes() != v.sizes()) fail("keys and values must have one shape");
+  if (q.size(2) != k.size(2) || q.size(2) < 1 || q.size(2) > SPH_ATTENTION_MAX_CHANNELS)
+    fail("heads of 1 to " + std::to_string(SPH_ATTENTION_MAX_CHANNELS) + " channels are needed, of queries as many as of keys");
+  if (k.size(1) < 1 || q.size(1) < 1 || q.size(1) % k.size(1) != 0) fail("query heads must be a multiple of key heads");
+  for (const Tensor* t : {&q_ptr, &k_ptr}) {
+    require_cuda(*t);
+    if (t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) < 2 || t->size(0) != q_ptr.size(0) || t->device() != q.device())
+      fail("q_ptr and k_ptr must be int32 [B+1] on the queries' device");
+  }
+  if (mask) {
+    require_cuda(*mask);
+    if (mask->scalar_type() != at::kBool || mask->dim() != 1 || mask->size(0) != k.size(0) || mask->device() != q.device())
+      fail("key_mask must be bool, one value a key, on the queries' device");
+  }
+  if (!(scale == scale)) fail("the scale is NaN");
+  // channels have to lie next to one another; rows and heads may lie anywhere
+  auto ready = [](const Tensor& t) { return t.size(2) == 1 || t.stride(2) == 1 ? t : t.contiguous(); };
+  return {ready(q), ready(k), ready(v), q_ptr, k_ptr, mask, scale};
+}
+
+// -> (out, lse or undefined)
+std::pair<Tensor, Tensor> attention_forward(const AttentionInputs& in, bool train) {
+  const c10::cuda::CUDAGuard guard(in.q.device());
+  const sph_attention a = in.args();
+  Tensor out = empty(in.q.sizes(), in.q.scalar_type(), in.q), lse;
+  if (train) lse = empty({a.n_q, a.q_heads}, at::kFloat, in.q);
+  const int64_t bytes = check(abi.sph_attention_scratch_bytes(&a, 0));
+  const Tensor scratch = bytes ? empty({bytes}, at::kByte, in.q) : Tensor();
+  check(abi.sph_attention_forward(&a, ptr(out), train ? static_cast<float*>(ptr(lse)) : nullptr, bytes ? ptr(scratch) : nullptr,
+                                  status_of(in.q), stream_of(in.q)));
+  return {out, lse};
+}
+
+struct AttentionLayer : public torch::autograd::Function<AttentionLayer> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_ptr,
+                        const Tensor& k_ptr, const optional<Tensor>& mask, double scale) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const auto [out, lse] = attention_forward(attention_inputs(q, k, v, q_ptr, k_ptr, mask, scale), true);
+    ctx->save_for_backward({q, k, v, q_ptr, k_ptr, mask.value_or(Tensor()), out, lse});
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    once_differentiable("cross_attention");
+    const auto saved = ctx->get_saved_variables();
+    const AttentionInputs in = attention_inputs(saved[0], saved[1], saved[2], saved[3], saved[4],
+                                                saved[5].defined() ? optional<Tensor>(saved[5]) : std::nullopt,
+                                                ctx->saved_data["scale"].toDouble());
+    const c10::cuda::CUDAGuard guard(in.q.device());
+    const Tensor d_out = grads[0].to(in.q.scalar_type()).contiguous();
+    Tensor dq, dk, dv;
+    if (ctx->needs_input_grad(0)) dq = empty(in.q.sizes(), in.q.scalar_type(), in.q);
+    if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
+      dk = empty(in.k.sizes(), in.k.scalar_type(), in.k);
+      dv = empty(in.v.sizes(), in.v.scalar_type(), in.v);
+    }
+    const sph_attention a = in.args();
+    const Tensor scratch = empty({std::max<int64_t>(16, check(abi.sph_attention_scratch_bytes(&a, 1)))}, at::kByte, in.q);
+    auto at_or_null = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    check(abi.sph_attention_backward(&a, ptr(d_out), ptr(saved[6]), static_cast<const float*>(ptr(saved[7])), ptr(scratch), at_or_null(dq),
+                                     at_or_null(dk), at_or_null(dv), stream_of(in.q)));
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_ptr, const Tensor& k_ptr,
+                       const optional<Tensor>& mask, double scale) {
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return AttentionLayer::apply(q, k, v, q_ptr, k_ptr, mask, scale);
+  return attention_forward(attention_inputs(q, k, v, q_ptr, k_ptr, mask, scale), false).first;
+}
+
 // Norm of many gradients (max_norm absent), or the norm with every gradient scaled into `out` (or where it is).
 Tensor grad_clip(const std::vector<Tensor>& grads, const optional<std::vector<Tensor>>& out, optional<double> max_norm, bool largest) {
   if (grads.empty()) fail("no gradients");
@@ -895,6 +1002,7 @@ PYBIND11_MODULE(sph_host, m) {
   m.def("epilogue_backward", &epilogue_backward);
   m.def("conv_layer", &conv_layer);
   m.def("residual_norm", &residual_norm);
+  m.def("cross_attention", &cross_attention);
   m.def("grad_clip", &grad_clip);
   m.def("init_tensor", &init_tensor);
   m.def("gather_rows", &gather_rows);
