@@ -11,6 +11,7 @@
 //
 // Rows that are no keys are read as zeros: what they hold does not matter, NaN included.  A query without keys has zeros.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.cuh"
 
@@ -431,7 +432,16 @@ __global__ void __launch_bounds__(kThreads) join_sum_kernel(const float* part, i
   }
 }
 
+int attention_forward_tc(const Params& p, bool bf16, int blocks, cudaStream_t st);      // attention_tc.cu
+
 namespace {
+
+// 16-bit rows in pieces of 16 bytes go to the tensor cores; there the largest score is found before it is scaled, so not with a
+// negative scale.
+bool on_tensor_cores(const sph_attention& a, const Params& p) {
+  return (a.dtype == SPH_F16 || a.dtype == SPH_BF16) && p.vec && p.scale >= 0.f;
+}
+constexpr int kTcTile = 128;
 
 int padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 int forward_smem(int dp) { return (3 * kTile * (dp + 4) + kTile * kScorePitch) * 4; }
@@ -448,7 +458,7 @@ struct Plan {
   int fwd_splits, dq_splits, dkv_splits;
   int fwd_blocks, dq_blocks, dkv_blocks;     // without the splits
 };
-Plan plan_of(const sph_attention& a, int sms) {
+Plan plan_of(const sph_attention& a, const Params& params, int sms) {
   const int group = a.q_heads / a.k_heads, dp = padded(a.channels);
   const int64_t room = 227 * 1024;
   auto per_sm = [&](int smem) { return std::min<int64_t>(room / (smem + 1024), 4); };
@@ -461,6 +471,11 @@ Plan plan_of(const sph_attention& a, int sms) {
   const int64_t k_real = std::max<int64_t>(1, div_up64(a.n_k, (int64_t)kTile * a.B)) * a.B * a.k_heads;
   p.fwd_splits = splits_for(q_real, sms * per_sm(forward_smem(dp)), a.n_k, a.B, 2 * kTile);
   p.dq_splits = splits_for(q_real, sms * per_sm(backward_smem(dp, false)), a.n_k, a.B, 2 * kTile);
+  if (on_tensor_cores(a, params)) {
+    p.fwd_blocks = most_tiles(a.n_q * group, kTcTile, a.B) * a.k_heads;
+    const int64_t real = std::max<int64_t>(1, div_up64(a.n_q * group, (int64_t)kTcTile * a.B)) * a.B * a.k_heads;
+    p.fwd_splits = splits_for(real, 2 * sms, a.n_k, a.B, 2 * kTcTile);
+  }
   p.dkv_splits = splits_for(k_real, sms * per_sm(backward_smem(dp, true)), a.n_q * group, a.B, 2 * kTile);
   return p;
 }
@@ -491,14 +506,15 @@ int backward(const Params& p, int blocks, cudaStream_t st) {
 unsigned grid_for(int64_t items, int64_t per_block) { return (unsigned)std::min<int64_t>(div_up64(items, per_block), 148 * 16); }
 
 template <typename T>
-int run_forward(Params p, const Plan& plan, void* scratch, cudaStream_t st) {
+int run_forward(Params p, const Plan& plan, bool tensor_cores, void* scratch, cudaStream_t st) {
   const int64_t rows = (int64_t)p.n_q * p.hq;
   p.splits = plan.fwd_splits;
   if (p.splits > 1) {
     p.part = (float*)scratch;
     p.part_lse = p.part + rows * p.d * p.splits;
   }
-  const int rc = forward<T>(p, plan.fwd_blocks * p.splits, st);
+  const int rc = tensor_cores ? attention_forward_tc(p, std::is_same<T, __nv_bfloat16>::value, plan.fwd_blocks * p.splits, st)
+                              : forward<T>(p, plan.fwd_blocks * p.splits, st);
   if (rc != SPH_OK || p.splits == 1) return rc;
   launch(join_forward_kernel<T>, grid_for(rows, kThreads / 32), kThreads, 0, st, p.part, p.part_lse, p.splits, rows, p.d, (T*)p.out, p.lse);
   SPH_LAUNCH_CHECK();
@@ -591,7 +607,7 @@ extern "C" int64_t sph_attention_scratch_bytes(const sph_attention* a, int backw
   if (rc != SPH_OK) return rc;
   const int sms = current_sm_count();
   if (sms <= 0) return SPH_ERR_CUDA;
-  const Plan plan = plan_of(*a, sms);
+  const Plan plan = plan_of(*a, p, sms);
   const int64_t rows = (int64_t)p.n_q * p.hq, k_values = (int64_t)p.n_k * p.hkv * p.d;
   if (!backward) return plan.fwd_splits > 1 ? plan.fwd_splits * rows * (p.d + 1) * 4 : 0;
   return ((rows + 3) / 4 * 4 + std::max(plan.dq_splits > 1 ? plan.dq_splits * rows * p.d : 0,
@@ -604,17 +620,19 @@ extern "C" int sph_attention_forward(const sph_attention* a, void* d_out, float*
   if (rc != SPH_OK) return rc;
   if (a->n_q == 0) return SPH_OK;
   SPH_CHECK_ARG(d_out, "null pointer");
+  SPH_CHECK_ARG(((uintptr_t)d_out & 15) == 0, "results must be 16-byte aligned");
   const int sms = current_sm_count();
   if (sms <= 0) return SPH_ERR_CUDA;
-  const Plan plan = plan_of(*a, sms);
+  const Plan plan = plan_of(*a, p, sms);
   SPH_CHECK_ARG(plan.fwd_splits == 1 || (d_scratch && (uintptr_t)d_scratch % 16 == 0), "the scratch must be 16-byte aligned");
   p.out = d_out;
   p.lse = d_lse;
   p.status = d_status;
   const cudaStream_t st = (cudaStream_t)stream;
-  if (a->dtype == SPH_F32) return run_forward<float>(p, plan, d_scratch, st);
-  if (a->dtype == SPH_F16) return run_forward<__half>(p, plan, d_scratch, st);
-  return run_forward<__nv_bfloat16>(p, plan, d_scratch, st);
+  const bool tc = on_tensor_cores(*a, p);
+  if (a->dtype == SPH_F32) return run_forward<float>(p, plan, tc, d_scratch, st);
+  if (a->dtype == SPH_F16) return run_forward<__half>(p, plan, tc, d_scratch, st);
+  return run_forward<__nv_bfloat16>(p, plan, tc, d_scratch, st);
 }
 
 extern "C" int sph_attention_backward(const sph_attention* a, const void* d_dout, const void* d_out, const float* d_lse, void* d_scratch,
@@ -627,7 +645,7 @@ extern "C" int sph_attention_backward(const sph_attention* a, const void* d_dout
   SPH_CHECK_ARG(d_scratch && (uintptr_t)d_scratch % 16 == 0, "the scratch must be 16-byte aligned");
   const int sms = current_sm_count();
   if (sms <= 0) return SPH_ERR_CUDA;
-  const Plan plan = plan_of(*a, sms);
+  const Plan plan = plan_of(*a, p, sms);
   p.d_out = d_dout;
   p.lse = const_cast<float*>(d_lse);
   p.dq = d_dq; p.dk = d_dk; p.dv = d_dv;

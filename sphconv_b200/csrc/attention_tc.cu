@@ -1,0 +1,314 @@
+// Cross attention on the Blackwell tensor cores (tcgen05), forward, for 16-bit rows of 8 to 128 channels in steps of 8.
+//
+//   S [128 x 128] = Q K^T   A = a tile of 128 query rows, B = 128 keys, both K-major in shared memory; S in TMEM
+//   P = 2^(scale log2 e S - top) in the rows' type, written over TMEM columns by the thread that has the row
+//   O [128 x d] += P V      A = P in TMEM, B = the same keys' values, MN-major in shared memory; O stays in TMEM
+//
+// A block has one tile of queries (heads that share a key head are rows of it) and walks a scan's keys, or a part of them.  Warps 0-3
+// do the softmax, a thread a row; warp 4 issues the MMAs; warps 5-7 copy keys and values with cp.async, which fills in zeros where
+// there is no key.  Two blocks share an SM, and one's softmax runs while the other's MMAs do.
+//   The running maximum follows S only when it has grown by more than 2^8: O is read, scaled and written again in those tiles alone,
+// P stays within 2^8 and a row's sum within float32.
+#include <algorithm>
+
+#include "attention_tc.cuh"
+
+namespace sph {
+namespace attn {
+
+namespace {
+
+constexpr int kN = 128;                       // keys of a tile
+constexpr int kSoftmaxWarps = 4, kMmaWarp = 4, kLoadWarp = 5, kLoadWarps = 3;
+constexpr int kThreadsTc = (kLoadWarp + kLoadWarps) * 32;
+constexpr int kLoaders = kLoadWarps * 32;
+constexpr float kSlack = 8.f;                 // log2 of how far a row's maximum may be above the one that P is taken against
+
+// DP: channels of a tile's rows in shared memory, 64 or 128.  128 channels of O leave no columns for P beside S: it lies in them.
+template <int DP>
+struct Shape {
+  static constexpr int kStages = DP == 64 ? 2 : 1;
+  static constexpr uint32_t kTileBytes = (DP / 64) * kM * 128u;
+  static constexpr bool kOverS = DP == 128;
+  static constexpr uint32_t kColS = 0, kColP = kOverS ? 0 : 128, kColO = kOverS ? 128 : 192, kCols = 256;
+  static constexpr int kSmem = 1024 + (1 + 2 * kStages) * (int)kTileBytes;
+};
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(kThreadsTc, 2) forward_tc_kernel(const __grid_constant__ Params p) {
+  using S = Shape<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t s_q_full, s_k_full[2], s_k_empty[2], s_v_full[2], s_v_empty[2], s_s_full, s_p_full, s_o_done;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  __shared__ Work s_work;
+
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = (int)uniform((uint32_t)tid >> 5);
+  const int split = blockIdx.x % p.splits, rest = blockIdx.x / p.splits;
+  const int head = rest % p.hkv, item = rest / p.hkv;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t q_at = base, k_at = base + S::kTileBytes, v_at = k_at + S::kStages * S::kTileBytes;
+  if (tid == 0) {
+    s_abort = 0;
+    mbar_init(smem_u32(&s_q_full), kLoaders);
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(smem_u32(&s_k_full[i]), kLoaders);
+      mbar_init(smem_u32(&s_v_full[i]), kLoaders);
+      mbar_init(smem_u32(&s_k_empty[i]), 1);
+      mbar_init(smem_u32(&s_v_empty[i]), 1);
+    }
+    mbar_init(smem_u32(&s_s_full), 1);
+    mbar_init(smem_u32(&s_p_full), kSoftmaxWarps);
+    mbar_init(smem_u32(&s_o_done), 1);
+    mbar_init_fence();
+  }
+  after_previous<false>();
+  if (blockIdx.x == 0 && p.status != nullptr) {            // scans that are not in order, or not within the rows
+    bool bad = false;
+    for (int b = tid; b <= p.B; b += kThreadsTc) {
+      const int q = __ldg(p.q_ptr + b), k = __ldg(p.k_ptr + b);
+      bad |= q < 0 || q > p.n_q || k < 0 || k > p.n_k;
+      if (b < p.B) bad |= q > __ldg(p.q_ptr + b + 1) || k > __ldg(p.k_ptr + b + 1);
+    }
+    if (bad) atomicOr(p.status, SPH_STATUS_BAD_INDEX);
+  }
+  if (warp == 0) {
+    const Work w = find_work<true>(p, item, kM);
+    if (lane == 0) s_work = w;
+  }
+  __syncthreads();
+  const Work w = s_work;
+  if (w.scan < 0) return;
+  const int2 keys = split_rows(w.nk, split, p.splits, kN);
+  const int tiles = (keys.y - keys.x + kN - 1) / kN;
+  const int rows = min(kM, w.nq * p.group - w.tile * kM);
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(&s_tmem), S::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = uniform(s_tmem);
+  volatile int* abort_flag = &s_abort;
+
+  if (warp < kSoftmaxWarps) {
+    // ======================= softmax: thread = row =======================
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const bool any_row = warp * 32 < rows;    // else this warp's lanes hold nothing that is read
+    const bool one = elect_one();
+    float top = -INFINITY, sum = 0.f;
+    bool dead = false;
+#pragma unroll 1
+    for (int j = 0; j < tiles; ++j) {
+      const int first = keys.x + j * kN, n = min(kN, keys.y - first);
+      const bool whole = n == kN && p.mask == nullptr;
+      uint4 bits;
+      if (!whole && any_row) bits = key_bits(p.mask, (int64_t)w.k0 + first, n);
+      if (!warp_wait(smem_u32(&s_s_full), (uint32_t)j & 1u, abort_flag)) { dead = true; break; }
+      tc_fence_after();
+      if (any_row) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kN / 32; ++c) {
+          uint32_t v[32];
+          tmem_ld32(lanes + S::kColS + 32 * c, v);
+          tmem_ld_wait();
+          if (whole) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) most = fmaxf(most, __uint_as_float(v[i]));
+          } else {
+            const uint32_t b = c == 0 ? bits.x : c == 1 ? bits.y : c == 2 ? bits.z : bits.w;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) most = fmaxf(most, b >> i & 1u ? __uint_as_float(v[i]) : -INFINITY);
+          }
+        }
+        most = most == -INFINITY ? most : most * p.scale_log2;       // scale >= 0; 0 times infinity is not wanted
+        const bool grown = most > top + kSlack;
+        float by = 1.f;
+        if (grown) {
+          by = exp2_approx(top - most);
+          top = most;
+          sum *= by;
+        }
+        if (j > 0) {
+          if (!warp_wait(smem_u32(&s_o_done), (uint32_t)(j - 1) & 1u, abort_flag)) { dead = true; break; }
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, grown)) {
+            for (int c = 0; c < p.d; c += 16) {
+              uint32_t v[16];
+              tmem_ld16(lanes + S::kColO + c, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * by);
+              tmem_st16(lanes + S::kColO + c, v);
+            }
+          }
+        }
+        const float minus = top == -INFINITY ? 0.f : -top;
+#pragma unroll
+        for (int c = 0; c < kN / 32; ++c) {
+          uint32_t v[32], h[16];
+          tmem_ld32(lanes + S::kColS + 32 * c, v);
+          tmem_ld_wait();
+          const uint32_t b = whole ? ~0u : c == 0 ? bits.x : c == 1 ? bits.y : c == 2 ? bits.z : bits.w;
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x = exp2_approx(fmaf(__uint_as_float(v[i]), p.scale_log2, minus));
+            float y = exp2_approx(fmaf(__uint_as_float(v[i + 1]), p.scale_log2, minus));
+            if (!whole) {
+              x = b >> i & 1u ? x : 0.f;
+              y = b >> (i + 1) & 1u ? y : 0.f;
+            }
+            sum += x;
+            sum += y;
+            h[i / 2] = pack2<BF16>(x, y);
+          }
+          tmem_st16(lanes + S::kColP + 16 * c, h);
+        }
+        tmem_st_wait();
+      } else if (j > 0) {
+        if (!warp_wait(smem_u32(&s_o_done), (uint32_t)(j - 1) & 1u, abort_flag)) { dead = true; break; }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (one) mbar_arrive(smem_u32(&s_p_full));
+    }
+    // ======================= epilogue =======================
+    if (!dead && (tiles == 0 || warp_wait(smem_u32(&s_o_done), (uint32_t)(tiles - 1) & 1u, abort_flag))) {
+      tc_fence_after();
+      const int r = warp * 32 + lane;
+      const bool mine = r < rows, none = sum == 0.f;
+      const int i = w.tile * kM + min(r, rows - 1);
+      const int64_t at = (int64_t)(w.q0 + i / p.group) * p.hq + head * p.group + i % p.group;
+      const float by = none ? 0.f : 1.f / sum, lse = none ? INFINITY : top + log2f(sum);
+      if (any_row) {
+        for (int c = 0; c < p.d; c += 16) {
+          uint32_t v[16];
+          if (tiles > 0) {
+            tmem_ld16(lanes + S::kColO + c, v);
+            tmem_ld_wait();
+          }
+          if (none) {                         // no keys: what O holds is not looked at
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = 0u;
+          }
+          if (mine) {
+            if (p.splits > 1) store16_float(v, by, p.part + ((int64_t)split * p.n_q * p.hq + at) * p.d + c, p.d - c);
+            else store16<BF16>(v, by, (uint16_t*)p.out + at * p.d + c, p.d - c);
+          }
+        }
+        if (mine && p.splits > 1) p.part_lse[(int64_t)split * p.n_q * p.hq + at] = lse;
+        else if (mine && p.lse) p.lse[at] = lse;
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ======================= MMA issuer =======================
+    const bool one = elect_one();
+    const uint32_t fmt = BF16 ? 1u : 0u;
+    const uint32_t idesc_s = make_idesc(1u, fmt, 0u, 0u, kM, kN);
+    const uint32_t idesc_o = make_idesc(1u, fmt, 0u, 1u, kM, (uint32_t)((p.d + 15) / 16 * 16));
+    const int steps = (p.d + 15) / 16;        // of 16 channels
+    const uint64_t q_desc = tile_desc(q_at, 16u);
+    auto scores = [&](int j) {                // S_j; false: a wait ran out
+      const int st = j % S::kStages;
+      if (!warp_wait(smem_u32(&s_k_full[st]), (uint32_t)(j / S::kStages) & 1u, abort_flag)) return false;
+      fence_proxy_async();
+      tc_fence_after();
+      if (one) {
+        const uint64_t k_desc = tile_desc(k_at + st * S::kTileBytes, 16u);
+#pragma unroll 1
+        for (int s = 0; s < steps; ++s) {
+          const uint32_t on = (uint32_t)(s >> 2) * (kM * 128u / 16u) + (uint32_t)(s & 3) * 2u;      // in 16 bytes
+          umma_f16(tmem + S::kColS, q_desc + on, k_desc + on, idesc_s, s ? 1u : 0u);
+        }
+        umma_commit(smem_u32(&s_k_empty[st]));
+        umma_commit(smem_u32(&s_s_full));
+      }
+      __syncwarp();
+      return true;
+    };
+    bool dead = tiles > 0 && !warp_wait(smem_u32(&s_q_full), 0u, abort_flag);
+    if (tiles > 0 && !dead) dead = !scores(0);
+#pragma unroll 1
+    for (int j = 0; j < tiles && !dead; ++j) {
+      if (!warp_wait(smem_u32(&s_p_full), (uint32_t)j & 1u, abort_flag)) break;
+      tc_fence_after();
+      if (!S::kOverS && j + 1 < tiles && !scores(j + 1)) break;
+      const int st = j % S::kStages;
+      if (!warp_wait(smem_u32(&s_v_full[st]), (uint32_t)(j / S::kStages) & 1u, abort_flag)) break;
+      fence_proxy_async();
+      tc_fence_after();
+      if (one) {
+        const uint64_t v_desc = tile_desc(v_at + st * S::kTileBytes, kM * 128u);
+#pragma unroll
+        for (int s = 0; s < kN / 16; ++s)
+          umma_f16_ta(tmem + S::kColO, tmem + S::kColP + 8 * s, v_desc + (uint64_t)(s * (2048 / 16)), idesc_o, j || s ? 1u : 0u);
+        umma_commit(smem_u32(&s_v_empty[st]));
+        umma_commit(smem_u32(&s_o_done));
+      }
+      __syncwarp();
+      if (S::kOverS && j + 1 < tiles) {       // S_j+1 goes where P_j is
+        if (!warp_wait(smem_u32(&s_o_done), (uint32_t)j & 1u, abort_flag)) break;
+        tc_fence_after();
+        if (!scores(j + 1)) break;
+      }
+    }
+  } else {
+    // ======================= loads =======================
+    const int t = tid - kLoadWarp * 32;
+    const Pieces pc = pieces_of(p.d);
+    if (tiles > 0) {
+      load_rows<kM, kLoaders>(q_at, t, rows, p.d, pc, p.q, [&](int r) {
+        const int i = w.tile * kM + r;
+        return (const uint16_t*)p.q + (int64_t)(w.q0 + i / p.group) * p.q_row + (head * p.group + i % p.group) * p.q_head;
+      }, [](int) { return true; });
+      cp_async_arrive_noinc(smem_u32(&s_q_full));
+    }
+    const uint16_t* k = (const uint16_t*)p.k + (int64_t)(w.k0 + keys.x) * p.k_row + head * p.k_head;
+    const uint16_t* v = (const uint16_t*)p.v + (int64_t)(w.k0 + keys.x) * p.v_row + head * p.v_head;
+    const uint8_t* mask = p.mask ? p.mask + w.k0 + keys.x : nullptr;
+#pragma unroll 1
+    for (int j = 0; j < tiles; ++j) {
+      const int st = j % S::kStages, n = min(kN, keys.y - keys.x - j * kN);
+      const uint32_t phase = ((uint32_t)(j / S::kStages) & 1u) ^ 1u;
+      auto key = [&](int r) { return mask == nullptr || __ldg(mask + (int64_t)j * kN + r) != 0; };
+      if (!warp_wait(smem_u32(&s_k_empty[st]), phase, abort_flag)) break;
+      load_rows<kM, kLoaders>(k_at + st * S::kTileBytes, t, n, p.d, pc, p.k, [&](int r) { return k + (int64_t)(j * kN + r) * p.k_row; }, key);
+      cp_async_arrive_noinc(smem_u32(&s_k_full[st]));
+      if (!warp_wait(smem_u32(&s_v_empty[st]), phase, abort_flag)) break;
+      load_rows<kM, kLoaders>(v_at + st * S::kTileBytes, t, n, p.d, pc, p.v, [&](int r) { return v + (int64_t)(j * kN + r) * p.v_row; }, key);
+      cp_async_arrive_noinc(smem_u32(&s_v_full[st]));
+    }
+    cp_async_wait_all();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (s_abort) {
+    wind_down(abort_flag, p.status);
+    __syncthreads();
+  }
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::kCols);
+  }
+}
+
+template <int DP, bool BF16>
+int start(const Params& p, int blocks, cudaStream_t st) {
+  SPH_CUDA(allow_smem(forward_tc_kernel<DP, BF16>, Shape<DP>::kSmem));
+  launch(forward_tc_kernel<DP, BF16>, blocks, kThreadsTc, Shape<DP>::kSmem, st, p);
+  SPH_LAUNCH_CHECK();
+  return SPH_OK;
+}
+
+}  // namespace
+
+int attention_forward_tc(const Params& p, bool bf16, int blocks, cudaStream_t st) {
+  if (p.d <= 64) return bf16 ? start<64, true>(p, blocks, st) : start<64, false>(p, blocks, st);
+  return bf16 ? start<128, true>(p, blocks, st) : start<128, false>(p, blocks, st);
+}
+
+}  // namespace attn
+}  // namespace sph
