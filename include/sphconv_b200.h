@@ -354,7 +354,8 @@ int sph_residual_norm_backward(const sph_norm* args, const void* d_dout, const v
  *   q [n_q, q_heads, channels], k, v [n_k, k_heads, channels] in `dtype` (SPH_F32, SPH_F16, SPH_BF16), channels consecutive, rows and
  *                heads any strides apart (in elements); at most SPH_ATTENTION_MAX_CHANNELS channels
  *   key_mask     [n_k] or null: rows where it is 0 are no keys, and may hold anything
- *   d_out, d_dq  [n_q, q_heads, channels]   d_dk, d_dv  [n_k, k_heads, channels], consecutive, as d_dout
+ *   d_out, d_dq  [n_q, q_heads, channels]   d_dk, d_dv  [n_k, k_heads, channels], consecutive and 16-byte aligned, as
+ *                d_dout
  *   d_lse        float [n_q, q_heads]: log2 of the sum of 2^(score log2 e), for the backward pass; may be null
  *   d_scratch    sph_attention_scratch_bytes(args, backward) bytes, 16-byte aligned (forward: null where that is 0)
  * Backward: d_dq may be null, and d_dk with d_dv.  Scores, softmax statistics and sums are fp32.  Results do not depend on the run. */
@@ -371,7 +372,7 @@ typedef struct sph_attention {
 int64_t sph_attention_scratch_bytes(const sph_attention* args, int backward);
 int sph_attention_forward(const sph_attention* args, void* d_out, float* d_lse, void* d_scratch, int32_t* d_status, void* stream);
 int sph_attention_backward(const sph_attention* args, const void* d_dout, const void* d_out, const float* d_lse, void* d_scratch,
-                           void* d_dq, void* d_dk, void* d_dv, void* stream);
+                           void* d_dq, void* d_dk, void* d_dv, int32_t* d_status, void* stream);
 
 /* The global norm of `count` gradients, and clipping by it:  *d_norm = sqrt(sum g^2) (SPH_NORM_2; sums in 64 bits) or max |g|
  * (SPH_NORM_MAX; NaN if any is), and  dst = src * min(1, max_norm / (*d_norm + 1e-6)).

@@ -100,7 +100,7 @@ SIGNATURES = {
     "sph_residual_norm_backward": (cint, [ctypes.POINTER(Norm), vp, vp, vp, vp, vp, vp, vp, ctypes.POINTER(vp), vp]),
     "sph_attention_scratch_bytes": (i64, [ctypes.POINTER(Attention), cint]),
     "sph_attention_forward": (cint, [ctypes.POINTER(Attention), vp, vp, vp, vp, vp]),
-    "sph_attention_backward": (cint, [ctypes.POINTER(Attention), vp, vp, vp, vp, vp, vp, vp, vp]),
+    "sph_attention_backward": (cint, [ctypes.POINTER(Attention), vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     "sph_grad_norm_scratch_bytes": (i64, [i32]),
     "sph_grad_norm": (cint, [ctypes.POINTER(ClipTensor), i32, cint, vp, vp, vp]),
     "sph_grad_clip": (cint, [ctypes.POINTER(ClipTensor), i32, cint, ctypes.c_float, vp, vp, vp]),

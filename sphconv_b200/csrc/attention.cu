@@ -433,6 +433,9 @@ __global__ void __launch_bounds__(kThreads) join_sum_kernel(const float* part, i
 }
 
 int attention_forward_tc(const Params& p, bool bf16, int blocks, cudaStream_t st);      // attention_tc.cu
+// attention_tc_bwd.cu
+int attention_backward_tc(const Params& p, bool bf16, bool keys, int blocks, cudaStream_t st);
+int attention_backward_tc_blocks(int d, bool keys);
 
 namespace {
 
@@ -475,6 +478,12 @@ Plan plan_of(const sph_attention& a, const Params& params, int sms) {
     p.fwd_blocks = most_tiles(a.n_q * group, kTcTile, a.B) * a.k_heads;
     const int64_t real = std::max<int64_t>(1, div_up64(a.n_q * group, (int64_t)kTcTile * a.B)) * a.B * a.k_heads;
     p.fwd_splits = splits_for(real, 2 * sms, a.n_k, a.B, 2 * kTcTile);
+    p.dq_blocks = p.fwd_blocks;
+    p.dkv_blocks = most_tiles(a.n_k, kTcTile, a.B) * a.k_heads;
+    const int64_t k_tiles_real = std::max<int64_t>(1, div_up64(a.n_k, (int64_t)kTcTile * a.B)) * a.B * a.k_heads;
+    p.dq_splits = splits_for(real, attention_backward_tc_blocks(a.channels, false) * sms, a.n_k, a.B, 2 * kTcTile);
+    p.dkv_splits = splits_for(k_tiles_real, attention_backward_tc_blocks(a.channels, true) * sms, a.n_q * group, a.B, 2 * kTcTile);
+    return p;
   }
   p.dkv_splits = splits_for(k_real, sms * per_sm(backward_smem(dp, true)), a.n_q * group, a.B, 2 * kTile);
   return p;
@@ -522,7 +531,8 @@ int run_forward(Params p, const Plan& plan, bool tensor_cores, void* scratch, cu
 }
 
 template <typename T>
-int run_backward(Params p, const Plan& plan, const void* out, void* scratch, cudaStream_t st) {
+int run_backward(Params p, const Plan& plan, bool tensor_cores, const void* out, void* scratch, cudaStream_t st) {
+  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   const int64_t rows = (int64_t)p.n_q * p.hq, k_values = (int64_t)p.n_k * p.hkv * p.d;
   float* delta = (float*)scratch;
   float* part = delta + (rows + 3) / 4 * 4;
@@ -534,7 +544,8 @@ int run_backward(Params p, const Plan& plan, const void* out, void* scratch, cud
   if (p.dq && rows) {
     p.splits = plan.dq_splits;
     p.part = part;
-    int rc = backward<T, false>(p, plan.dq_blocks * p.splits, st);
+    const int rc = tensor_cores ? attention_backward_tc(p, bf16, false, plan.dq_blocks * p.splits, st)
+                                : backward<T, false>(p, plan.dq_blocks * p.splits, st);
     if (rc != SPH_OK) return rc;
     if (p.splits > 1) {
       launch(join_sum_kernel<T>, grid_for(rows * p.d, kThreads), kThreads, 0, st, part, p.splits, rows * p.d, (T*)p.dq);
@@ -545,7 +556,8 @@ int run_backward(Params p, const Plan& plan, const void* out, void* scratch, cud
     p.splits = plan.dkv_splits;
     p.part = part;
     p.part2 = part + k_values * p.splits;
-    int rc = backward<T, true>(p, plan.dkv_blocks * p.splits, st);
+    const int rc = tensor_cores ? attention_backward_tc(p, bf16, true, plan.dkv_blocks * p.splits, st)
+                                : backward<T, true>(p, plan.dkv_blocks * p.splits, st);
     if (rc != SPH_OK) return rc;
     if (p.splits > 1) {
       launch(join_sum_kernel<T>, grid_for(k_values, kThreads), kThreads, 0, st, p.part, p.splits, k_values, (T*)p.dk);
@@ -636,22 +648,25 @@ extern "C" int sph_attention_forward(const sph_attention* a, void* d_out, float*
 }
 
 extern "C" int sph_attention_backward(const sph_attention* a, const void* d_dout, const void* d_out, const float* d_lse, void* d_scratch,
-                                      void* d_dq, void* d_dk, void* d_dv, void* stream) {
+                                      void* d_dq, void* d_dk, void* d_dv, int32_t* d_status, void* stream) {
   Params p;
   const int rc = fill(a, __func__, &p);
   if (rc != SPH_OK) return rc;
   SPH_CHECK_ARG(a->n_q == 0 || (d_dout && d_out && d_lse), "null pointer");
   SPH_CHECK_ARG(!!d_dk == !!d_dv, "the gradients of keys and values come together");
   SPH_CHECK_ARG(d_scratch && (uintptr_t)d_scratch % 16 == 0, "the scratch must be 16-byte aligned");
+  SPH_CHECK_ARG((((uintptr_t)d_dout | (uintptr_t)d_out | (uintptr_t)d_dq | (uintptr_t)d_dk | (uintptr_t)d_dv) & 15) == 0,
+                "gradients and results must be 16-byte aligned");
   const int sms = current_sm_count();
   if (sms <= 0) return SPH_ERR_CUDA;
   const Plan plan = plan_of(*a, p, sms);
   p.d_out = d_dout;
   p.lse = const_cast<float*>(d_lse);
   p.dq = d_dq; p.dk = d_dk; p.dv = d_dv;
-  p.vec = p.vec && ((uintptr_t)d_dout & 15) == 0;
+  p.status = d_status;
   const cudaStream_t st = (cudaStream_t)stream;
-  if (a->dtype == SPH_F32) return run_backward<float>(p, plan, d_out, d_scratch, st);
-  if (a->dtype == SPH_F16) return run_backward<__half>(p, plan, d_out, d_scratch, st);
-  return run_backward<__nv_bfloat16>(p, plan, d_out, d_scratch, st);
+  const bool tc = on_tensor_cores(*a, p);
+  if (a->dtype == SPH_F32) return run_backward<float>(p, plan, tc, d_out, d_scratch, st);
+  if (a->dtype == SPH_F16) return run_backward<__half>(p, plan, tc, d_out, d_scratch, st);
+  return run_backward<__nv_bfloat16>(p, plan, tc, d_out, d_scratch, st);
 }

@@ -799,7 +799,8 @@ struct AttentionLayer : public torch::autograd::Function<AttentionLayer> {
                                                 saved[5].defined() ? optional<Tensor>(saved[5]) : std::nullopt,
                                                 ctx->saved_data["scale"].toDouble());
     const c10::cuda::CUDAGuard guard(in.q.device());
-    const Tensor d_out = grads[0].to(in.q.scalar_type()).contiguous();
+    Tensor d_out = grads[0].to(in.q.scalar_type()).contiguous();
+    if ((uintptr_t)ptr(d_out) % 16 != 0) d_out = d_out.clone();
     Tensor dq, dk, dv;
     if (ctx->needs_input_grad(0)) dq = empty(in.q.sizes(), in.q.scalar_type(), in.q);
     if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
@@ -810,7 +811,7 @@ struct AttentionLayer : public torch::autograd::Function<AttentionLayer> {
     const Tensor scratch = empty({std::max<int64_t>(16, check(abi.sph_attention_scratch_bytes(&a, 1)))}, at::kByte, in.q);
     auto at_or_null = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
     check(abi.sph_attention_backward(&a, ptr(d_out), ptr(saved[6]), static_cast<const float*>(ptr(saved[7])), ptr(scratch), at_or_null(dq),
-                                     at_or_null(dk), at_or_null(dv), stream_of(in.q)));
+                                     at_or_null(dk), at_or_null(dv), status_of(in.q), stream_of(in.q)));
     return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
