@@ -34,8 +34,70 @@ struct Shape {
   static constexpr int kSmem = 1024 + (1 + 2 * kStages) * (int)kTileBytes;
 };
 
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// The largest of a row's 128 scores at TMEM `at`, of those whose bit is set (WHOLE: all).
+template <bool WHOLE>
+__device__ __forceinline__ float row_max(uint32_t at, const uint4& bits) {
+  float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t v[2][32];
+    tmem_ld32(at + 64 * h, v[0]);
+    tmem_ld32(at + 64 * h + 32, v[1]);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t b = word(bits, 2 * h + k);
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        float x = __uint_as_float(v[k][i]), y = __uint_as_float(v[k][i + 1]);
+        if (!WHOLE) {
+          x = b >> i & 1u ? x : -INFINITY;
+          y = b >> (i + 1) & 1u ? y : -INFINITY;
+        }
+        most[i / 2 & 3] = max3(most[i / 2 & 3], x, y);
+      }
+    }
+  }
+  return max3(max3(most[0], most[1], most[2]), most[3], most[3]);
+}
+
+// P = 2^(scale S + minus) of a row's scores at TMEM `at`, 0 where the bit is not set, to TMEM `to` in the rows' type, which may be the
+// first half of `at`; returns the sum of P before rounding.
+template <bool WHOLE, bool BF16>
+__device__ __forceinline__ float row_exp(uint32_t at, uint32_t to, const uint4& bits, float scale, float minus) {
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  const float2 scale2 = make_float2(scale, scale), minus2 = make_float2(minus, minus);
+  uint32_t v[2][32];
+  tmem_ld32(at, v[0]);
+#pragma unroll
+  for (int c = 0; c < kN / 32; ++c) {
+    uint32_t(&x)[32] = v[c & 1];
+    tmem_ld_wait();
+    if (c + 1 < kN / 32) tmem_ld32(at + 32 * (c + 1), v[(c + 1) & 1]);
+    const uint32_t b = word(bits, c);
+    uint32_t h[16];
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float2 e = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, minus2);
+      float2 y = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+      if (!WHOLE) {
+        y.x = b >> i & 1u ? y.x : 0.f;
+        y.y = b >> (i + 1) & 1u ? y.y : 0.f;
+      }
+      sum[i / 2 & 1] = add2(sum[i / 2 & 1], y);
+      h[i / 2] = pack2<BF16>(y.x, y.y);
+    }
+    tmem_st16(to + 16 * c, h);
+  }
+  const float2 s = add2(sum[0], sum[1]);
+  return s.x + s.y;
+}
+
 template <int DP, bool BF16>
-__global__ void __launch_bounds__(kThreadsTc, 2) forward_tc_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreadsTc, 2)
+forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ TileMap k_map, const __grid_constant__ TileMap v_map) {
   using S = Shape<DP>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_q_full, s_k_full[2], s_k_empty[2], s_v_full[2], s_v_empty[2], s_s_full, s_p_full, s_o_done;
@@ -53,8 +115,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) forward_tc_kernel(const __grid_
     s_abort = 0;
     mbar_init(smem_u32(&s_q_full), kLoaders);
     for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(smem_u32(&s_k_full[i]), kLoaders);
-      mbar_init(smem_u32(&s_v_full[i]), kLoaders);
+      mbar_init(smem_u32(&s_k_full[i]), kLoadWarps);
+      mbar_init(smem_u32(&s_v_full[i]), kLoadWarps);
       mbar_init(smem_u32(&s_k_empty[i]), 1);
       mbar_init(smem_u32(&s_v_empty[i]), 1);
     }
@@ -109,21 +171,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) forward_tc_kernel(const __grid_
       if (!warp_wait(smem_u32(&s_s_full), (uint32_t)j & 1u, abort_flag)) { dead = true; break; }
       tc_fence_after();
       if (any_row) {
-        float most = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < kN / 32; ++c) {
-          uint32_t v[32];
-          tmem_ld32(lanes + S::kColS + 32 * c, v);
-          tmem_ld_wait();
-          if (whole) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) most = fmaxf(most, __uint_as_float(v[i]));
-          } else {
-            const uint32_t b = c == 0 ? bits.x : c == 1 ? bits.y : c == 2 ? bits.z : bits.w;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) most = fmaxf(most, b >> i & 1u ? __uint_as_float(v[i]) : -INFINITY);
-          }
-        }
+        const uint32_t at_s = lanes + S::kColS;
+        float most = whole ? row_max<true>(at_s, bits) : row_max<false>(at_s, bits);
         most = most == -INFINITY ? most : most * p.scale_log2;       // scale >= 0; 0 times infinity is not wanted
         const bool grown = most > top + kSlack;
         float by = 1.f;
@@ -147,26 +196,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) forward_tc_kernel(const __grid_
           }
         }
         const float minus = top == -INFINITY ? 0.f : -top;
-#pragma unroll
-        for (int c = 0; c < kN / 32; ++c) {
-          uint32_t v[32], h[16];
-          tmem_ld32(lanes + S::kColS + 32 * c, v);
-          tmem_ld_wait();
-          const uint32_t b = whole ? ~0u : c == 0 ? bits.x : c == 1 ? bits.y : c == 2 ? bits.z : bits.w;
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float x = exp2_approx(fmaf(__uint_as_float(v[i]), p.scale_log2, minus));
-            float y = exp2_approx(fmaf(__uint_as_float(v[i + 1]), p.scale_log2, minus));
-            if (!whole) {
-              x = b >> i & 1u ? x : 0.f;
-              y = b >> (i + 1) & 1u ? y : 0.f;
-            }
-            sum += x;
-            sum += y;
-            h[i / 2] = pack2<BF16>(x, y);
-          }
-          tmem_st16(lanes + S::kColP + 16 * c, h);
-        }
+        sum += whole ? row_exp<true, BF16>(at_s, lanes + S::kColP, bits, p.scale_log2, minus)
+                     : row_exp<false, BF16>(at_s, lanes + S::kColP, bits, p.scale_log2, minus);
         tmem_st_wait();
       } else if (j > 0) {
         if (!warp_wait(smem_u32(&s_o_done), (uint32_t)(j - 1) & 1u, abort_flag)) { dead = true; break; }
@@ -266,20 +297,34 @@ __global__ void __launch_bounds__(kThreadsTc, 2) forward_tc_kernel(const __grid_
       }, [](int) { return true; });
       cp_async_arrive_noinc(smem_u32(&s_q_full));
     }
-    const uint16_t* k = (const uint16_t*)p.k + (int64_t)(w.k0 + keys.x) * p.k_row + head * p.k_head;
-    const uint16_t* v = (const uint16_t*)p.v + (int64_t)(w.k0 + keys.x) * p.v_row + head * p.v_head;
     const uint8_t* mask = p.mask ? p.mask + w.k0 + keys.x : nullptr;
+    const bool one = elect_one();
+    // 128 rows from key `first` of the part on: whole tiles by TMA, others row by row
+    auto bring = [&](uint32_t to, const TileMap& m, const void* x, int64_t row_stride, int64_t head_stride, int first, int n, uint32_t bar) {
+      if (n == kN && mask == nullptr && m.usable) {
+        if (one && warp == kLoadWarp) {
+          mbar_arrive_expect_tx(bar, S::kTileBytes);
+          tma_tile<DP>(to, kM * 128u, m, head, w.k0 + keys.x + first, bar);
+        } else if (one) {
+          mbar_arrive(bar);
+        }
+        return;
+      }
+      const uint16_t* from = (const uint16_t*)x + (int64_t)(w.k0 + keys.x + first) * row_stride + head * head_stride;
+      load_rows<kM, kLoaders>(to, t, n, p.d, pc, x, [&](int r) { return from + r * row_stride; },
+                             [&](int r) { return mask == nullptr || __ldg(mask + first + r) != 0; });
+      cp_async_arrive(bar);
+      __syncwarp();
+      if (one) mbar_arrive(bar);
+    };
 #pragma unroll 1
     for (int j = 0; j < tiles; ++j) {
-      const int st = j % S::kStages, n = min(kN, keys.y - keys.x - j * kN);
+      const int st = j % S::kStages, first = j * kN, n = min(kN, keys.y - keys.x - first);
       const uint32_t phase = ((uint32_t)(j / S::kStages) & 1u) ^ 1u;
-      auto key = [&](int r) { return mask == nullptr || __ldg(mask + (int64_t)j * kN + r) != 0; };
       if (!warp_wait(smem_u32(&s_k_empty[st]), phase, abort_flag)) break;
-      load_rows<kM, kLoaders>(k_at + st * S::kTileBytes, t, n, p.d, pc, p.k, [&](int r) { return k + (int64_t)(j * kN + r) * p.k_row; }, key);
-      cp_async_arrive_noinc(smem_u32(&s_k_full[st]));
+      bring(k_at + st * S::kTileBytes, k_map, p.k, p.k_row, p.k_head, first, n, smem_u32(&s_k_full[st]));
       if (!warp_wait(smem_u32(&s_v_empty[st]), phase, abort_flag)) break;
-      load_rows<kM, kLoaders>(v_at + st * S::kTileBytes, t, n, p.d, pc, p.v, [&](int r) { return v + (int64_t)(j * kN + r) * p.v_row; }, key);
-      cp_async_arrive_noinc(smem_u32(&s_v_full[st]));
+      bring(v_at + st * S::kTileBytes, v_map, p.v, p.v_row, p.v_head, first, n, smem_u32(&s_v_full[st]));
     }
     cp_async_wait_all();
   }
@@ -297,13 +342,48 @@ __global__ void __launch_bounds__(kThreadsTc, 2) forward_tc_kernel(const __grid_
 
 template <int DP, bool BF16>
 int start(const Params& p, int blocks, cudaStream_t st) {
+  TileMap k_map, v_map;
+  make_tile_map(&k_map, p.k, p.n_k, p.hkv, p.d, p.k_row, p.k_head, kN, 1);
+  make_tile_map(&v_map, p.v, p.n_k, p.hkv, p.d, p.v_row, p.v_head, kN, 1);
   SPH_CUDA(allow_smem(forward_tc_kernel<DP, BF16>, Shape<DP>::kSmem));
-  launch(forward_tc_kernel<DP, BF16>, blocks, kThreadsTc, Shape<DP>::kSmem, st, p);
+  launch(forward_tc_kernel<DP, BF16>, blocks, kThreadsTc, Shape<DP>::kSmem, st, p, k_map, v_map);
   SPH_LAUNCH_CHECK();
   return SPH_OK;
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return (EncodeTiled)f;
+  }();
+  return fn;
+}
+
 }  // namespace
+
+void make_tile_map(TileMap* m, const void* x, int64_t rows, int heads, int d, int64_t row_stride, int64_t head_stride, int tile, int group) {
+  *m = TileMap{};
+  const EncodeTiled encode = encode_tiled();
+  if (encode == nullptr || rows < 1 || tile % group != 0) return;
+  // a dimension of one entry has any stride
+  const int64_t hs = heads > 1 ? head_stride * 2 : 128, rs = rows > 1 ? row_stride * 2 : 128;
+  if (hs <= 0 || rs <= 0 || hs % 16 != 0 || rs % 16 != 0 || ((uintptr_t)x & 15) != 0) return;
+  m->rows_inside = group == 1 && hs > rs;
+  const bool in = m->rows_inside;
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)(in ? rows : heads), (cuuint64_t)(in ? heads : rows)};
+  const cuuint64_t strides[2] = {(cuuint64_t)(in ? rs : hs), (cuuint64_t)(in ? hs : rs)};
+  const cuuint32_t box[3] = {64, (cuuint32_t)(in ? tile : group), (cuuint32_t)(in ? 1 : tile / group)}, steps[3] = {1, 1, 1};
+  m->usable = encode(&m->map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(x), dims, strides, box, steps,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 int attention_forward_tc(const Params& p, bool bf16, int blocks, cudaStream_t st) {
   if (p.d <= 64) return bf16 ? start<64, true>(p, blocks, st) : start<64, false>(p, blocks, st);

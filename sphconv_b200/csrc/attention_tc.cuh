@@ -5,6 +5,8 @@
 // along its rows (MN-major: products with P or dS).
 #pragma once
 
+#include <cuda.h>
+
 #include <type_traits>
 
 #include "attention.cuh"
@@ -62,6 +64,39 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// Two float32 operations an instruction.
+__device__ __forceinline__ uint64_t as_pair(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 of_pair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as_pair(a)), "l"(as_pair(b)), "l"(as_pair(c)));
+  return of_pair(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_pair(a)), "l"(as_pair(b)));
+  return of_pair(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_pair(a)), "l"(as_pair(b)));
+  return of_pair(r);
+}
+
 // Two values rounded to the rows' type, the first in the lower half.
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -71,6 +106,31 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
   const __half2 v = __floats2half2_rn(a, b);
   return *(const uint32_t*)&v;
+}
+
+// Rows of one head, or of the heads of a group, as TMA brings them to a tile: blocks of 64 channels, zeros behind the last one.
+struct TileMap {
+  CUtensorMap map;                            // [heads][rows] or [rows][heads] of channels, the smaller stride inside
+  int rows_inside;
+  int usable;                                 // 0: strides or a group that a map cannot have; rows are copied with cp.async
+};
+
+// Rows `first` on of `head` to the tile at `to`, whose blocks are `block` bytes; by one thread, which has announced the bytes.
+template <int DP>
+__device__ __forceinline__ void tma_tile(uint32_t to, uint32_t block, const TileMap& m, int head, int first, uint32_t bar) {
+  const int a = m.rows_inside ? first : head, b = m.rows_inside ? head : first;
+#pragma unroll
+  for (int x = 0; x < DP; x += 64)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            to + (uint32_t)(x / 64) * block),
+        "l"(&m.map), "r"(x), "r"(a), "r"(b), "r"(bar)
+        : "memory");
+}
+
+// The barrier gets an arrival more, which comes when this thread's copies so far have landed: the warp's own arrival follows at once.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // How `threads` loading threads share a tile's 16-byte pieces: `lanes` of them (a power of two) a row.
@@ -137,6 +197,10 @@ __device__ __forceinline__ uint4 key_bits(const uint8_t* mask, int64_t first, in
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+
+// Host: a map of x [rows][heads][d] with strides in elements, for tiles of `tile` rows of a head, or (group > 1) of the rows of `group`
+// heads taken together.
+void make_tile_map(TileMap* m, const void* x, int64_t rows, int heads, int d, int64_t row_stride, int64_t head_stride, int tile, int group);
 
 // What a kernel does when a wait ran out, in front of its last barrier: report, and let what is in flight end.
 __device__ __forceinline__ void wind_down(volatile int* aborted, int* status) {
