@@ -440,9 +440,9 @@ int attention_backward_tc_blocks(int d, bool keys);
 namespace {
 
 // 16-bit rows in pieces of 16 bytes go to the tensor cores; there the largest score is found before it is scaled, so not with a
-// negative scale.
+// scale that is negative or zero.
 bool on_tensor_cores(const sph_attention& a, const Params& p) {
-  return (a.dtype == SPH_F16 || a.dtype == SPH_BF16) && p.vec && p.scale >= 0.f;
+  return (a.dtype == SPH_F16 || a.dtype == SPH_BF16) && p.vec && p.scale > 0.f;
 }
 constexpr int kTcTile = 128;
 

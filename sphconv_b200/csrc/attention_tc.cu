@@ -1,12 +1,15 @@
 // Cross attention on the Blackwell tensor cores (tcgen05), forward, for 16-bit rows of 8 to 128 channels in steps of 8.
 //
-//   S [128 x 128] = Q K^T   A = a tile of 128 query rows, B = 128 keys, both K-major in shared memory; S in TMEM
-//   P = 2^(scale log2 e S - top) in the rows' type, written over TMEM columns by the thread that has the row
+//   S [128 x 64] = Q K^T    A = a tile of 128 query rows, B = 64 keys, K-major in shared memory; S in TMEM
+//   P = 2^(scale log2 e S - top) in the rows' type, written over S by the thread that has the row
 //   O [128 x d] += P V      A = P in TMEM, B = the same keys' values, MN-major in shared memory; O stays in TMEM
 //
 // A block has one tile of queries (heads that share a key head are rows of it) and walks a scan's keys, or a part of them.  Warps 0-3
-// do the softmax, a thread a row; warp 4 issues the MMAs; warps 5-7 copy keys and values with cp.async, which fills in zeros where
-// there is no key.  Two blocks share an SM, and one's softmax runs while the other's MMAs do.
+// do the softmax, a thread a row; warp 4 issues the MMAs; warps 5-7 bring keys and values: whole tiles by TMA, tiles with keys
+// missing (the scan's end, a mask) row by row with cp.async, which fills in zeros.  S has two places, so that the next scores are there
+// when a row's softmax ends, and two blocks share an SM.
+//   Queries of up to 64 channels are an operand in TMEM: from shared memory, A and B of an MMA of 64 columns take 48 cycles to
+// read and 32 to multiply.  128 channels leave no columns for them.
 //   The running maximum follows S only when it has grown by more than 2^8: O is read, scaled and written again in those tiles alone,
 // P stays within 2^8 and a row's sum within float32.
 #include <algorithm>
@@ -18,81 +21,36 @@ namespace attn {
 
 namespace {
 
-constexpr int kN = 128;                       // keys of a tile
+constexpr int kN = 64;                        // keys of a tile
 constexpr int kSoftmaxWarps = 4, kMmaWarp = 4, kLoadWarp = 5, kLoadWarps = 3;
 constexpr int kThreadsTc = (kLoadWarp + kLoadWarps) * 32;
 constexpr int kLoaders = kLoadWarps * 32;
 constexpr float kSlack = 8.f;                 // log2 of how far a row's maximum may be above the one that P is taken against
 
-// DP: channels of a tile's rows in shared memory, 64 or 128.  128 channels of O leave no columns for P beside S: it lies in them.
+// DP: channels of a tile's rows, 64 or 128.
 template <int DP>
 struct Shape {
-  static constexpr int kStages = DP == 64 ? 2 : 1;
-  static constexpr uint32_t kTileBytes = (DP / 64) * kM * 128u;
-  static constexpr bool kOverS = DP == 128;
-  static constexpr uint32_t kColS = 0, kColP = kOverS ? 0 : 128, kColO = kOverS ? 128 : 192, kCols = 256;
-  static constexpr int kSmem = 1024 + (1 + 2 * kStages) * (int)kTileBytes;
+  static constexpr bool kQInTmem = DP == 64;
+  static constexpr int kStages = DP == 64 ? 4 : 2;
+  static constexpr uint32_t kQBytes = kQInTmem ? 0 : (DP / 64) * kM * 128u, kTileBytes = (DP / 64) * kN * 128u;
+  static constexpr uint32_t kColS = 0, kColO = 2 * kN, kColQ = kColO + DP, kCols = 256;
+  static constexpr int kSmem = 1024 + (int)kQBytes + 2 * kStages * (int)kTileBytes;
 };
 
-__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-
-// The largest of a row's 128 scores at TMEM `at`, of those whose bit is set (WHOLE: all).
-template <bool WHOLE>
-__device__ __forceinline__ float row_max(uint32_t at, const uint4& bits) {
-  float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t v[2][32];
-    tmem_ld32(at + 64 * h, v[0]);
-    tmem_ld32(at + 64 * h + 32, v[1]);
-    tmem_ld_wait();
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint32_t b = word(bits, 2 * h + k);
-#pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        float x = __uint_as_float(v[k][i]), y = __uint_as_float(v[k][i + 1]);
-        if (!WHOLE) {
-          x = b >> i & 1u ? x : -INFINITY;
-          y = b >> (i + 1) & 1u ? y : -INFINITY;
-        }
-        most[i / 2 & 3] = max3(most[i / 2 & 3], x, y);
-      }
-    }
-  }
-  return max3(max3(most[0], most[1], most[2]), most[3], most[3]);
-}
-
-// P = 2^(scale S + minus) of a row's scores at TMEM `at`, 0 where the bit is not set, to TMEM `to` in the rows' type, which may be the
-// first half of `at`; returns the sum of P before rounding.
-template <bool WHOLE, bool BF16>
-__device__ __forceinline__ float row_exp(uint32_t at, uint32_t to, const uint4& bits, float scale, float minus) {
+// P = 2^(scale s + minus) of 64 scores in the rows' type, and the sum of P before rounding.
+template <bool BF16>
+__device__ __forceinline__ float row_exp(const uint32_t (&s)[kN], uint32_t (&h)[kN / 2], float scale, float minus) {
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   const float2 scale2 = make_float2(scale, scale), minus2 = make_float2(minus, minus);
-  uint32_t v[2][32];
-  tmem_ld32(at, v[0]);
 #pragma unroll
-  for (int c = 0; c < kN / 32; ++c) {
-    uint32_t(&x)[32] = v[c & 1];
-    tmem_ld_wait();
-    if (c + 1 < kN / 32) tmem_ld32(at + 32 * (c + 1), v[(c + 1) & 1]);
-    const uint32_t b = word(bits, c);
-    uint32_t h[16];
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const float2 e = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, minus2);
-      float2 y = make_float2(exp2_approx(e.x), exp2_approx(e.y));
-      if (!WHOLE) {
-        y.x = b >> i & 1u ? y.x : 0.f;
-        y.y = b >> (i + 1) & 1u ? y.y : 0.f;
-      }
-      sum[i / 2 & 1] = add2(sum[i / 2 & 1], y);
-      h[i / 2] = pack2<BF16>(y.x, y.y);
-    }
-    tmem_st16(to + 16 * c, h);
+  for (int i = 0; i < kN; i += 2) {
+    const float2 e = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, minus2);
+    const float2 y = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+    sum[i / 2 & 1] = add2(sum[i / 2 & 1], y);
+    h[i / 2] = pack2<BF16>(y.x, y.y);
   }
-  const float2 s = add2(sum[0], sum[1]);
-  return s.x + s.y;
+  const float2 t = add2(sum[0], sum[1]);
+  return t.x + t.y;
 }
 
 template <int DP, bool BF16>
@@ -100,7 +58,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2)
 forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ TileMap k_map, const __grid_constant__ TileMap v_map) {
   using S = Shape<DP>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t s_q_full, s_k_full[2], s_k_empty[2], s_v_full[2], s_v_empty[2], s_s_full, s_p_full, s_o_done;
+  __shared__ __align__(8) uint64_t s_q_full, s_k_full[S::kStages], s_k_empty[S::kStages], s_v_full[S::kStages], s_v_empty[S::kStages];
+  __shared__ __align__(8) uint64_t s_s_full[2], s_p_full[2], s_o_done[2];       // of even and odd tiles
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ Work s_work;
@@ -110,19 +69,21 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
   const int split = blockIdx.x % p.splits, rest = blockIdx.x / p.splits;
   const int head = rest % p.hkv, item = rest / p.hkv;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t q_at = base, k_at = base + S::kTileBytes, v_at = k_at + S::kStages * S::kTileBytes;
+  const uint32_t q_at = base, k_at = base + S::kQBytes, v_at = k_at + S::kStages * S::kTileBytes;
   if (tid == 0) {
     s_abort = 0;
-    mbar_init(smem_u32(&s_q_full), kLoaders);
+    mbar_init(smem_u32(&s_q_full), S::kQInTmem ? kSoftmaxWarps : kLoadWarps);
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(smem_u32(&s_k_full[i]), kLoadWarps);
       mbar_init(smem_u32(&s_v_full[i]), kLoadWarps);
       mbar_init(smem_u32(&s_k_empty[i]), 1);
       mbar_init(smem_u32(&s_v_empty[i]), 1);
     }
-    mbar_init(smem_u32(&s_s_full), 1);
-    mbar_init(smem_u32(&s_p_full), kSoftmaxWarps);
-    mbar_init(smem_u32(&s_o_done), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&s_s_full[i]), 1);
+      mbar_init(smem_u32(&s_p_full[i]), kSoftmaxWarps);
+      mbar_init(smem_u32(&s_o_done[i]), 1);
+    }
     mbar_init_fence();
   }
   after_previous<false>();
@@ -160,59 +121,85 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
     const bool any_row = warp * 32 < rows;    // else this warp's lanes hold nothing that is read
     const bool one = elect_one();
+    const int r = warp * 32 + lane;
+    const bool mine = r < rows;
+    const int row_i = w.tile * kM + min(r, rows - 1);
+    const int64_t row_q = w.q0 + row_i / p.group;
+    const int row_h = head * p.group + row_i % p.group;
+    if (S::kQInTmem && tiles > 0) {
+      const uint4* from = (const uint4*)((const uint16_t*)p.q + row_q * p.q_row + row_h * p.q_head);
+      const int pieces = p.d / 8;
+      uint32_t v[32];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const uint4 x = mine && c < pieces ? __ldg(from + c) : make_uint4(0u, 0u, 0u, 0u);
+        v[4 * c] = x.x; v[4 * c + 1] = x.y; v[4 * c + 2] = x.z; v[4 * c + 3] = x.w;
+      }
+      tmem_st32(lanes + S::kColQ, v);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (one) mbar_arrive(smem_u32(&s_q_full));
+    }
     float top = -INFINITY, sum = 0.f;
     bool dead = false;
 #pragma unroll 1
     for (int j = 0; j < tiles; ++j) {
-      const int first = keys.x + j * kN, n = min(kN, keys.y - first);
+      const int first = keys.x + j * kN, n = min(kN, keys.y - first), b = j & 1;
       const bool whole = n == kN && p.mask == nullptr;
-      uint4 bits;
+      uint2 bits = make_uint2(~0u, ~0u);
       if (!whole && any_row) bits = key_bits(p.mask, (int64_t)w.k0 + first, n);
-      if (!warp_wait(smem_u32(&s_s_full), (uint32_t)j & 1u, abort_flag)) { dead = true; break; }
-      tc_fence_after();
+      if (!warp_wait(smem_u32(&s_s_full[b]), (uint32_t)(j >> 1) & 1u, abort_flag)) { dead = true; break; }
       if (any_row) {
-        const uint32_t at_s = lanes + S::kColS;
-        float most = whole ? row_max<true>(at_s, bits) : row_max<false>(at_s, bits);
-        most = most == -INFINITY ? most : most * p.scale_log2;       // scale >= 0; 0 times infinity is not wanted
-        const bool grown = most > top + kSlack;
-        float by = 1.f;
-        if (grown) {
-          by = exp2_approx(top - most);
-          top = most;
-          sum *= by;
+        tc_fence_after();
+        uint32_t v[kN], h[kN / 2];
+        tmem_ld64(lanes + S::kColS + kN * b, v);
+        tmem_ld_wait();
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < kN; ++i) v[i] = (i < 32 ? bits.x >> i : bits.y >> (i - 32)) & 1u ? v[i] : 0xff800000u;      // -infinity
         }
-        if (j > 0) {
-          if (!warp_wait(smem_u32(&s_o_done), (uint32_t)(j - 1) & 1u, abort_flag)) { dead = true; break; }
-          tc_fence_after();
-          if (__any_sync(0xffffffffu, grown)) {
+        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kN; i += 2) most[i / 2 & 3] = max3(most[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        most[0] = max3(max3(most[0], most[1], most[2]), most[3], most[3]);
+        most[0] = most[0] == -INFINITY ? most[0] : most[0] * p.scale_log2;         // scale > 0
+        const bool grown = most[0] > top + kSlack;
+        if (__any_sync(0xffffffffu, grown)) {
+          float by = 1.f;
+          if (grown) {
+            by = exp2_approx(top - most[0]);
+            top = most[0];
+            sum *= by;
+          }
+          if (j > 0) {
+            if (!warp_wait(smem_u32(&s_o_done[b ^ 1]), (uint32_t)((j - 1) >> 1) & 1u, abort_flag)) { dead = true; break; }
+            tc_fence_after();
+#pragma unroll 1
             for (int c = 0; c < p.d; c += 16) {
-              uint32_t v[16];
-              tmem_ld16(lanes + S::kColO + c, v);
+              uint32_t o[16];
+              tmem_ld16(lanes + S::kColO + c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * by);
-              tmem_st16(lanes + S::kColO + c, v);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+              tmem_st16(lanes + S::kColO + c, o);
             }
           }
         }
-        const float minus = top == -INFINITY ? 0.f : -top;
-        sum += whole ? row_exp<true, BF16>(at_s, lanes + S::kColP, bits, p.scale_log2, minus)
-                     : row_exp<false, BF16>(at_s, lanes + S::kColP, bits, p.scale_log2, minus);
+        // scores without a key: 2^(-inf); where all of the row's so far are, against 0
+        sum += row_exp<BF16>(v, h, p.scale_log2, top == -INFINITY ? 0.f : -top);
+        tmem_st32(lanes + S::kColS + kN * b, h);
         tmem_st_wait();
-      } else if (j > 0) {
-        if (!warp_wait(smem_u32(&s_o_done), (uint32_t)(j - 1) & 1u, abort_flag)) { dead = true; break; }
+        tc_fence_before();
       }
-      tc_fence_before();
       __syncwarp();
-      if (one) mbar_arrive(smem_u32(&s_p_full));
+      if (one) mbar_arrive(smem_u32(&s_p_full[b]));
     }
     // ======================= epilogue =======================
-    if (!dead && (tiles == 0 || warp_wait(smem_u32(&s_o_done), (uint32_t)(tiles - 1) & 1u, abort_flag))) {
+    if (!dead && (tiles == 0 || warp_wait(smem_u32(&s_o_done[(tiles - 1) & 1]), (uint32_t)((tiles - 1) >> 1) & 1u, abort_flag))) {
       tc_fence_after();
-      const int r = warp * 32 + lane;
-      const bool mine = r < rows, none = sum == 0.f;
-      const int i = w.tile * kM + min(r, rows - 1);
-      const int64_t at = (int64_t)(w.q0 + i / p.group) * p.hq + head * p.group + i % p.group;
+      const bool none = sum == 0.f;
+      const int64_t at = row_q * p.hq + row_h;
       const float by = none ? 0.f : 1.f / sum, lse = none ? INFINITY : top + log2f(sum);
       if (any_row) {
         for (int c = 0; c < p.d; c += 16) {
@@ -249,69 +236,62 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
       tc_fence_after();
       if (one) {
         const uint64_t k_desc = tile_desc(k_at + st * S::kTileBytes, 16u);
+        const uint32_t to = tmem + S::kColS + kN * (j & 1);
 #pragma unroll 1
         for (int s = 0; s < steps; ++s) {
-          const uint32_t on = (uint32_t)(s >> 2) * (kM * 128u / 16u) + (uint32_t)(s & 3) * 2u;      // in 16 bytes
-          umma_f16(tmem + S::kColS, q_desc + on, k_desc + on, idesc_s, s ? 1u : 0u);
+          const uint32_t in = (uint32_t)(s & 3) * 2u;                 // of a block, in 16 bytes
+          const uint64_t k_s = k_desc + (uint32_t)(s >> 2) * (kN * 8u) + in;
+          if (S::kQInTmem) umma_f16_ta(to, tmem + S::kColQ + 8 * s, k_s, idesc_s, s ? 1u : 0u);
+          else umma_f16(to, q_desc + (uint32_t)(s >> 2) * (kM * 8u) + in, k_s, idesc_s, s ? 1u : 0u);
         }
         umma_commit(smem_u32(&s_k_empty[st]));
-        umma_commit(smem_u32(&s_s_full));
+        umma_commit(smem_u32(&s_s_full[j & 1]));
       }
       __syncwarp();
       return true;
     };
     bool dead = tiles > 0 && !warp_wait(smem_u32(&s_q_full), 0u, abort_flag);
-    if (tiles > 0 && !dead) dead = !scores(0);
+    for (int j = 0; j < 2 && j < tiles && !dead; ++j) dead = !scores(j);
 #pragma unroll 1
     for (int j = 0; j < tiles && !dead; ++j) {
-      if (!warp_wait(smem_u32(&s_p_full), (uint32_t)j & 1u, abort_flag)) break;
-      tc_fence_after();
-      if (!S::kOverS && j + 1 < tiles && !scores(j + 1)) break;
-      const int st = j % S::kStages;
+      const int st = j % S::kStages, b = j & 1;
       if (!warp_wait(smem_u32(&s_v_full[st]), (uint32_t)(j / S::kStages) & 1u, abort_flag)) break;
+      if (!warp_wait(smem_u32(&s_p_full[b]), (uint32_t)(j >> 1) & 1u, abort_flag)) break;
       fence_proxy_async();
       tc_fence_after();
       if (one) {
-        const uint64_t v_desc = tile_desc(v_at + st * S::kTileBytes, kM * 128u);
+        const uint64_t v_desc = tile_desc(v_at + st * S::kTileBytes, kN * 128u);
 #pragma unroll
         for (int s = 0; s < kN / 16; ++s)
-          umma_f16_ta(tmem + S::kColO, tmem + S::kColP + 8 * s, v_desc + (uint64_t)(s * (2048 / 16)), idesc_o, j || s ? 1u : 0u);
+          umma_f16_ta(tmem + S::kColO, tmem + S::kColS + kN * b + 8 * s, v_desc + (uint64_t)(s * (2048 / 16)), idesc_o, j || s ? 1u : 0u);
         umma_commit(smem_u32(&s_v_empty[st]));
-        umma_commit(smem_u32(&s_o_done));
+        umma_commit(smem_u32(&s_o_done[b]));
       }
       __syncwarp();
-      if (S::kOverS && j + 1 < tiles) {       // S_j+1 goes where P_j is
-        if (!warp_wait(smem_u32(&s_o_done), (uint32_t)j & 1u, abort_flag)) break;
-        tc_fence_after();
-        if (!scores(j + 1)) break;
+      if (j + 2 < tiles) {                    // S_j+2 goes where P_j is
+        if (!warp_wait(smem_u32(&s_o_done[b]), (uint32_t)(j >> 1) & 1u, abort_flag)) break;
+        if (!scores(j + 2)) break;
       }
     }
   } else {
     // ======================= loads =======================
     const int t = tid - kLoadWarp * 32;
     const Pieces pc = pieces_of(p.d);
-    if (tiles > 0) {
-      load_rows<kM, kLoaders>(q_at, t, rows, p.d, pc, p.q, [&](int r) {
-        const int i = w.tile * kM + r;
-        return (const uint16_t*)p.q + (int64_t)(w.q0 + i / p.group) * p.q_row + (head * p.group + i % p.group) * p.q_head;
-      }, [](int) { return true; });
-      cp_async_arrive_noinc(smem_u32(&s_q_full));
-    }
     const uint8_t* mask = p.mask ? p.mask + w.k0 + keys.x : nullptr;
     const bool one = elect_one();
-    // 128 rows from key `first` of the part on: whole tiles by TMA, others row by row
+    // 64 rows from key `first` of the part on: whole tiles by TMA, others row by row
     auto bring = [&](uint32_t to, const TileMap& m, const void* x, int64_t row_stride, int64_t head_stride, int first, int n, uint32_t bar) {
       if (n == kN && mask == nullptr && m.usable) {
         if (one && warp == kLoadWarp) {
           mbar_arrive_expect_tx(bar, S::kTileBytes);
-          tma_tile<DP>(to, kM * 128u, m, head, w.k0 + keys.x + first, bar);
+          tma_tile<DP>(to, kN * 128u, m, head, w.k0 + keys.x + first, bar);
         } else if (one) {
           mbar_arrive(bar);
         }
         return;
       }
       const uint16_t* from = (const uint16_t*)x + (int64_t)(w.k0 + keys.x + first) * row_stride + head * head_stride;
-      load_rows<kM, kLoaders>(to, t, n, p.d, pc, x, [&](int r) { return from + r * row_stride; },
+      load_rows<kN, kLoaders>(to, t, n, p.d, pc, x, [&](int r) { return from + r * row_stride; },
                              [&](int r) { return mask == nullptr || __ldg(mask + first + r) != 0; });
       cp_async_arrive(bar);
       __syncwarp();
@@ -323,6 +303,15 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
       const uint32_t phase = ((uint32_t)(j / S::kStages) & 1u) ^ 1u;
       if (!warp_wait(smem_u32(&s_k_empty[st]), phase, abort_flag)) break;
       bring(k_at + st * S::kTileBytes, k_map, p.k, p.k_row, p.k_head, first, n, smem_u32(&s_k_full[st]));
+      if (!S::kQInTmem && j == 0) {           // behind the first keys, which take longer
+        load_rows<kM, kLoaders>(q_at, t, rows, p.d, pc, p.q, [&](int r) {
+          const int i = w.tile * kM + r;
+          return (const uint16_t*)p.q + (int64_t)(w.q0 + i / p.group) * p.q_row + (head * p.group + i % p.group) * p.q_head;
+        }, [](int) { return true; });
+        cp_async_arrive(smem_u32(&s_q_full));
+        __syncwarp();
+        if (one) mbar_arrive(smem_u32(&s_q_full));
+      }
       if (!warp_wait(smem_u32(&s_v_empty[st]), phase, abort_flag)) break;
       bring(v_at + st * S::kTileBytes, v_map, p.v, p.v_row, p.v_head, first, n, smem_u32(&s_v_full[st]));
     }

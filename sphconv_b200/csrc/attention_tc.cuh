@@ -51,6 +51,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+      "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
+      "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+      "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
                "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
@@ -185,17 +194,16 @@ __device__ __forceinline__ void store16_float(const uint32_t (&v)[16], float by,
   }
 }
 
-// Which of the 128 keys from `first` on, of `n`, are none: bit i of word w is key 32 w + i.  By whole warps.
-__device__ __forceinline__ uint4 key_bits(const uint8_t* mask, int64_t first, int n) {
+// Which of the 64 keys from `first` on, of `n`, are some: bit i of word w is key 32 w + i.  By whole warps.
+__device__ __forceinline__ uint2 key_bits(const uint8_t* mask, int64_t first, int n) {
   const int lane = threadIdx.x & 31;
-  uint32_t w[4];
+  uint32_t w[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const int r = 32 * i + lane;
-    const bool key = r < n && (mask == nullptr || __ldg(mask + first + r) != 0);
-    w[i] = __ballot_sync(0xffffffffu, key);
+    w[i] = __ballot_sync(0xffffffffu, r < n && (mask == nullptr || __ldg(mask + first + r) != 0));
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return make_uint2(w[0], w[1]);
 }
 
 // Host: a map of x [rows][heads][d] with strides in elements, for tiles of `tile` rows of a head, or (group > 1) of the rows of `group`

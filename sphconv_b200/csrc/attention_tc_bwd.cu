@@ -111,14 +111,8 @@ __global__ void __launch_bounds__(kThreadsTc, 2) backward_tc_kernel(const __grid
     for (int j = 0; j < tiles; ++j) {
       const int st = j % S::kStages, first = span.x + j * kC, n = min(kC, span.y - first);
       const bool whole = KEYS || (n == kC && p.mask == nullptr);
-      uint32_t bits[2] = {~0u, ~0u};
-      if (!whole && any_row) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int c = 32 * i + lane;
-          bits[i] = __ballot_sync(0xffffffffu, c < n && (p.mask == nullptr || __ldg(p.mask + (int64_t)w.k0 + first + c) != 0));
-        }
-      }
+      uint2 bits = make_uint2(~0u, ~0u);
+      if (!whole && any_row) bits = key_bits(p.mask, (int64_t)w.k0 + first, n);
       if (KEYS && !warp_wait(smem_u32(&s_stat_full[st]), (uint32_t)(j / S::kStages) & 1u, abort_flag)) { dead = true; break; }
       if (!warp_wait(smem_u32(&s_s_full), (uint32_t)j & 1u, abort_flag)) { dead = true; break; }
       tc_fence_after();
@@ -129,7 +123,7 @@ __global__ void __launch_bounds__(kThreadsTc, 2) backward_tc_kernel(const __grid
           for (int i = 0; i < 16; ++i) {
             const float l = KEYS ? s_lse[st][c + i] : lse, dl = KEYS ? s_delta[st][c + i] : delta;
             float x = exp2_approx(fmaf(__uint_as_float(v[i]), p.scale_log2, BF16 ? -l : kShiftP - l));
-            if (!whole) x = bits[c >> 5] >> ((c & 31) + i) & 1u ? x : 0.f;
+            if (!whole) x = (c < 32 ? bits.x : bits.y) >> ((c & 31) + i) & 1u ? x : 0.f;
             v[i] = __float_as_uint(x);
             u[i] = __float_as_uint(x * (__uint_as_float(u[i]) - dl));
           }
