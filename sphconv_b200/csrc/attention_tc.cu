@@ -5,13 +5,15 @@
 //   O [128 x d] += P V      A = P in TMEM, B = the same keys' values, MN-major in shared memory; O stays in TMEM
 //
 // A block has one tile of queries (heads that share a key head are rows of it) and walks a scan's keys, or a part of them.  Warps 0-3
-// do the softmax, a thread a row; warp 4 issues the MMAs; warps 5-7 bring keys and values: whole tiles by TMA, tiles with keys
-// missing (the scan's end, a mask) row by row with cp.async, which fills in zeros.  S has two places, so that the next scores are there
-// when a row's softmax ends, and two blocks share an SM.
+// do the softmax, a thread a row; warps 4 and 5 issue the MMAs of S and of O (one warp for both took 1100 cycles a tile, most of
+// them waits that were over); warps 6 and 7 bring keys and values: whole tiles by TMA, tiles with keys missing (the scan's end, a
+// mask) row by row with cp.async, which fills in zeros.  S has two places, so that the next scores are there when a row's softmax
+// ends, and two blocks share an SM.
 //   Queries of up to 64 channels are an operand in TMEM: from shared memory, A and B of an MMA of 64 columns take 48 cycles to
 // read and 32 to multiply.  128 channels leave no columns for them.
-//   The running maximum follows S only when it has grown by more than 2^8: O is read, scaled and written again in those tiles alone,
-// P stays within 2^8 and a row's sum within float32.
+//   P is taken against the row's maximum in its first tile, without looking for another one: what shows that the maximum has grown
+// too far is the sum of P over a tile, above 2^12.  Only then it is searched, O is read, scaled and written again, and P made anew.
+// Any P is below 2^12 then, which is no matter to a floating-point type.
 #include <algorithm>
 
 #include "attention_tc.cuh"
@@ -22,10 +24,10 @@ namespace attn {
 namespace {
 
 constexpr int kN = 64;                        // keys of a tile
-constexpr int kSoftmaxWarps = 4, kMmaWarp = 4, kLoadWarp = 5, kLoadWarps = 3;
+constexpr int kSoftmaxWarps = 4, kScoreWarp = 4, kOutWarp = 5, kLoadWarp = 6, kLoadWarps = 2;
 constexpr int kThreadsTc = (kLoadWarp + kLoadWarps) * 32;
 constexpr int kLoaders = kLoadWarps * 32;
-constexpr float kSlack = 8.f;                 // log2 of how far a row's maximum may be above the one that P is taken against
+constexpr float kMostSum = 4096.f;            // of a row's P over a tile: above it the row's maximum is taken anew
 
 // DP: channels of a tile's rows, 64 or 128.
 template <int DP>
@@ -51,6 +53,13 @@ __device__ __forceinline__ float row_exp(const uint32_t (&s)[kN], uint32_t (&h)[
   }
   const float2 t = add2(sum[0], sum[1]);
   return t.x + t.y;
+}
+
+__device__ __forceinline__ float row_max(const uint32_t (&s)[kN]) {
+  float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < kN; i += 2) most[i / 2 & 3] = max3(most[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+  return max3(max3(most[0], most[1], most[2]), most[3], most[3]);
 }
 
 template <int DP, bool BF16>
@@ -106,7 +115,7 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
   const int2 keys = split_rows(w.nk, split, p.splits, kN);
   const int tiles = (keys.y - keys.x + kN - 1) / kN;
   const int rows = min(kM, w.nq * p.group - w.tile * kM);
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     tmem_alloc(smem_u32(&s_tmem), S::kCols);
     tmem_relinquish();
   }
@@ -159,19 +168,18 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
 #pragma unroll
           for (int i = 0; i < kN; ++i) v[i] = (i < 32 ? bits.x >> i : bits.y >> (i - 32)) & 1u ? v[i] : 0xff800000u;      // -infinity
         }
-        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < kN; i += 2) most[i / 2 & 3] = max3(most[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-        most[0] = max3(max3(most[0], most[1], most[2]), most[3], most[3]);
-        most[0] = most[0] == -INFINITY ? most[0] : most[0] * p.scale_log2;         // scale > 0
-        const bool grown = most[0] > top + kSlack;
-        if (__any_sync(0xffffffffu, grown)) {
+        // scores without a key: 2^(-inf); where all of the row's so far are, against 0
+        float add = row_exp<BF16>(v, h, p.scale_log2, top == -INFINITY ? 0.f : -top);
+        const bool anew = top == -INFINITY || !(add <= kMostSum);
+        if (__any_sync(0xffffffffu, anew)) {
           float by = 1.f;
-          if (grown) {
-            by = exp2_approx(top - most[0]);
-            top = most[0];
+          const float most = row_max(v) * p.scale_log2;               // scale > 0
+          if (anew && most > top) {
+            by = exp2_approx(top - most);
+            top = most;
             sum *= by;
           }
+          add = row_exp<BF16>(v, h, p.scale_log2, top == -INFINITY ? 0.f : -top);
           if (j > 0) {
             if (!warp_wait(smem_u32(&s_o_done[b ^ 1]), (uint32_t)((j - 1) >> 1) & 1u, abort_flag)) { dead = true; break; }
             tc_fence_after();
@@ -186,8 +194,7 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
             }
           }
         }
-        // scores without a key: 2^(-inf); where all of the row's so far are, against 0
-        sum += row_exp<BF16>(v, h, p.scale_log2, top == -INFINITY ? 0.f : -top);
+        sum += add;
         tmem_st32(lanes + S::kColS + kN * b, h);
         tmem_st_wait();
         tc_fence_before();
@@ -221,57 +228,56 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
         else if (mine && p.lse) p.lse[at] = lse;
       }
     }
-  } else if (warp == kMmaWarp) {
-    // ======================= MMA issuer =======================
+  } else if (warp == kScoreWarp) {
+    // ======================= MMAs of S =======================
     const bool one = elect_one();
-    const uint32_t fmt = BF16 ? 1u : 0u;
-    const uint32_t idesc_s = make_idesc(1u, fmt, 0u, 0u, kM, kN);
-    const uint32_t idesc_o = make_idesc(1u, fmt, 0u, 1u, kM, (uint32_t)((p.d + 15) / 16 * 16));
+    const uint32_t idesc = make_idesc(1u, BF16 ? 1u : 0u, 0u, 0u, kM, kN);
     const int steps = (p.d + 15) / 16;        // of 16 channels
-    const uint64_t q_desc = tile_desc(q_at, 16u);
-    auto scores = [&](int j) {                // S_j; false: a wait ran out
-      const int st = j % S::kStages;
-      if (!warp_wait(smem_u32(&s_k_full[st]), (uint32_t)(j / S::kStages) & 1u, abort_flag)) return false;
-      fence_proxy_async();
-      tc_fence_after();
-      if (one) {
-        const uint64_t k_desc = tile_desc(k_at + st * S::kTileBytes, 16u);
-        const uint32_t to = tmem + S::kColS + kN * (j & 1);
-#pragma unroll 1
-        for (int s = 0; s < steps; ++s) {
-          const uint32_t in = (uint32_t)(s & 3) * 2u;                 // of a block, in 16 bytes
-          const uint64_t k_s = k_desc + (uint32_t)(s >> 2) * (kN * 8u) + in;
-          if (S::kQInTmem) umma_f16_ta(to, tmem + S::kColQ + 8 * s, k_s, idesc_s, s ? 1u : 0u);
-          else umma_f16(to, q_desc + (uint32_t)(s >> 2) * (kM * 8u) + in, k_s, idesc_s, s ? 1u : 0u);
-        }
-        umma_commit(smem_u32(&s_k_empty[st]));
-        umma_commit(smem_u32(&s_s_full[j & 1]));
-      }
-      __syncwarp();
-      return true;
-    };
+    const uint64_t q_desc = tile_desc(q_at, 16u), k_desc0 = tile_desc(k_at, 16u);
     bool dead = tiles > 0 && !warp_wait(smem_u32(&s_q_full), 0u, abort_flag);
-    for (int j = 0; j < 2 && j < tiles && !dead; ++j) dead = !scores(j);
 #pragma unroll 1
     for (int j = 0; j < tiles && !dead; ++j) {
+      const int st = j % S::kStages, b = j & 1;
+      if (!warp_wait(smem_u32(&s_k_full[st]), (uint32_t)(j / S::kStages) & 1u, abort_flag)) break;
+      if (j >= 2 && !warp_wait(smem_u32(&s_o_done[b]), (uint32_t)((j - 2) >> 1) & 1u, abort_flag)) break;      // S goes where P was
+      fence_proxy_async();
+      tc_fence_after();
+      const uint64_t k_desc = k_desc0 + (uint32_t)st * (S::kTileBytes / 16u);
+      const uint32_t to = tmem + S::kColS + kN * b;
+      if (one) {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+          if (s >= steps) break;
+          const uint64_t k_s = k_desc + (uint32_t)((s >> 2) * (kN * 8) + (s & 3) * 2);
+          if (S::kQInTmem) umma_f16_ta(to, tmem + S::kColQ + 8 * s, k_s, idesc, s ? 1u : 0u);
+          else umma_f16(to, q_desc + (uint32_t)((s >> 2) * (kM * 8) + (s & 3) * 2), k_s, idesc, s ? 1u : 0u);
+        }
+        umma_commit(smem_u32(&s_s_full[b]));
+        umma_commit(smem_u32(&s_k_empty[st]));
+      }
+      __syncwarp();
+    }
+  } else if (warp == kOutWarp) {
+    // ======================= MMAs of O =======================
+    const bool one = elect_one();
+    const uint32_t idesc = make_idesc(1u, BF16 ? 1u : 0u, 0u, 1u, kM, (uint32_t)((p.d + 15) / 16 * 16));
+    const uint64_t v_desc0 = tile_desc(v_at, kN * 128u);
+#pragma unroll 1
+    for (int j = 0; j < tiles; ++j) {
       const int st = j % S::kStages, b = j & 1;
       if (!warp_wait(smem_u32(&s_v_full[st]), (uint32_t)(j / S::kStages) & 1u, abort_flag)) break;
       if (!warp_wait(smem_u32(&s_p_full[b]), (uint32_t)(j >> 1) & 1u, abort_flag)) break;
       fence_proxy_async();
       tc_fence_after();
+      const uint64_t v_desc = v_desc0 + (uint32_t)st * (S::kTileBytes / 16u);
       if (one) {
-        const uint64_t v_desc = tile_desc(v_at + st * S::kTileBytes, kN * 128u);
 #pragma unroll
         for (int s = 0; s < kN / 16; ++s)
-          umma_f16_ta(tmem + S::kColO, tmem + S::kColS + kN * b + 8 * s, v_desc + (uint64_t)(s * (2048 / 16)), idesc_o, j || s ? 1u : 0u);
-        umma_commit(smem_u32(&s_v_empty[st]));
+          umma_f16_ta(tmem + S::kColO, tmem + S::kColS + kN * b + 8 * s, v_desc + (uint64_t)(s * (2048 / 16)), idesc, j || s ? 1u : 0u);
         umma_commit(smem_u32(&s_o_done[b]));
+        umma_commit(smem_u32(&s_v_empty[st]));
       }
       __syncwarp();
-      if (j + 2 < tiles) {                    // S_j+2 goes where P_j is
-        if (!warp_wait(smem_u32(&s_o_done[b]), (uint32_t)(j >> 1) & 1u, abort_flag)) break;
-        if (!scores(j + 2)) break;
-      }
     }
   } else {
     // ======================= loads =======================
@@ -323,7 +329,7 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
     wind_down(abort_flag, p.status);
     __syncthreads();
   }
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, S::kCols);
   }
