@@ -444,17 +444,23 @@ namespace {
 bool on_tensor_cores(const sph_attention& a, const Params& p) {
   return (a.dtype == SPH_F16 || a.dtype == SPH_BF16) && p.vec && p.scale > 0.f;
 }
-constexpr int kTcTile = 128;
+constexpr int kTcTile = 128, kTcStep = 64;
 
 int padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 int forward_smem(int dp) { return (3 * kTile * (dp + 4) + kTile * kScorePitch) * 4; }
 int backward_smem(int dp, bool keys) { return (4 * kTile * (dp + 4) + (keys ? 2 : 1) * kTile * kScorePitch) * 4; }
 
-// Parts that fill the GPU: as many as blocks are missing, none shorter than `least` rows on average.
-int splits_for(int64_t blocks, int64_t room, int64_t rows, int B, int64_t least) {
-  const int64_t mean = rows / std::max(B, 1);
-  const int64_t most = std::max<int64_t>(1, mean / least);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({room / std::max<int64_t>(blocks, 1), most, 64}));
+// Parts that the walk of `blocks` blocks over `tiles` tiles each is split into, where `slots` blocks run at a time: what takes the
+// fewest rounds of tiles, with kStart tiles' time for a block to start and end, and that of writing and reading parts of `values`.
+int splits_for(int64_t blocks, int64_t slots, int64_t tiles, int64_t values) {
+  constexpr int64_t kStart = 8, kMost = 64, kValues = 500000;      // values of a part in a tile's time, 0.7 us
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int64_t s = 1; s <= std::min(kMost, std::max<int64_t>(1, tiles / 2)); ++s) {
+    const int64_t cost = div_up64(blocks * s, slots) * (div_up64(tiles, s) + kStart) + (s > 1 ? 4 + s * values / kValues : 0);
+    if (cost < least) { least = cost; best = (int)s; }
+  }
+  return best;
 }
 
 struct Plan {
@@ -470,22 +476,21 @@ Plan plan_of(const sph_attention& a, const Params& params, int sms) {
   p.fwd_blocks = p.dq_blocks = (int)(q_tiles * a.k_heads);
   p.dkv_blocks = (int)(k_tiles * a.k_heads);
   // tiles that there really are, if scans are of like length
-  const int64_t q_real = std::max<int64_t>(1, div_up64(a.n_q * group, (int64_t)kTile * a.B)) * a.B * a.k_heads;
-  const int64_t k_real = std::max<int64_t>(1, div_up64(a.n_k, (int64_t)kTile * a.B)) * a.B * a.k_heads;
-  p.fwd_splits = splits_for(q_real, sms * per_sm(forward_smem(dp)), a.n_k, a.B, 2 * kTile);
-  p.dq_splits = splits_for(q_real, sms * per_sm(backward_smem(dp, false)), a.n_k, a.B, 2 * kTile);
+  const int64_t B = std::max(a.B, 1);
+  auto real = [&](int64_t rows, int64_t size) { return std::max<int64_t>(1, div_up64(rows, size * B)) * B * a.k_heads; };
+  auto walk = [&](int64_t rows, int64_t size) { return div_up64(rows, B * size); };
+  const int64_t q_rows = a.n_q * group, q_values = a.n_q * a.q_heads * a.channels, k_values = 2 * a.n_k * a.k_heads * a.channels;
   if (on_tensor_cores(a, params)) {
-    p.fwd_blocks = most_tiles(a.n_q * group, kTcTile, a.B) * a.k_heads;
-    const int64_t real = std::max<int64_t>(1, div_up64(a.n_q * group, (int64_t)kTcTile * a.B)) * a.B * a.k_heads;
-    p.fwd_splits = splits_for(real, 2 * sms, a.n_k, a.B, 2 * kTcTile);
-    p.dq_blocks = p.fwd_blocks;
+    p.fwd_blocks = p.dq_blocks = most_tiles(q_rows, kTcTile, a.B) * a.k_heads;
     p.dkv_blocks = most_tiles(a.n_k, kTcTile, a.B) * a.k_heads;
-    const int64_t k_tiles_real = std::max<int64_t>(1, div_up64(a.n_k, (int64_t)kTcTile * a.B)) * a.B * a.k_heads;
-    p.dq_splits = splits_for(real, attention_backward_tc_blocks(a.channels, false) * sms, a.n_k, a.B, 2 * kTcTile);
-    p.dkv_splits = splits_for(k_tiles_real, attention_backward_tc_blocks(a.channels, true) * sms, a.n_q * group, a.B, 2 * kTcTile);
+    p.fwd_splits = splits_for(real(q_rows, kTcTile), 2 * sms, walk(a.n_k, kTcStep), q_values);
+    p.dq_splits = splits_for(real(q_rows, kTcTile), attention_backward_tc_blocks(a.channels, false) * sms, walk(a.n_k, kTcStep), q_values);
+    p.dkv_splits = splits_for(real(a.n_k, kTcTile), attention_backward_tc_blocks(a.channels, true) * sms, walk(q_rows, kTcStep), k_values);
     return p;
   }
-  p.dkv_splits = splits_for(k_real, sms * per_sm(backward_smem(dp, true)), a.n_q * group, a.B, 2 * kTile);
+  p.fwd_splits = splits_for(real(q_rows, kTile), sms * per_sm(forward_smem(dp)), walk(a.n_k, kTile), q_values);
+  p.dq_splits = splits_for(real(q_rows, kTile), sms * per_sm(backward_smem(dp, false)), walk(a.n_k, kTile), q_values);
+  p.dkv_splits = splits_for(real(a.n_k, kTile), sms * per_sm(backward_smem(dp, true)), walk(q_rows, kTile), k_values);
   return p;
 }
 

@@ -4,16 +4,17 @@
 //   P = 2^(scale log2 e S - top) in the rows' type, written over S by the thread that has the row
 //   O [128 x d] += P V      A = P in TMEM, B = the same keys' values, MN-major in shared memory; O stays in TMEM
 //
-// A block has one tile of queries (heads that share a key head are rows of it) and walks a scan's keys, or a part of them.  Warps 0-3
-// do the softmax, a thread a row; warps 4 and 5 issue the MMAs of S and of O (one warp for both took 1100 cycles a tile, most of
-// them waits that were over); warps 6 and 7 bring keys and values: whole tiles by TMA, tiles with keys missing (the scan's end, a
-// mask) row by row with cp.async, which fills in zeros.  S has two places, so that the next scores are there when a row's softmax
-// ends, and two blocks share an SM.
-//   Queries of up to 64 channels are an operand in TMEM: from shared memory, A and B of an MMA of 64 columns take 48 cycles to
-// read and 32 to multiply.  128 channels leave no columns for them.
+// A block has one tile of queries (heads that share a key head are rows of it) and walks a scan's keys, or a part of them; two blocks
+// share an SM.  Keys and values come by TMA where a tile has all of its rows, and row by row with cp.async, which fills in zeros, where
+// keys are missing (the scan's end, a mask).
 //   P is taken against the row's maximum in its first tile, without looking for another one: what shows that the maximum has grown
 // too far is the sum of P over a tile, above 2^12.  Only then it is searched, O is read, scaled and written again, and P made anew.
 // Any P is below 2^12 then, which is no matter to a floating-point type.
+//
+// Warps 0-3 do the softmax, a thread a row; warps 4 and 5 issue the MMAs of S and of O (one warp for both took 1100 cycles a tile, most of
+// them waits that were over); warps 6 and 7 load.  S has two places, so that the next scores are there when a row's softmax ends.
+// Queries of up to 64 channels are an operand in TMEM: from shared memory, A and B of an MMA of 64 columns take 48 cycles to read and 32
+// to multiply.  128 channels leave no columns for them.
 #include <algorithm>
 
 #include "attention_tc.cuh"
@@ -24,10 +25,167 @@ namespace attn {
 namespace {
 
 constexpr int kN = 64;                        // keys of a tile
-constexpr int kSoftmaxWarps = 4, kScoreWarp = 4, kOutWarp = 5, kLoadWarp = 6, kLoadWarps = 2;
-constexpr int kThreadsTc = (kLoadWarp + kLoadWarps) * 32;
-constexpr int kLoaders = kLoadWarps * 32;
 constexpr float kMostSum = 4096.f;            // of a row's P over a tile: above it the row's maximum is taken anew
+
+// P = 2^(scale s + minus) of N scores in the rows' type, and the sum of P before rounding.
+template <bool BF16, int N>
+__device__ __forceinline__ float row_exp(const uint32_t (&s)[N], uint32_t* h, float scale, float minus) {
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  const float2 scale2 = make_float2(scale, scale), minus2 = make_float2(minus, minus);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float2 e = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, minus2);
+    const float2 y = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+    sum[i / 2 & 1] = add2(sum[i / 2 & 1], y);
+    h[i / 2] = pack2<BF16>(y.x, y.y);
+  }
+  const float2 t = add2(sum[0], sum[1]);
+  return t.x + t.y;
+}
+
+template <int N>
+__device__ __forceinline__ float row_max(const uint32_t (&s)[N]) {
+  float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < N; i += 2) most[i / 2 & 3] = max3(most[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+  return max3(max3(most[0], most[1], most[2]), most[3], most[3]);
+}
+
+// Scores without a key are -infinity.
+template <int N>
+__device__ __forceinline__ void leave_out(uint32_t (&s)[N], uint32_t keys) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] = keys >> i & 1u ? s[i] : 0xff800000u;
+}
+
+// A row of O in TMEM times `by`.
+__device__ __forceinline__ void scale_row(uint32_t at, int d, float by) {
+#pragma unroll 1
+  for (int c = 0; c < d; c += 16) {
+    uint32_t o[16];
+    tmem_ld16(at + c, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+    tmem_st16(at + c, o);
+  }
+}
+
+// Scans that are not in order, or not within the rows, are reported by the first block.
+__device__ __forceinline__ void report_scans(const Params& p) {
+  if (blockIdx.x != 0 || p.status == nullptr) return;
+  bool bad = false;
+  for (int b = threadIdx.x; b <= p.B; b += blockDim.x) {
+    const int q = __ldg(p.q_ptr + b), k = __ldg(p.k_ptr + b);
+    bad |= q < 0 || q > p.n_q || k < 0 || k > p.n_k;
+    if (b < p.B) bad |= q > __ldg(p.q_ptr + b + 1) || k > __ldg(p.k_ptr + b + 1);
+  }
+  if (bad) atomicOr(p.status, SPH_STATUS_BAD_INDEX);
+}
+
+// What of the work is a block's: a tile of queries of one key head against a part of the keys.
+struct Part {
+  int split, head, item;
+  __device__ __forceinline__ explicit Part(const Params& p) {
+    split = blockIdx.x % p.splits;
+    head = blockIdx.x / p.splits % p.hkv;
+    item = blockIdx.x / p.splits / p.hkv;
+  }
+};
+
+// Row r of a block's tile: of which query and head it is.
+struct Row {
+  int64_t q;
+  int h;
+  __device__ __forceinline__ Row(const Params& p, const Work& w, int head, int r) {
+    const int i = w.tile * kM + r;
+    q = w.q0 + i / p.group;
+    h = head * p.group + i % p.group;
+  }
+  __device__ __forceinline__ const uint16_t* query(const Params& p) const { return (const uint16_t*)p.q + q * p.q_row + h * p.q_head; }
+  __device__ __forceinline__ int64_t out(const Params& p) const { return q * p.hq + h; }
+};
+
+// The query rows of a tile to shared memory; the warp's arrival included.
+template <int THREADS>
+__device__ __forceinline__ void load_queries(uint32_t to, int t, int rows, const Params& p, const Work& w, int head, uint32_t bar, bool one) {
+  load_rows<kM, THREADS>(to, t, rows, p.d, pieces_of(p.d), p.q, [&](int r) { return Row(p, w, head, r).query(p); }, [](int) { return true; });
+  cp_async_arrive(bar);
+  __syncwarp();
+  if (one) mbar_arrive(bar);
+}
+
+// Whether tile j of a part's keys or values comes by TMA: all of its rows are there.
+__device__ __forceinline__ bool by_tma(const Params& p, const TileMap& m, const int2& keys, int j) {
+  return m.usable && p.mask == nullptr && keys.y - keys.x - j * kN >= kN;
+}
+
+// Tile j of a part's keys, or values, to shared memory, by all loading threads; `first` of their warps issues the TMA loads.
+template <int DP, int THREADS>
+__device__ __forceinline__ void load_keys(uint32_t to, int t, bool first, bool one, const Params& p, const TileMap& m, const void* x,
+                                          int64_t row_stride, int64_t head_stride, const Work& w, const int2& keys, int head, int j,
+                                          uint32_t bar) {
+  const int at = w.k0 + keys.x + j * kN;
+  if (by_tma(p, m, keys, j)) {
+    if (one && first) {
+      mbar_arrive_expect_tx(bar, DP * kN * 2u);
+      tma_tile<DP>(to, kN * 128u, m, head, at, bar);
+    } else if (one) {
+      mbar_arrive(bar);
+    }
+    return;
+  }
+  const uint16_t* from = (const uint16_t*)x + (int64_t)at * row_stride + head * head_stride;
+  load_rows<kN, THREADS>(to, t, keys.y - keys.x - j * kN, p.d, pieces_of(p.d), x, [&](int r) { return from + r * row_stride; },
+                        [&](int r) { return p.mask == nullptr || __ldg(p.mask + at + r) != 0; });
+  cp_async_arrive(bar);
+  __syncwarp();
+  if (one) mbar_arrive(bar);
+}
+
+// S = Q K^T of one tile; by one thread.
+template <int DP, bool Q_IN_TMEM>
+__device__ __forceinline__ void issue_scores(uint32_t to, uint32_t q_tmem, uint64_t q_desc, uint64_t k_desc, uint32_t idesc, int steps) {
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    if (s >= steps) break;
+    const int in = (s & 3) * 2, block = s >> 2;                       // of a block of 64 channels, in 16 bytes
+    const uint64_t k_s = k_desc + (uint32_t)(block * kN * 8 + in);
+    if (Q_IN_TMEM) umma_f16_ta(to, q_tmem + 8 * s, k_s, idesc, s ? 1u : 0u);
+    else umma_f16(to, q_desc + (uint32_t)(block * kM * 8 + in), k_s, idesc, s ? 1u : 0u);
+  }
+}
+// O += P V of one tile.
+__device__ __forceinline__ void issue_out(uint32_t to, uint32_t p_at, uint64_t v_desc, uint32_t idesc, bool first) {
+#pragma unroll
+  for (int s = 0; s < kN / 16; ++s) umma_f16_ta(to, p_at + 8 * s, v_desc + (uint64_t)(s * (2048 / 16)), idesc, !first || s ? 1u : 0u);
+}
+
+// A row's part of the result, from its accumulator at TMEM `at_o`.
+template <bool BF16>
+__device__ __forceinline__ void store_out(const Params& p, const Work& w, const Part& part, uint32_t at_o, int r, int rows, float top, float sum) {
+  const bool none = sum == 0.f, mine = r < rows;
+  const int64_t at = Row(p, w, part.head, min(r, rows - 1)).out(p), part_at = (int64_t)part.split * p.n_q * p.hq + at;
+  const float by = none ? 0.f : 1.f / sum, lse = none ? INFINITY : top + log2f(sum);
+#pragma unroll 1
+  for (int c = 0; c < p.d; c += 16) {
+    uint32_t v[16];
+    tmem_ld16(at_o + c, v);
+    tmem_ld_wait();
+    if (none) {                               // no keys: what O holds is not looked at
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = 0u;
+    }
+    if (!mine) continue;
+    if (p.splits > 1) store16_float(v, by, p.part + part_at * p.d + c, p.d - c);
+    else store16<BF16>(v, by, (uint16_t*)p.out + at * p.d + c, p.d - c);
+  }
+  if (mine && p.splits > 1) p.part_lse[part_at] = lse;
+  else if (mine && p.lse) p.lse[at] = lse;
+}
+
+constexpr int kScoreWarp = 4, kOutWarp = 5, kLoadWarp = 6, kLoadWarps = 2;
+constexpr int kThreadsTc = (kLoadWarp + kLoadWarps) * 32, kLoaders = kLoadWarps * 32;
 
 // DP: channels of a tile's rows, 64 or 128.
 template <int DP>
@@ -39,35 +197,14 @@ struct Shape {
   static constexpr int kSmem = 1024 + (int)kQBytes + 2 * kStages * (int)kTileBytes;
 };
 
-// P = 2^(scale s + minus) of 64 scores in the rows' type, and the sum of P before rounding.
-template <bool BF16>
-__device__ __forceinline__ float row_exp(const uint32_t (&s)[kN], uint32_t (&h)[kN / 2], float scale, float minus) {
-  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-  const float2 scale2 = make_float2(scale, scale), minus2 = make_float2(minus, minus);
-#pragma unroll
-  for (int i = 0; i < kN; i += 2) {
-    const float2 e = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, minus2);
-    const float2 y = make_float2(exp2_approx(e.x), exp2_approx(e.y));
-    sum[i / 2 & 1] = add2(sum[i / 2 & 1], y);
-    h[i / 2] = pack2<BF16>(y.x, y.y);
-  }
-  const float2 t = add2(sum[0], sum[1]);
-  return t.x + t.y;
-}
-
-__device__ __forceinline__ float row_max(const uint32_t (&s)[kN]) {
-  float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int i = 0; i < kN; i += 2) most[i / 2 & 3] = max3(most[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-  return max3(max3(most[0], most[1], most[2]), most[3], most[3]);
-}
-
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kThreadsTc, 2)
 forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ TileMap k_map, const __grid_constant__ TileMap v_map) {
   using S = Shape<DP>;
+  constexpr int kStages = S::kStages;
+  constexpr uint32_t kTileBytes = S::kTileBytes, kColS = S::kColS, kColO = S::kColO;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t s_q_full, s_k_full[S::kStages], s_k_empty[S::kStages], s_v_full[S::kStages], s_v_empty[S::kStages];
+  __shared__ __align__(8) uint64_t s_q_full, s_k_full[kStages], s_k_empty[kStages], s_v_full[kStages], s_v_empty[kStages];
   __shared__ __align__(8) uint64_t s_s_full[2], s_p_full[2], s_o_done[2];       // of even and odd tiles
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
@@ -75,14 +212,13 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = (int)uniform((uint32_t)tid >> 5);
-  const int split = blockIdx.x % p.splits, rest = blockIdx.x / p.splits;
-  const int head = rest % p.hkv, item = rest / p.hkv;
+  const Part part(p);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t q_at = base, k_at = base + S::kQBytes, v_at = k_at + S::kStages * S::kTileBytes;
+  const uint32_t q_at = base, k_at = base + S::kQBytes, v_at = k_at + kStages * kTileBytes;
   if (tid == 0) {
     s_abort = 0;
-    mbar_init(smem_u32(&s_q_full), S::kQInTmem ? kSoftmaxWarps : kLoadWarps);
-    for (int i = 0; i < S::kStages; ++i) {
+    mbar_init(smem_u32(&s_q_full), S::kQInTmem ? kScoreWarp : kLoadWarps);
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(&s_k_full[i]), kLoadWarps);
       mbar_init(smem_u32(&s_v_full[i]), kLoadWarps);
       mbar_init(smem_u32(&s_k_empty[i]), 1);
@@ -90,29 +226,21 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&s_s_full[i]), 1);
-      mbar_init(smem_u32(&s_p_full[i]), kSoftmaxWarps);
+      mbar_init(smem_u32(&s_p_full[i]), 4);
       mbar_init(smem_u32(&s_o_done[i]), 1);
     }
     mbar_init_fence();
   }
   after_previous<false>();
-  if (blockIdx.x == 0 && p.status != nullptr) {            // scans that are not in order, or not within the rows
-    bool bad = false;
-    for (int b = tid; b <= p.B; b += kThreadsTc) {
-      const int q = __ldg(p.q_ptr + b), k = __ldg(p.k_ptr + b);
-      bad |= q < 0 || q > p.n_q || k < 0 || k > p.n_k;
-      if (b < p.B) bad |= q > __ldg(p.q_ptr + b + 1) || k > __ldg(p.k_ptr + b + 1);
-    }
-    if (bad) atomicOr(p.status, SPH_STATUS_BAD_INDEX);
-  }
+  report_scans(p);
   if (warp == 0) {
-    const Work w = find_work<true>(p, item, kM);
+    const Work w = find_work<true>(p, part.item, kM);
     if (lane == 0) s_work = w;
   }
   __syncthreads();
   const Work w = s_work;
   if (w.scan < 0) return;
-  const int2 keys = split_rows(w.nk, split, p.splits, kN);
+  const int2 keys = split_rows(w.nk, part.split, p.splits, kN);
   const int tiles = (keys.y - keys.x + kN - 1) / kN;
   const int rows = min(kM, w.nq * p.group - w.tile * kM);
   if (warp == kScoreWarp) {
@@ -125,23 +253,18 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
   const uint32_t tmem = uniform(s_tmem);
   volatile int* abort_flag = &s_abort;
 
-  if (warp < kSoftmaxWarps) {
+  if (warp < kScoreWarp) {
     // ======================= softmax: thread = row =======================
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
     const bool any_row = warp * 32 < rows;    // else this warp's lanes hold nothing that is read
     const bool one = elect_one();
-    const int r = warp * 32 + lane;
-    const bool mine = r < rows;
-    const int row_i = w.tile * kM + min(r, rows - 1);
-    const int64_t row_q = w.q0 + row_i / p.group;
-    const int row_h = head * p.group + row_i % p.group;
     if (S::kQInTmem && tiles > 0) {
-      const uint4* from = (const uint4*)((const uint16_t*)p.q + row_q * p.q_row + row_h * p.q_head);
-      const int pieces = p.d / 8;
+      const int r = warp * 32 + lane, pieces = p.d / 8;
+      const uint4* from = (const uint4*)Row(p, w, part.head, min(r, rows - 1)).query(p);
       uint32_t v[32];
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        const uint4 x = mine && c < pieces ? __ldg(from + c) : make_uint4(0u, 0u, 0u, 0u);
+        const uint4 x = r < rows && c < pieces ? __ldg(from + c) : make_uint4(0u, 0u, 0u, 0u);
         v[4 * c] = x.x; v[4 * c + 1] = x.y; v[4 * c + 2] = x.z; v[4 * c + 3] = x.w;
       }
       tmem_st32(lanes + S::kColQ, v);
@@ -161,165 +284,102 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
       if (!warp_wait(smem_u32(&s_s_full[b]), (uint32_t)(j >> 1) & 1u, abort_flag)) { dead = true; break; }
       if (any_row) {
         tc_fence_after();
-        uint32_t v[kN], h[kN / 2];
-        tmem_ld64(lanes + S::kColS + kN * b, v);
+        uint32_t v[2][kN / 2], h[kN / 2];
+        tmem_ld32(lanes + kColS + kN * b, v[0]);
+        tmem_ld32(lanes + kColS + kN * b + 32, v[1]);
         tmem_ld_wait();
         if (!whole) {
-#pragma unroll
-          for (int i = 0; i < kN; ++i) v[i] = (i < 32 ? bits.x >> i : bits.y >> (i - 32)) & 1u ? v[i] : 0xff800000u;      // -infinity
+          leave_out(v[0], bits.x);
+          leave_out(v[1], bits.y);
         }
-        // scores without a key: 2^(-inf); where all of the row's so far are, against 0
-        float add = row_exp<BF16>(v, h, p.scale_log2, top == -INFINITY ? 0.f : -top);
+        auto exps = [&]() {                   // where all of the row's scores so far are -infinity, against 0
+          const float minus = top == -INFINITY ? 0.f : -top;
+          return row_exp<BF16>(v[0], h, p.scale_log2, minus) + row_exp<BF16>(v[1], h + 16, p.scale_log2, minus);
+        };
+        float add = exps();
         const bool anew = top == -INFINITY || !(add <= kMostSum);
         if (__any_sync(0xffffffffu, anew)) {
           float by = 1.f;
-          const float most = row_max(v) * p.scale_log2;               // scale > 0
+          const float most = fmaxf(row_max(v[0]), row_max(v[1])) * p.scale_log2;        // scale > 0
           if (anew && most > top) {
             by = exp2_approx(top - most);
             top = most;
             sum *= by;
           }
-          add = row_exp<BF16>(v, h, p.scale_log2, top == -INFINITY ? 0.f : -top);
+          add = exps();
           if (j > 0) {
             if (!warp_wait(smem_u32(&s_o_done[b ^ 1]), (uint32_t)((j - 1) >> 1) & 1u, abort_flag)) { dead = true; break; }
             tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < p.d; c += 16) {
-              uint32_t o[16];
-              tmem_ld16(lanes + S::kColO + c, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
-              tmem_st16(lanes + S::kColO + c, o);
-            }
+            scale_row(lanes + kColO, p.d, by);
           }
         }
         sum += add;
-        tmem_st32(lanes + S::kColS + kN * b, h);
+        tmem_st32(lanes + kColS + kN * b, h);
         tmem_st_wait();
         tc_fence_before();
       }
       __syncwarp();
       if (one) mbar_arrive(smem_u32(&s_p_full[b]));
     }
-    // ======================= epilogue =======================
     if (!dead && (tiles == 0 || warp_wait(smem_u32(&s_o_done[(tiles - 1) & 1]), (uint32_t)((tiles - 1) >> 1) & 1u, abort_flag))) {
       tc_fence_after();
-      const bool none = sum == 0.f;
-      const int64_t at = row_q * p.hq + row_h;
-      const float by = none ? 0.f : 1.f / sum, lse = none ? INFINITY : top + log2f(sum);
-      if (any_row) {
-        for (int c = 0; c < p.d; c += 16) {
-          uint32_t v[16];
-          if (tiles > 0) {
-            tmem_ld16(lanes + S::kColO + c, v);
-            tmem_ld_wait();
-          }
-          if (none) {                         // no keys: what O holds is not looked at
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = 0u;
-          }
-          if (mine) {
-            if (p.splits > 1) store16_float(v, by, p.part + ((int64_t)split * p.n_q * p.hq + at) * p.d + c, p.d - c);
-            else store16<BF16>(v, by, (uint16_t*)p.out + at * p.d + c, p.d - c);
-          }
-        }
-        if (mine && p.splits > 1) p.part_lse[(int64_t)split * p.n_q * p.hq + at] = lse;
-        else if (mine && p.lse) p.lse[at] = lse;
-      }
+      if (any_row) store_out<BF16>(p, w, part, lanes + kColO, warp * 32 + lane, rows, top, sum);
     }
   } else if (warp == kScoreWarp) {
     // ======================= MMAs of S =======================
     const bool one = elect_one();
     const uint32_t idesc = make_idesc(1u, BF16 ? 1u : 0u, 0u, 0u, kM, kN);
     const int steps = (p.d + 15) / 16;        // of 16 channels
-    const uint64_t q_desc = tile_desc(q_at, 16u), k_desc0 = tile_desc(k_at, 16u);
+    const uint64_t q_desc = tile_desc(q_at, 16u), k_desc = tile_desc(k_at, 16u);
     bool dead = tiles > 0 && !warp_wait(smem_u32(&s_q_full), 0u, abort_flag);
+    if (!S::kQInTmem) fence_proxy_async();
 #pragma unroll 1
     for (int j = 0; j < tiles && !dead; ++j) {
-      const int st = j % S::kStages, b = j & 1;
-      if (!warp_wait(smem_u32(&s_k_full[st]), (uint32_t)(j / S::kStages) & 1u, abort_flag)) break;
+      const int st = j % kStages, b = j & 1;
+      if (!warp_wait(smem_u32(&s_k_full[st]), (uint32_t)(j / kStages) & 1u, abort_flag)) break;
+      if (!by_tma(p, k_map, keys, j)) fence_proxy_async();
       if (j >= 2 && !warp_wait(smem_u32(&s_o_done[b]), (uint32_t)((j - 2) >> 1) & 1u, abort_flag)) break;      // S goes where P was
-      fence_proxy_async();
       tc_fence_after();
-      const uint64_t k_desc = k_desc0 + (uint32_t)st * (S::kTileBytes / 16u);
-      const uint32_t to = tmem + S::kColS + kN * b;
       if (one) {
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
-          if (s >= steps) break;
-          const uint64_t k_s = k_desc + (uint32_t)((s >> 2) * (kN * 8) + (s & 3) * 2);
-          if (S::kQInTmem) umma_f16_ta(to, tmem + S::kColQ + 8 * s, k_s, idesc, s ? 1u : 0u);
-          else umma_f16(to, q_desc + (uint32_t)((s >> 2) * (kM * 8) + (s & 3) * 2), k_s, idesc, s ? 1u : 0u);
-        }
+        issue_scores<DP, S::kQInTmem>(tmem + kColS + kN * b, tmem + S::kColQ, q_desc, k_desc + (uint32_t)st * (kTileBytes / 16u), idesc, steps);
         umma_commit(smem_u32(&s_s_full[b]));
         umma_commit(smem_u32(&s_k_empty[st]));
       }
-      __syncwarp();
     }
   } else if (warp == kOutWarp) {
     // ======================= MMAs of O =======================
     const bool one = elect_one();
     const uint32_t idesc = make_idesc(1u, BF16 ? 1u : 0u, 0u, 1u, kM, (uint32_t)((p.d + 15) / 16 * 16));
-    const uint64_t v_desc0 = tile_desc(v_at, kN * 128u);
+    const uint64_t v_desc = tile_desc(v_at, kN * 128u);
 #pragma unroll 1
     for (int j = 0; j < tiles; ++j) {
-      const int st = j % S::kStages, b = j & 1;
-      if (!warp_wait(smem_u32(&s_v_full[st]), (uint32_t)(j / S::kStages) & 1u, abort_flag)) break;
+      const int st = j % kStages, b = j & 1;
+      if (!warp_wait(smem_u32(&s_v_full[st]), (uint32_t)(j / kStages) & 1u, abort_flag)) break;
+      if (!by_tma(p, v_map, keys, j)) fence_proxy_async();
       if (!warp_wait(smem_u32(&s_p_full[b]), (uint32_t)(j >> 1) & 1u, abort_flag)) break;
-      fence_proxy_async();
       tc_fence_after();
-      const uint64_t v_desc = v_desc0 + (uint32_t)st * (S::kTileBytes / 16u);
       if (one) {
-#pragma unroll
-        for (int s = 0; s < kN / 16; ++s)
-          umma_f16_ta(tmem + S::kColO, tmem + S::kColS + kN * b + 8 * s, v_desc + (uint64_t)(s * (2048 / 16)), idesc, j || s ? 1u : 0u);
+        issue_out(tmem + kColO, tmem + kColS + kN * b, v_desc + (uint32_t)st * (kTileBytes / 16u), idesc, j == 0);
         umma_commit(smem_u32(&s_o_done[b]));
         umma_commit(smem_u32(&s_v_empty[st]));
       }
-      __syncwarp();
     }
   } else {
     // ======================= loads =======================
     const int t = tid - kLoadWarp * 32;
-    const Pieces pc = pieces_of(p.d);
-    const uint8_t* mask = p.mask ? p.mask + w.k0 + keys.x : nullptr;
-    const bool one = elect_one();
-    // 64 rows from key `first` of the part on: whole tiles by TMA, others row by row
-    auto bring = [&](uint32_t to, const TileMap& m, const void* x, int64_t row_stride, int64_t head_stride, int first, int n, uint32_t bar) {
-      if (n == kN && mask == nullptr && m.usable) {
-        if (one && warp == kLoadWarp) {
-          mbar_arrive_expect_tx(bar, S::kTileBytes);
-          tma_tile<DP>(to, kN * 128u, m, head, w.k0 + keys.x + first, bar);
-        } else if (one) {
-          mbar_arrive(bar);
-        }
-        return;
-      }
-      const uint16_t* from = (const uint16_t*)x + (int64_t)(w.k0 + keys.x + first) * row_stride + head * head_stride;
-      load_rows<kN, kLoaders>(to, t, n, p.d, pc, x, [&](int r) { return from + r * row_stride; },
-                             [&](int r) { return mask == nullptr || __ldg(mask + first + r) != 0; });
-      cp_async_arrive(bar);
-      __syncwarp();
-      if (one) mbar_arrive(bar);
-    };
+    const bool one = elect_one(), first = warp == kLoadWarp;
 #pragma unroll 1
     for (int j = 0; j < tiles; ++j) {
-      const int st = j % S::kStages, first = j * kN, n = min(kN, keys.y - keys.x - first);
-      const uint32_t phase = ((uint32_t)(j / S::kStages) & 1u) ^ 1u;
+      const int st = j % kStages;
+      const uint32_t phase = ((uint32_t)(j / kStages) & 1u) ^ 1u;
       if (!warp_wait(smem_u32(&s_k_empty[st]), phase, abort_flag)) break;
-      bring(k_at + st * S::kTileBytes, k_map, p.k, p.k_row, p.k_head, first, n, smem_u32(&s_k_full[st]));
-      if (!S::kQInTmem && j == 0) {           // behind the first keys, which take longer
-        load_rows<kM, kLoaders>(q_at, t, rows, p.d, pc, p.q, [&](int r) {
-          const int i = w.tile * kM + r;
-          return (const uint16_t*)p.q + (int64_t)(w.q0 + i / p.group) * p.q_row + (head * p.group + i % p.group) * p.q_head;
-        }, [](int) { return true; });
-        cp_async_arrive(smem_u32(&s_q_full));
-        __syncwarp();
-        if (one) mbar_arrive(smem_u32(&s_q_full));
-      }
+      load_keys<DP, kLoaders>(k_at + st * kTileBytes, t, first, one, p, k_map, p.k, p.k_row, p.k_head, w, keys, part.head, j,
+                               smem_u32(&s_k_full[st]));
+      if (!S::kQInTmem && j == 0)
+        load_queries<kLoaders>(q_at, t, rows, p, w, part.head, smem_u32(&s_q_full), one);    // behind the first keys
       if (!warp_wait(smem_u32(&s_v_empty[st]), phase, abort_flag)) break;
-      bring(v_at + st * S::kTileBytes, v_map, p.v, p.v_row, p.v_head, first, n, smem_u32(&s_v_full[st]));
+      load_keys<DP, kLoaders>(v_at + st * kTileBytes, t, first, one, p, v_map, p.v, p.v_row, p.v_head, w, keys, part.head, j,
+                               smem_u32(&s_v_full[st]));
     }
     cp_async_wait_all();
   }
