@@ -435,7 +435,6 @@ __global__ void __launch_bounds__(kThreads) join_sum_kernel(const float* part, i
 int attention_forward_tc(const Params& p, bool bf16, int blocks, cudaStream_t st);      // attention_tc.cu
 // attention_tc_bwd.cu
 int attention_backward_tc(const Params& p, bool bf16, bool keys, int blocks, cudaStream_t st);
-int attention_backward_tc_blocks(int d, bool keys);
 
 namespace {
 
@@ -484,8 +483,8 @@ Plan plan_of(const sph_attention& a, const Params& params, int sms) {
     p.fwd_blocks = p.dq_blocks = most_tiles(q_rows, kTcTile, a.B) * a.k_heads;
     p.dkv_blocks = most_tiles(a.n_k, kTcTile, a.B) * a.k_heads;
     p.fwd_splits = splits_for(real(q_rows, kTcTile), 2 * sms, walk(a.n_k, kTcStep), q_values);
-    p.dq_splits = splits_for(real(q_rows, kTcTile), attention_backward_tc_blocks(a.channels, false) * sms, walk(a.n_k, kTcStep), q_values);
-    p.dkv_splits = splits_for(real(a.n_k, kTcTile), attention_backward_tc_blocks(a.channels, true) * sms, walk(q_rows, kTcStep), k_values);
+    p.dq_splits = splits_for(real(q_rows, kTcTile), sms, walk(a.n_k, kTcStep), q_values);
+    p.dkv_splits = splits_for(real(a.n_k, kTcTile), sms, walk(q_rows, kTcStep), k_values);
     return p;
   }
   p.fwd_splits = splits_for(real(q_rows, kTile), sms * per_sm(forward_smem(dp)), walk(a.n_k, kTile), q_values);
