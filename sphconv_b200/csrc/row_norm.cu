@@ -6,7 +6,8 @@
 //   norm(x) = x / sqrt(mean(x^2) + eps), or (x - mean(x)) / sqrt(var(x) + eps) with CENTER
 //
 // One pass: a row is read once into registers, by 1 to 512 threads that hold E values each, reduced among them (shuffles, or shared
-// memory where they are more than a warp) and written.  Statistics and sums are float32; rows are rounded once.  Bound by HBM.
+// memory where they are more than a warp) and written.  Statistics and sums are float32; rows are rounded once.  Bound by HBM: a thread has
+// its columns' parameters in registers and asks for its next row in front of the work on this one.
 // The variance is the mean of squared deviations, which the values in registers make as cheap as the mean of squares.
 //
 // Backward reads the block, the residual, the gate and the two gradients, makes `out` again in float32 (the rounded one would shift
@@ -40,58 +41,92 @@ struct Params {
   float eps;
 };
 
+// Rows are loaded and kept as words of their bits: 16 bytes, or one element, a piece.
 template <typename T> struct Row;
 template <> struct Row<float> {
   static constexpr int kVec = 4;
-  static __device__ __forceinline__ float get(float v) { return v; }
-  static __device__ __forceinline__ float put(float v) { return v; }
+  using Bits = uint32_t;
+  static __device__ __forceinline__ float get(uint32_t v) { return __uint_as_float(v); }
+  static __device__ __forceinline__ uint32_t put(float v) { return __float_as_uint(v); }
+  static __device__ __forceinline__ void unpack(float* x, uint32_t w) { x[0] = __uint_as_float(w); }
+  static __device__ __forceinline__ uint32_t pack(const float* x) { return __float_as_uint(x[0]); }
 };
 template <> struct Row<__half> {
   static constexpr int kVec = 8;
-  static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
-  static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
+  using Bits = uint16_t;
+  static __device__ __forceinline__ float get(uint16_t v) { return __half2float(__ushort_as_half(v)); }
+  static __device__ __forceinline__ uint16_t put(float v) { return __half_as_ushort(__float2half_rn(v)); }
+  static __device__ __forceinline__ void unpack(float* x, uint32_t w) {
+    const float2 f = __half22float2(*(const __half2*)&w);
+    x[0] = f.x; x[1] = f.y;
+  }
+  static __device__ __forceinline__ uint32_t pack(const float* x) {
+    const __half2 h = __floats2half2_rn(x[0], x[1]);
+    return *(const uint32_t*)&h;
+  }
 };
 template <> struct Row<__nv_bfloat16> {
   static constexpr int kVec = 8;
-  static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
-  static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
+  using Bits = uint16_t;
+  static __device__ __forceinline__ float get(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+  static __device__ __forceinline__ uint16_t put(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+  static __device__ __forceinline__ void unpack(float* x, uint32_t w) {
+    x[0] = __uint_as_float(w << 16);
+    x[1] = __uint_as_float(w & 0xffff0000u);
+  }
+  static __device__ __forceinline__ uint32_t pack(const float* x) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[0], x[1]);
+    return *(const uint32_t*)&h;
+  }
 };
 
 // A thread's values of a row: NV pieces of VEC consecutive ones, piece j at (j * lanes + t) * VEC.
 template <typename T, int VEC, int NV>
 struct Tile {
   static constexpr int E = VEC * NV;
-  struct __align__(VEC * sizeof(T)) Piece { T v[VEC]; };
+  using R = Row<T>;
+  using Bits = typename R::Bits;
+  static constexpr int kWords = VEC > 1 ? 4 : 1;
+  struct Raw { uint32_t w[NV][kWords]; };     // as they lie in memory
 
   static __device__ __forceinline__ int column(int j, int t, int lanes) { return (j * lanes + t) * VEC; }
 
-  static __device__ __forceinline__ void load(float (&x)[E], const void* base, int64_t row, int c, int t, int lanes, bool active) {
-    const T* p = (const T*)base + row * c;
+  static __device__ __forceinline__ void fetch(Raw& r, const void* base, int64_t row, int c, int t, int lanes, bool active) {
+    const Bits* p = (const Bits*)base + row * c;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = column(j, t, lanes);
-      Piece q;
-      if (active && at < c) {
-        q = *(const Piece*)(p + at);          // c is a multiple of VEC
+      const bool some = active && at < c;     // c is a multiple of VEC
+      if constexpr (VEC > 1) {
+        const uint4 q = some ? *(const uint4*)(p + at) : make_uint4(0u, 0u, 0u, 0u);
+        r.w[j][0] = q.x; r.w[j][1] = q.y; r.w[j][2] = q.z; r.w[j][3] = q.w;
       } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) q.v[i] = Row<T>::put(0.f);
+        r.w[j][0] = some ? (uint32_t)p[at] : 0u;
       }
+    }
+  }
+  static __device__ __forceinline__ void values(float (&x)[E], const Raw& r) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) x[j * VEC + i] = Row<T>::get(q.v[i]);
+    for (int j = 0; j < NV; ++j) {
+      if constexpr (VEC > 1) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) R::unpack(&x[j * VEC + i * (VEC / 4)], r.w[j][i]);
+      } else {
+        x[j] = R::get((Bits)r.w[j][0]);
+      }
     }
   }
   static __device__ __forceinline__ void store(const float (&x)[E], void* base, int64_t row, int c, int t, int lanes, bool active) {
-    T* p = (T*)base + row * c;
+    Bits* p = (Bits*)base + row * c;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = column(j, t, lanes);
-      if (active && at < c) {
-        Piece q;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) q.v[i] = Row<T>::put(x[j * VEC + i]);
-        *(Piece*)(p + at) = q;
-      }
+      if (!active || at >= c) continue;
+      if constexpr (VEC > 1)
+        *(uint4*)(p + at) = make_uint4(R::pack(&x[j * VEC]), R::pack(&x[j * VEC + VEC / 4]), R::pack(&x[j * VEC + VEC / 2]),
+                                       R::pack(&x[j * VEC + 3 * VEC / 4]));
+      else
+        p[at] = R::put(x[j]);
     }
   }
   // a parameter [c] of float32 or of 16 bits, or `other` where there is none; 16-byte aligned where rows come in pieces
@@ -189,133 +224,163 @@ __device__ __forceinline__ void statistics(const float (&x)[VEC * NV], Reducer& 
       if (!CENTER || (j * red.lanes + t) * VEC + i < c) s[0] = fmaf(d, d, s[0]);       // behind the row are zeros
     }
   red.sum(s);
-  inv = 1.f / sqrtf(s[0] / (float)c + eps);
+  inv = rsqrtf(s[0] / (float)c + eps);
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
-
+// 16-bit rows round what is left of it to 8 or 11 bits: 2^-21 is enough
 template <typename T>
-__device__ __forceinline__ float row_gate(const Params& p, int64_t row, bool active) {
-  return active ? sigmoid(Row<T>::get(((const T*)p.gate)[row])) : 0.f;
+__device__ __forceinline__ float sigmoid(float x) {
+  if (sizeof(T) == 2) return __fdividef(1.f, 1.f + __expf(-x));
+  return 1.f / (1.f + expf(-x));
 }
 
-template <typename T, int VEC, int NV, bool CENTER>
-__global__ void __launch_bounds__(512) forward_kernel(const __grid_constant__ Params p) {
+// BIAS: there may be biases.  THREADS: most threads of a block; a small one leaves room for three on an SM (rows of 64 bf16 channels 85 ->
+// FWD us), two backward, whose sums take the registers.
+template <typename T, int VEC, int NV, bool CENTER, bool BIAS, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) forward_kernel(const __grid_constant__ Params p) {
   using X = Tile<T, VEC, NV>;
   constexpr int E = X::E;
   __shared__ float slots[2][kMaxWarps][4];
   after_previous();
   const int lanes = p.lanes, c = p.c, t = threadIdx.x & (lanes - 1), rows = blockDim.x / lanes;
+  const bool gated = p.gate && !p.gate_row;
   Reducer red{slots, lanes, 0};
-  for (int64_t base = (int64_t)blockIdx.x * rows; base < p.n; base += (int64_t)gridDim.x * rows) {
-    const int64_t row = base + threadIdx.x / lanes;
+  float weight[E], scale[E], next_weight[E];
+  X::param(weight, p.param[0], p.param_dtype[0], 1.f, c, t, lanes);
+  X::param(scale, p.param[2], p.param_dtype[2], 1.f, c, t, lanes);
+  X::param(next_weight, p.param[3], p.param_dtype[3], 1.f, c, t, lanes);
+  typename X::Raw raw_x, raw_b, raw_g;
+  typename Row<T>::Bits raw_rg = 0;
+  auto fetch = [&](int64_t row) {
+    const bool some = row < p.n;
+    X::fetch(raw_x, p.residual, row, c, t, lanes, some);
+    if (p.block) X::fetch(raw_b, p.block, row, c, t, lanes, some);
+    if (gated) X::fetch(raw_g, p.gate, row, c, t, lanes, some);
+    else if (p.gate && some) raw_rg = ((const typename Row<T>::Bits*)p.gate)[row];
+  };
+  const int64_t first = (int64_t)blockIdx.x * rows, step = (int64_t)gridDim.x * rows;
+  const int mine = threadIdx.x / lanes;
+  if (first < p.n) fetch(first + mine);
+  for (int64_t base = first; base < p.n; base += step) {
+    const int64_t row = base + mine;
     const bool active = row < p.n;
-    float out[E], b[E], g[E], w[E];
+    float out[E], b[E], g[E];
     float mean = 0.f, inv = 1.f;
-    X::load(out, p.residual, row, c, t, lanes, active);
+    X::values(out, raw_x);
+    if (p.block) X::values(b, raw_b);
+    if (gated) X::values(g, raw_g);
+    const float rg = p.gate && !gated ? sigmoid<T>(Row<T>::get(raw_rg)) : 1.f;
+    if (base + step < p.n) fetch(row + step);
     if (p.block) {
-      X::load(b, p.block, row, c, t, lanes, active);
-      const bool gated = p.gate && !p.gate_row;
-      if (gated) X::load(g, p.gate, row, c, t, lanes, active);
-      const float rg = p.gate && p.gate_row ? row_gate<T>(p, row, active) : 1.f;
       if (p.param[0]) {
         statistics<CENTER, VEC, NV>(b, red, c, t, p.eps, mean, inv);
-        X::param(w, p.param[0], p.param_dtype[0], 1.f, c, t, lanes);
 #pragma unroll
-        for (int e = 0; e < E; ++e) b[e] = (b[e] - mean) * inv * w[e];
-        if (p.param[1]) {
+        for (int e = 0; e < E; ++e) b[e] = (b[e] - mean) * inv * weight[e];
+        if (BIAS && p.param[1]) {
+          float w[E];
           X::param(w, p.param[1], p.param_dtype[1], 0.f, c, t, lanes);
 #pragma unroll
           for (int e = 0; e < E; ++e) b[e] += w[e];
         }
       }
       if (p.stats && t == 0 && active) *(float2*)(p.stats + row * 4) = make_float2(mean, inv);
-      X::param(w, p.param[2], p.param_dtype[2], 1.f, c, t, lanes);
 #pragma unroll
-      for (int e = 0; e < E; ++e) out[e] = fmaf(w[e] * (gated ? sigmoid(g[e]) : rg), b[e], out[e]);
+      for (int e = 0; e < E; ++e) out[e] = fmaf(scale[e] * (gated ? sigmoid<T>(g[e]) : rg), b[e], out[e]);
       if (p.out) X::store(out, p.out, row, c, t, lanes, active);
     }
     if (p.normed) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)                                  // what a bias added behind the row's end
-        if (X::column(j, t, lanes) >= c) {
+        if (BIAS && X::column(j, t, lanes) >= c) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i) out[j * VEC + i] = 0.f;
         }
       statistics<CENTER, VEC, NV>(out, red, c, t, p.eps, mean, inv);
       if (p.stats && t == 0 && active) *(float2*)(p.stats + row * 4 + 2) = make_float2(mean, inv);
-      X::param(w, p.param[3], p.param_dtype[3], 1.f, c, t, lanes);
-      X::param(b, p.param[4], p.param_dtype[4], 0.f, c, t, lanes);
 #pragma unroll
-      for (int e = 0; e < E; ++e) out[e] = fmaf((out[e] - mean) * inv, w[e], b[e]);
+      for (int e = 0; e < E; ++e) out[e] = (out[e] - mean) * inv * next_weight[e];
+      if (BIAS && p.param[4]) {
+        X::param(b, p.param[4], p.param_dtype[4], 0.f, c, t, lanes);
+#pragma unroll
+        for (int e = 0; e < E; ++e) out[e] += b[e];
+      }
       X::store(out, p.normed, row, c, t, lanes, active);
     }
   }
 }
 
-template <typename T, int VEC, int NV, bool CENTER>
-__global__ void __launch_bounds__(512) backward_kernel(const __grid_constant__ Params p) {
+template <typename T, int VEC, int NV, bool CENTER, bool BIAS, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) backward_kernel(const __grid_constant__ Params p) {
   using X = Tile<T, VEC, NV>;
   constexpr int E = X::E;
   __shared__ float slots[2][kMaxWarps][4];
   extern __shared__ float columns[];                                // rows of a block > 1: [kBlock][E]
   after_previous();
   const int lanes = p.lanes, c = p.c, t = threadIdx.x & (lanes - 1), rows = blockDim.x / lanes;
+  const bool gated = p.gate && !p.gate_row;
   const float per_c = 1.f / (float)c;
   Reducer red{slots, lanes, 0};
+  float weight[E], scale[E], next_weight[E];
+  X::param(weight, p.param[0], p.param_dtype[0], 1.f, c, t, lanes);
+  X::param(scale, p.param[2], p.param_dtype[2], 1.f, c, t, lanes);
+  X::param(next_weight, p.param[3], p.param_dtype[3], 1.f, c, t, lanes);
   float sums[kSums][E];
 #pragma unroll
   for (int s = 0; s < kSums; ++s)
 #pragma unroll
     for (int e = 0; e < E; ++e) sums[s][e] = 0.f;
-  for (int64_t base = (int64_t)blockIdx.x * rows; base < p.n; base += (int64_t)gridDim.x * rows) {
-    const int64_t row = base + threadIdx.x / lanes;
+  typename X::Raw raw_x, raw_b, raw_g, raw_d, raw_n;
+  typename Row<T>::Bits raw_rg = 0;
+  float4 raw_st = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto fetch = [&](int64_t row) {
+    const bool some = row < p.n;
+    raw_st = some ? *(const float4*)(p.stats + row * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    X::fetch(raw_x, p.residual, row, c, t, lanes, some);
+    if (p.block) X::fetch(raw_b, p.block, row, c, t, lanes, some);
+    if (gated) X::fetch(raw_g, p.gate, row, c, t, lanes, some);
+    else if (p.gate) raw_rg = some ? ((const typename Row<T>::Bits*)p.gate)[row] : (typename Row<T>::Bits)0;
+    if (p.d_out) X::fetch(raw_d, p.d_out, row, c, t, lanes, some);
+    if (p.d_normed) X::fetch(raw_n, p.d_normed, row, c, t, lanes, some);
+  };
+  const int64_t first = (int64_t)blockIdx.x * rows, step = (int64_t)gridDim.x * rows;
+  const int mine = threadIdx.x / lanes;
+  if (first < p.n) fetch(first + mine);
+  for (int64_t base = first; base < p.n; base += step) {
+    const int64_t row = base + mine;
     const bool active = row < p.n;
-    const bool gated = p.gate && !p.gate_row;
-    float x[E], b[E], g[E], w[E], total[E], dn[E];
-    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (active) st = *(const float4*)(p.stats + row * 4);
+    float x[E], b[E], g[E], total[E], dn[E];
+    const float4 st = raw_st;
     const float mb = p.param[0] ? st.x : 0.f, ib = p.param[0] ? st.y : 1.f;
-    X::load(x, p.residual, row, c, t, lanes, active);
-    float rg = 1.f;
-    if (p.block) {
-      X::load(b, p.block, row, c, t, lanes, active);
-      if (gated) X::load(g, p.gate, row, c, t, lanes, active);
-      else if (p.gate) rg = row_gate<T>(p, row, active);
-    }
+    const float rg = p.gate && !gated ? sigmoid<T>(Row<T>::get(raw_rg)) : 1.f;
+    X::values(x, raw_x);
+    if (p.block) X::values(b, raw_b);
+    if (gated) X::values(g, raw_g);
     if (p.d_out) {
-      X::load(total, p.d_out, row, c, t, lanes, active);
+      X::values(total, raw_d);
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) total[e] = 0.f;
     }
-    if (p.d_normed) X::load(dn, p.d_normed, row, c, t, lanes, active);
+    if (p.d_normed) X::values(dn, raw_n);
+    if (base + step < p.n) fetch(row + step);
+    float bias[E];                                                  // in a register only where there is one
+    if (BIAS) X::param(bias, p.param[1], p.param_dtype[1], 0.f, c, t, lanes);
     if (p.block) {                                                  // b: the normalised block; x: out
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         b[e] = (b[e] - mb) * ib;
-        g[e] = gated ? sigmoid(g[e]) : rg;
+        g[e] = gated ? sigmoid<T>(g[e]) : rg;
       }
     }
     if (p.d_normed) {
-      if (p.block) {
-        float w2[E];
-        X::param(w, p.param[0], p.param_dtype[0], 1.f, c, t, lanes);
-        X::param(w2, p.param[1], p.param_dtype[1], 0.f, c, t, lanes);
-#pragma unroll
-        for (int e = 0; e < E; ++e) w[e] = fmaf(b[e], w[e], w2[e]);
-        X::param(w2, p.param[2], p.param_dtype[2], 1.f, c, t, lanes);
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = fmaf(w2[e] * g[e], w[e], x[e]);
-      }
-      X::param(w, p.param[3], p.param_dtype[3], 1.f, c, t, lanes);
       float s[2] = {0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < E; ++e) {
+        if (p.block) x[e] = fmaf(scale[e] * g[e], BIAS ? fmaf(b[e], weight[e], bias[e]) : b[e] * weight[e], x[e]);
         x[e] = (x[e] - st.z) * st.w;                                // the normalised out; dn is zero behind the row's end
         sums[3][e] = fmaf(dn[e], x[e], sums[3][e]);
-        sums[4][e] += dn[e];
-        dn[e] *= w[e];
+        if (BIAS) sums[4][e] += dn[e];
+        dn[e] *= next_weight[e];
         s[0] = fmaf(dn[e], x[e], s[0]);
         s[1] += dn[e];
       }
@@ -323,39 +388,36 @@ __global__ void __launch_bounds__(512) backward_kernel(const __grid_constant__ P
       s[0] *= per_c;
       s[1] = CENTER ? s[1] * per_c : 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) total[e] = fmaf(st.w, dn[e] - s[1] - x[e] * s[0], total[e]);
+      for (int j = 0; j < NV; ++j) {
+        const bool inside = X::column(j, t, lanes) < c;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (X::column(j, t, lanes) >= c) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) total[j * VEC + i] = 0.f;
+        for (int i = 0; i < VEC; ++i) {
+          const int e = j * VEC + i;
+          total[e] = inside ? fmaf(st.w, dn[e] - s[1] - x[e] * s[0], total[e]) : 0.f;
         }
+      }
     }
     if (p.d_residual) X::store(total, p.d_residual, row, c, t, lanes, active);
     if (p.block) {
       float s[3] = {0.f, 0.f, 0.f};
-      X::param(w, p.param[0], p.param_dtype[0], 1.f, c, t, lanes);
-      X::param(x, p.param[1], p.param_dtype[1], 0.f, c, t, lanes);
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = fmaf(b[e], w[e], x[e]);    // inner
-      X::param(dn, p.param[2], p.param_dtype[2], 1.f, c, t, lanes);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
+        const float inner = BIAS ? fmaf(b[e], weight[e], bias[e]) : b[e] * weight[e];
         const float tg = total[e] * g[e];                           // gradient of scale * inner
-        const float d_inner = tg * dn[e];
-        sums[2][e] = fmaf(tg, x[e], sums[2][e]);
+        const float d_inner = tg * scale[e];
+        sums[2][e] = fmaf(tg, inner, sums[2][e]);
         sums[0][e] = fmaf(d_inner, b[e], sums[0][e]);
-        sums[1][e] += d_inner;
-        x[e] = d_inner * x[e] * (1.f - g[e]);                       // gradient of the gate's logit
+        if (BIAS) sums[1][e] += d_inner;
+        x[e] = d_inner * inner * (1.f - g[e]);                      // gradient of the gate's logit
         s[2] += x[e];
-        dn[e] = d_inner * w[e];
+        dn[e] = d_inner * weight[e];
         s[0] = fmaf(dn[e], b[e], s[0]);
         s[1] += dn[e];
       }
       if (gated && p.d_gate) X::store(x, p.d_gate, row, c, t, lanes, active);
       if (p.param[0] || p.gate_row) {
         red.sum(s);
-        if (p.gate_row && p.d_gate && t == 0 && active) ((T*)p.d_gate)[row] = Row<T>::put(s[2]);
+        if (p.gate_row && p.d_gate && t == 0 && active) ((typename Row<T>::Bits*)p.d_gate)[row] = Row<T>::put(s[2]);
       }
       if (p.param[0]) {
         s[0] *= per_c;
@@ -370,7 +432,7 @@ __global__ void __launch_bounds__(512) backward_kernel(const __grid_constant__ P
   if (p.partial == nullptr) return;
 #pragma unroll
   for (int s = 0; s < kSums; ++s) {
-    if (p.param[s] == nullptr) continue;
+    if (p.param[s] == nullptr || (!BIAS && (s == 1 || s == 4))) continue;
     float* to = p.partial + ((int64_t)blockIdx.x * kSums + s) * c;
     if (rows > 1) {
       __syncthreads();
@@ -485,27 +547,30 @@ int fill(const sph_norm* a, const char* who, Params* p) {
   return SPH_OK;
 }
 
-template <typename T, int VEC, int NV>
-void start(bool backward, bool center, int grid, const Shape& s, cudaStream_t st, const Params& p) {
+template <typename T, int VEC, int NV, bool CENTER, bool BIAS, int THREADS>
+void start(bool backward, int grid, const Shape& s, cudaStream_t st, const Params& p) {
   const size_t smem = backward && s.threads > s.lanes ? (size_t)kBlock * VEC * NV * sizeof(float) : 0;
-  if (backward) {
-    if (center) launch(backward_kernel<T, VEC, NV, true>, grid, s.threads, smem, st, p);
-    else launch(backward_kernel<T, VEC, NV, false>, grid, s.threads, smem, st, p);
-  } else {
-    if (center) launch(forward_kernel<T, VEC, NV, true>, grid, s.threads, 0, st, p);
-    else launch(forward_kernel<T, VEC, NV, false>, grid, s.threads, 0, st, p);
-  }
+  if (backward) launch(backward_kernel<T, VEC, NV, CENTER, BIAS, THREADS>, grid, s.threads, smem, st, p);
+  else launch(forward_kernel<T, VEC, NV, CENTER, BIAS, THREADS>, grid, s.threads, 0, st, p);
+}
+template <typename T, int VEC, int NV, int THREADS>
+void start(bool backward, bool center, int grid, const Shape& s, cudaStream_t st, const Params& p) {
+  if (center) start<T, VEC, NV, true, true, THREADS>(backward, grid, s, st, p);
+  else if (p.param[1] || p.param[4]) start<T, VEC, NV, false, true, THREADS>(backward, grid, s, st, p);
+  else start<T, VEC, NV, false, false, THREADS>(backward, grid, s, st, p);
 }
 template <typename T>
 void start(bool backward, bool center, int grid, const Shape& s, cudaStream_t st, const Params& p) {
   constexpr int V = Row<T>::kVec;
-  const bool wide = s.vec * s.nv == 16;
+  const bool wide = s.vec * s.nv == 16, large = s.threads > kBlock;
   if (s.vec == 1) {
-    if (wide) start<T, 1, 16>(backward, center, grid, s, st, p);
-    else start<T, 1, 8>(backward, center, grid, s, st, p);
+    if (wide) start<T, 1, 16, 512>(backward, center, grid, s, st, p);
+    else if (large) start<T, 1, 8, 512>(backward, center, grid, s, st, p);
+    else start<T, 1, 8, kBlock>(backward, center, grid, s, st, p);
   } else {
-    if (wide) start<T, V, 16 / V>(backward, center, grid, s, st, p);
-    else start<T, V, 8 / V>(backward, center, grid, s, st, p);
+    if (wide) start<T, V, 16 / V, 512>(backward, center, grid, s, st, p);
+    else if (large) start<T, V, 8 / V, 512>(backward, center, grid, s, st, p);
+    else start<T, V, 8 / V, kBlock>(backward, center, grid, s, st, p);
   }
 }
 int start(int dtype, bool backward, bool center, int grid, const Shape& s, cudaStream_t st, Params& p) {
@@ -539,7 +604,7 @@ extern "C" int sph_residual_norm(const sph_norm* a, void* d_out, void* d_normed,
                      (p.gate_row || aligned16(a->gate)) && aligned16(d_out) && aligned16(d_normed) && params_aligned(p);
   Shape s;
   if (!shape_of(a->c, e, whole, &s)) { set_error("%s: too many channels", __func__); return SPH_ERR_LIMIT; }
-  return start(a->dtype, false, a->center != 0, grid_of(s, a->n, sms, 2048 / s.threads), s, (cudaStream_t)stream, p);
+  return start(a->dtype, false, a->center != 0, grid_of(s, a->n, sms, std::max(1, 768 / s.threads)), s, (cudaStream_t)stream, p);
 }
 
 extern "C" int64_t sph_residual_norm_scratch_bytes(int64_t n, int32_t c) {
