@@ -79,33 +79,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return y;
 }
 
-// Two float32 operations an instruction.
-__device__ __forceinline__ uint64_t as_pair(float2 v) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
-  return r;
-}
-__device__ __forceinline__ float2 of_pair(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as_pair(a)), "l"(as_pair(b)), "l"(as_pair(c)));
-  return of_pair(r);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_pair(a)), "l"(as_pair(b)));
-  return of_pair(r);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_pair(a)), "l"(as_pair(b)));
-  return of_pair(r);
-}
-
 // Two values rounded to the rows' type, the first in the lower half.
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {

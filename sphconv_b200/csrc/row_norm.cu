@@ -6,8 +6,9 @@
 //   norm(x) = x / sqrt(mean(x^2) + eps), or (x - mean(x)) / sqrt(var(x) + eps) with CENTER
 //
 // One pass: a row is read once into registers, by 1 to 512 threads that hold E values each, reduced among them (shuffles, or shared
-// memory where they are more than a warp) and written.  Statistics and sums are float32; rows are rounded once.  Bound by HBM: a thread has
-// its columns' parameters in registers and asks for its next row in front of the work on this one.
+// memory where they are more than a warp) and written.  Statistics and sums are float32; rows are rounded once.  A thread has its columns'
+// parameters in registers and asks for its next row in front of the work on this one; what is between it and HBM's rate is then the
+// number of its instructions, so values go two to a float32 operation.
 // The variance is the mean of squared deviations, which the values in registers make as cheap as the mean of squares.
 //
 // Backward reads the block, the residual, the gate and the two gradients, makes `out` again in float32 (the rounded one would shift
@@ -48,20 +49,15 @@ template <> struct Row<float> {
   using Bits = uint32_t;
   static __device__ __forceinline__ float get(uint32_t v) { return __uint_as_float(v); }
   static __device__ __forceinline__ uint32_t put(float v) { return __float_as_uint(v); }
-  static __device__ __forceinline__ void unpack(float* x, uint32_t w) { x[0] = __uint_as_float(w); }
-  static __device__ __forceinline__ uint32_t pack(const float* x) { return __float_as_uint(x[0]); }
 };
 template <> struct Row<__half> {
   static constexpr int kVec = 8;
   using Bits = uint16_t;
   static __device__ __forceinline__ float get(uint16_t v) { return __half2float(__ushort_as_half(v)); }
   static __device__ __forceinline__ uint16_t put(float v) { return __half_as_ushort(__float2half_rn(v)); }
-  static __device__ __forceinline__ void unpack(float* x, uint32_t w) {
-    const float2 f = __half22float2(*(const __half2*)&w);
-    x[0] = f.x; x[1] = f.y;
-  }
-  static __device__ __forceinline__ uint32_t pack(const float* x) {
-    const __half2 h = __floats2half2_rn(x[0], x[1]);
+  static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*(const __half2*)&w); }
+  static __device__ __forceinline__ uint32_t pack(float2 x) {
+    const __half2 h = __float22half2_rn(x);
     return *(const uint32_t*)&h;
   }
 };
@@ -70,17 +66,14 @@ template <> struct Row<__nv_bfloat16> {
   using Bits = uint16_t;
   static __device__ __forceinline__ float get(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
   static __device__ __forceinline__ uint16_t put(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
-  static __device__ __forceinline__ void unpack(float* x, uint32_t w) {
-    x[0] = __uint_as_float(w << 16);
-    x[1] = __uint_as_float(w & 0xffff0000u);
-  }
-  static __device__ __forceinline__ uint32_t pack(const float* x) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x[0], x[1]);
+  static __device__ __forceinline__ float2 unpack(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+  static __device__ __forceinline__ uint32_t pack(float2 x) {
+    const __nv_bfloat162 h = __float22bfloat162_rn(x);
     return *(const uint32_t*)&h;
   }
 };
 
-// A thread's values of a row: NV pieces of VEC consecutive ones, piece j at (j * lanes + t) * VEC.
+// A thread's values of a row: NV pieces of VEC consecutive ones, piece j at (j * lanes + t) * VEC; in pairs for the arithmetic.
 template <typename T, int VEC, int NV>
 struct Tile {
   static constexpr int E = VEC * NV;
@@ -105,73 +98,69 @@ struct Tile {
       }
     }
   }
-  static __device__ __forceinline__ void values(float (&x)[E], const Raw& r) {
+  static constexpr int P = E / 2;             // pairs
+  using Pairs = float2[P];
+  // piece and place in it of value e
+  static __device__ __forceinline__ bool inside(int e, int c, int t, int lanes) { return column(e / VEC, t, lanes) < c; }
+
+  static __device__ __forceinline__ void values(Pairs& x, const Raw& r) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if constexpr (VEC > 1) {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) R::unpack(&x[j * VEC + i * (VEC / 4)], r.w[j][i]);
-      } else {
-        x[j] = R::get((Bits)r.w[j][0]);
-      }
+    for (int k = 0; k < P; ++k) {
+      const int e = 2 * k;
+      if constexpr (VEC == 1) x[k] = make_float2(R::get((Bits)r.w[e][0]), R::get((Bits)r.w[e + 1][0]));
+      else if constexpr (VEC == 4) x[k] = make_float2(__uint_as_float(r.w[e / 4][e % 4]), __uint_as_float(r.w[e / 4][e % 4 + 1]));
+      else x[k] = R::unpack(r.w[e / 8][e % 8 / 2]);
     }
   }
-  static __device__ __forceinline__ void store(const float (&x)[E], void* base, int64_t row, int c, int t, int lanes, bool active) {
+  static __device__ __forceinline__ void store(const Pairs& x, void* base, int64_t row, int c, int t, int lanes, bool active) {
     Bits* p = (Bits*)base + row * c;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = column(j, t, lanes);
       if (!active || at >= c) continue;
-      if constexpr (VEC > 1)
-        *(uint4*)(p + at) = make_uint4(R::pack(&x[j * VEC]), R::pack(&x[j * VEC + VEC / 4]), R::pack(&x[j * VEC + VEC / 2]),
-                                       R::pack(&x[j * VEC + 3 * VEC / 4]));
+      if constexpr (VEC == 1)
+        p[at] = R::put(j % 2 ? x[j / 2].y : x[j / 2].x);
+      else if constexpr (VEC == 4)
+        *(uint4*)(p + at) = make_uint4(__float_as_uint(x[2 * j].x), __float_as_uint(x[2 * j].y), __float_as_uint(x[2 * j + 1].x),
+                                       __float_as_uint(x[2 * j + 1].y));
       else
-        p[at] = R::put(x[j]);
+        *(uint4*)(p + at) = make_uint4(R::pack(x[4 * j]), R::pack(x[4 * j + 1]), R::pack(x[4 * j + 2]), R::pack(x[4 * j + 3]));
     }
   }
   // a parameter [c] of float32 or of 16 bits, or `other` where there is none; 16-byte aligned where rows come in pieces
-  static __device__ __forceinline__ void param(float (&x)[E], const void* p, int dtype, float other, int c, int t, int lanes) {
+  static __device__ __forceinline__ void param(Pairs& x, const void* p, int dtype, float other, int c, int t, int lanes) {
+    auto wide = [&](uint32_t bits) { return dtype == SPH_F16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16); };
+#pragma unroll
+    for (int k = 0; k < P; ++k) x[k] = make_float2(other, other);
+    if (p == nullptr) return;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = column(j, t, lanes);
+      if (at >= c) continue;
       if constexpr (VEC > 1) {
-        if (p == nullptr || at >= c) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) x[j * VEC + i] = other;
-        } else if (dtype == SPH_F32) {
-#pragma unroll
-          for (int i = 0; i < VEC / 4; ++i) {
-            const float4 f = __ldg((const float4*)((const float*)p + at) + i);
-            x[j * VEC + 4 * i] = f.x; x[j * VEC + 4 * i + 1] = f.y;
-            x[j * VEC + 4 * i + 2] = f.z; x[j * VEC + 4 * i + 3] = f.w;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC / 4; ++i) {
-            const uint2 h = __ldg((const uint2*)((const unsigned short*)p + at) + i);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const unsigned short bits = (unsigned short)((k < 2 ? h.x : h.y) >> (16 * (k & 1)));
-              x[j * VEC + 4 * i + k] =
-                  dtype == SPH_F16 ? __half2float(__ushort_as_half(bits)) : __uint_as_float((unsigned)bits << 16);
-            }
+        for (int i = 0; i < VEC; i += 4) {
+          float2 &a = x[(j * VEC + i) / 2], &b = x[(j * VEC + i) / 2 + 1];
+          if (dtype == SPH_F32) {
+            const float4 f = __ldg((const float4*)((const float*)p + at + i));
+            a = make_float2(f.x, f.y);
+            b = make_float2(f.z, f.w);
+          } else {
+            const uint2 h = __ldg((const uint2*)((const unsigned short*)p + at + i));
+            a = make_float2(wide(h.x & 0xffffu), wide(h.x >> 16));
+            b = make_float2(wide(h.y & 0xffffu), wide(h.y >> 16));
           }
         }
       } else {
-        float v = other;
-        if (p && at < c) {
-          if (dtype == SPH_F32) {
-            v = __ldg((const float*)p + at);
-          } else {
-            const unsigned short bits = __ldg((const unsigned short*)p + at);
-            v = dtype == SPH_F16 ? __half2float(__ushort_as_half(bits)) : __uint_as_float((unsigned)bits << 16);
-          }
-        }
-        x[j] = v;
+        const float v = dtype == SPH_F32 ? __ldg((const float*)p + at) : wide(__ldg((const unsigned short*)p + at));
+        if (j % 2) x[j / 2].y = v; else x[j / 2].x = v;
       }
     }
   }
 };
+
+__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float both(float2 v) { return v.x + v.y; }
 
 // Sums over the threads of a row, in every one of them.  More than a warp: the block is one row, and calls alternate between two
 // places in shared memory, so that one barrier a call is enough.
@@ -202,29 +191,34 @@ struct Reducer {
   }
 };
 
-// mean and 1/deviation of a row
-template <bool CENTER, int VEC, int NV>
-__device__ __forceinline__ void statistics(const float (&x)[VEC * NV], Reducer& red, int c, int t, float eps, float& mean, float& inv) {
-  constexpr int E = VEC * NV;
+// mean and 1/deviation of a row, whose values behind the end are zeros
+template <typename X, bool CENTER>
+__device__ __forceinline__ void statistics(const typename X::Pairs& x, Reducer& red, int c, int t, float eps, float& mean, float& inv) {
+  const float per_c = 1.f / (float)c;
   mean = 0.f;
   float s[1];
+  float2 a = pair(0.f);
   if (CENTER) {
-    s[0] = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) s[0] += x[e];
+    for (int k = 0; k < X::P; ++k) a = add2(a, x[k]);
+    s[0] = both(a);
     red.sum(s);
-    mean = s[0] / (float)c;
+    mean = s[0] * per_c;
+    a = pair(0.f);
   }
-  s[0] = 0.f;
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float d = x[j * VEC + i] - mean;
-      if (!CENTER || (j * red.lanes + t) * VEC + i < c) s[0] = fmaf(d, d, s[0]);       // behind the row are zeros
+  for (int k = 0; k < X::P; ++k) {
+    float2 d = x[k];
+    if (CENTER) {
+      d = add2(d, pair(-mean));
+      if (!X::inside(2 * k, c, t, red.lanes)) d.x = 0.f;
+      if (!X::inside(2 * k + 1, c, t, red.lanes)) d.y = 0.f;
     }
+    a = fma2(d, d, a);
+  }
+  s[0] = both(a);
   red.sum(s);
-  inv = rsqrtf(s[0] / (float)c + eps);
+  inv = rsqrtf(fmaf(s[0], per_c, eps));
 }
 
 // 16-bit rows round what is left of it to 8 or 11 bits: 2^-21 is enough
@@ -233,19 +227,22 @@ __device__ __forceinline__ float sigmoid(float x) {
   if (sizeof(T) == 2) return __fdividef(1.f, 1.f + __expf(-x));
   return 1.f / (1.f + expf(-x));
 }
+template <typename T>
+__device__ __forceinline__ float2 sigmoid(float2 x) { return make_float2(sigmoid<T>(x.x), sigmoid<T>(x.y)); }
 
 // BIAS: there may be biases.  THREADS: most threads of a block; a small one leaves room for three on an SM (rows of 64 bf16 channels 85 ->
 // FWD us), two backward, whose sums take the registers.
 template <typename T, int VEC, int NV, bool CENTER, bool BIAS, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) forward_kernel(const __grid_constant__ Params p) {
   using X = Tile<T, VEC, NV>;
-  constexpr int E = X::E;
+  constexpr int P = X::P;
+  using Pairs = typename X::Pairs;
   __shared__ float slots[2][kMaxWarps][4];
   after_previous();
   const int lanes = p.lanes, c = p.c, t = threadIdx.x & (lanes - 1), rows = blockDim.x / lanes;
   const bool gated = p.gate && !p.gate_row;
   Reducer red{slots, lanes, 0};
-  float weight[E], scale[E], next_weight[E];
+  Pairs weight, scale, next_weight;
   X::param(weight, p.param[0], p.param_dtype[0], 1.f, c, t, lanes);
   X::param(scale, p.param[2], p.param_dtype[2], 1.f, c, t, lanes);
   X::param(next_weight, p.param[3], p.param_dtype[3], 1.f, c, t, lanes);
@@ -264,7 +261,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) forward_kerne
   for (int64_t base = first; base < p.n; base += step) {
     const int64_t row = base + mine;
     const bool active = row < p.n;
-    float out[E], b[E], g[E];
+    Pairs out, b, g;
     float mean = 0.f, inv = 1.f;
     X::values(out, raw_x);
     if (p.block) X::values(b, raw_b);
@@ -273,36 +270,37 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) forward_kerne
     if (base + step < p.n) fetch(row + step);
     if (p.block) {
       if (p.param[0]) {
-        statistics<CENTER, VEC, NV>(b, red, c, t, p.eps, mean, inv);
+        statistics<X, CENTER>(b, red, c, t, p.eps, mean, inv);
 #pragma unroll
-        for (int e = 0; e < E; ++e) b[e] = (b[e] - mean) * inv * weight[e];
+        for (int k = 0; k < P; ++k) b[k] = mul2(CENTER ? fma2(b[k], pair(inv), pair(-mean * inv)) : mul2(b[k], pair(inv)), weight[k]);
         if (BIAS && p.param[1]) {
-          float w[E];
+          Pairs w;
           X::param(w, p.param[1], p.param_dtype[1], 0.f, c, t, lanes);
 #pragma unroll
-          for (int e = 0; e < E; ++e) b[e] += w[e];
+          for (int k = 0; k < P; ++k) b[k] = add2(b[k], w[k]);
         }
       }
       if (p.stats && t == 0 && active) *(float2*)(p.stats + row * 4) = make_float2(mean, inv);
 #pragma unroll
-      for (int e = 0; e < E; ++e) out[e] = fmaf(scale[e] * (gated ? sigmoid<T>(g[e]) : rg), b[e], out[e]);
+      for (int k = 0; k < P; ++k) out[k] = fma2(mul2(scale[k], gated ? sigmoid<T>(g[k]) : pair(rg)), b[k], out[k]);
       if (p.out) X::store(out, p.out, row, c, t, lanes, active);
     }
     if (p.normed) {
+      if (BIAS || CENTER) {                                         // what a bias, or a mean, left behind the row's end
 #pragma unroll
-      for (int j = 0; j < NV; ++j)                                  // what a bias added behind the row's end
-        if (BIAS && X::column(j, t, lanes) >= c) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) out[j * VEC + i] = 0.f;
+        for (int k = 0; k < P; ++k) {
+          if (!X::inside(2 * k, c, t, lanes)) out[k].x = 0.f;
+          if (!X::inside(2 * k + 1, c, t, lanes)) out[k].y = 0.f;
         }
-      statistics<CENTER, VEC, NV>(out, red, c, t, p.eps, mean, inv);
+      }
+      statistics<X, CENTER>(out, red, c, t, p.eps, mean, inv);
       if (p.stats && t == 0 && active) *(float2*)(p.stats + row * 4 + 2) = make_float2(mean, inv);
 #pragma unroll
-      for (int e = 0; e < E; ++e) out[e] = (out[e] - mean) * inv * next_weight[e];
+      for (int k = 0; k < P; ++k) out[k] = mul2(CENTER ? fma2(out[k], pair(inv), pair(-mean * inv)) : mul2(out[k], pair(inv)), next_weight[k]);
       if (BIAS && p.param[4]) {
         X::param(b, p.param[4], p.param_dtype[4], 0.f, c, t, lanes);
 #pragma unroll
-        for (int e = 0; e < E; ++e) out[e] += b[e];
+        for (int k = 0; k < P; ++k) out[k] = add2(out[k], b[k]);
       }
       X::store(out, p.normed, row, c, t, lanes, active);
     }
@@ -312,7 +310,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) forward_kerne
 template <typename T, int VEC, int NV, bool CENTER, bool BIAS, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) backward_kernel(const __grid_constant__ Params p) {
   using X = Tile<T, VEC, NV>;
-  constexpr int E = X::E;
+  constexpr int E = X::E, P = X::P;
+  using Pairs = typename X::Pairs;
   __shared__ float slots[2][kMaxWarps][4];
   extern __shared__ float columns[];                                // rows of a block > 1: [kBlock][E]
   after_previous();
@@ -320,15 +319,15 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) backward_kern
   const bool gated = p.gate && !p.gate_row;
   const float per_c = 1.f / (float)c;
   Reducer red{slots, lanes, 0};
-  float weight[E], scale[E], next_weight[E];
+  Pairs weight, scale, next_weight;
   X::param(weight, p.param[0], p.param_dtype[0], 1.f, c, t, lanes);
   X::param(scale, p.param[2], p.param_dtype[2], 1.f, c, t, lanes);
   X::param(next_weight, p.param[3], p.param_dtype[3], 1.f, c, t, lanes);
-  float sums[kSums][E];
+  float2 sums[kSums][P];
 #pragma unroll
   for (int s = 0; s < kSums; ++s)
 #pragma unroll
-    for (int e = 0; e < E; ++e) sums[s][e] = 0.f;
+    for (int k = 0; k < P; ++k) sums[s][k] = pair(0.f);
   typename X::Raw raw_x, raw_b, raw_g, raw_d, raw_n;
   typename Row<T>::Bits raw_rg = 0;
   float4 raw_st = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -348,7 +347,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) backward_kern
   for (int64_t base = first; base < p.n; base += step) {
     const int64_t row = base + mine;
     const bool active = row < p.n;
-    float x[E], b[E], g[E], total[E], dn[E];
+    Pairs x, b, g, total, dn;
     const float4 st = raw_st;
     const float mb = p.param[0] ? st.x : 0.f, ib = p.param[0] ? st.y : 1.f;
     const float rg = p.gate && !gated ? sigmoid<T>(Row<T>::get(raw_rg)) : 1.f;
@@ -359,71 +358,82 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) backward_kern
       X::values(total, raw_d);
     } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) total[e] = 0.f;
+      for (int k = 0; k < P; ++k) total[k] = pair(0.f);
     }
     if (p.d_normed) X::values(dn, raw_n);
     if (base + step < p.n) fetch(row + step);
-    float bias[E];                                                  // in a register only where there is one
+    Pairs bias;                                                     // in registers only where there is one
     if (BIAS) X::param(bias, p.param[1], p.param_dtype[1], 0.f, c, t, lanes);
-    if (p.block) {                                                  // b: the normalised block; x: out
+    auto inner = [&](int k) { return BIAS ? fma2(b[k], weight[k], bias[k]) : mul2(b[k], weight[k]); };
+    if (p.block) {                                                  // b: the normalised block
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        b[e] = (b[e] - mb) * ib;
-        g[e] = gated ? sigmoid<T>(g[e]) : rg;
+      for (int k = 0; k < P; ++k) {
+        b[k] = CENTER ? fma2(b[k], pair(ib), pair(-mb * ib)) : mul2(b[k], pair(ib));
+        g[k] = gated ? sigmoid<T>(g[k]) : pair(rg);
       }
     }
     if (p.d_normed) {
-      float s[2] = {0.f, 0.f};
+      float2 s0 = pair(0.f), s1 = pair(0.f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (p.block) x[e] = fmaf(scale[e] * g[e], BIAS ? fmaf(b[e], weight[e], bias[e]) : b[e] * weight[e], x[e]);
-        x[e] = (x[e] - st.z) * st.w;                                // the normalised out; dn is zero behind the row's end
-        sums[3][e] = fmaf(dn[e], x[e], sums[3][e]);
-        if (BIAS) sums[4][e] += dn[e];
-        dn[e] *= next_weight[e];
-        s[0] = fmaf(dn[e], x[e], s[0]);
-        s[1] += dn[e];
+      for (int k = 0; k < P; ++k) {
+        if (p.block) x[k] = fma2(mul2(scale[k], g[k]), inner(k), x[k]);
+        x[k] = CENTER ? fma2(x[k], pair(st.w), pair(-st.z * st.w)) : mul2(x[k], pair(st.w));        // the normalised out; dn is zero behind the row
+        sums[3][k] = fma2(dn[k], x[k], sums[3][k]);
+        if (BIAS) sums[4][k] = add2(sums[4][k], dn[k]);
+        dn[k] = mul2(dn[k], next_weight[k]);
+        s0 = fma2(dn[k], x[k], s0);
+        if (CENTER) s1 = add2(s1, dn[k]);
       }
+      float s[CENTER ? 2 : 1];
+      s[0] = both(s0);
+      if (CENTER) s[CENTER] = both(s1);
       red.sum(s);
-      s[0] *= per_c;
-      s[1] = CENTER ? s[1] * per_c : 0.f;
+      const float2 along = pair(-st.w * s[0] * per_c), across = pair(CENTER ? -st.w * s[CENTER] * per_c : 0.f);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const bool inside = X::column(j, t, lanes) < c;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const int e = j * VEC + i;
-          total[e] = inside ? fmaf(st.w, dn[e] - s[1] - x[e] * s[0], total[e]) : 0.f;
-        }
+      for (int k = 0; k < P; ++k) {
+        total[k] = fma2(dn[k], pair(st.w), fma2(x[k], along, total[k]));
+        if (CENTER) total[k] = add2(total[k], across);
+        if (!X::inside(2 * k, c, t, lanes)) total[k].x = 0.f;
+        if (!X::inside(2 * k + 1, c, t, lanes)) total[k].y = 0.f;
       }
     }
     if (p.d_residual) X::store(total, p.d_residual, row, c, t, lanes, active);
     if (p.block) {
-      float s[3] = {0.f, 0.f, 0.f};
+      float2 s0 = pair(0.f), s1 = pair(0.f), s2 = pair(0.f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float inner = BIAS ? fmaf(b[e], weight[e], bias[e]) : b[e] * weight[e];
-        const float tg = total[e] * g[e];                           // gradient of scale * inner
-        const float d_inner = tg * scale[e];
-        sums[2][e] = fmaf(tg, inner, sums[2][e]);
-        sums[0][e] = fmaf(d_inner, b[e], sums[0][e]);
-        if (BIAS) sums[1][e] += d_inner;
-        x[e] = d_inner * inner * (1.f - g[e]);                      // gradient of the gate's logit
-        s[2] += x[e];
-        dn[e] = d_inner * weight[e];
-        s[0] = fmaf(dn[e], b[e], s[0]);
-        s[1] += dn[e];
+      for (int k = 0; k < P; ++k) {
+        const float2 in = inner(k), tg = mul2(total[k], g[k]), d_inner = mul2(tg, scale[k]);         // tg: gradient of scale * inner
+        sums[2][k] = fma2(tg, in, sums[2][k]);
+        sums[0][k] = fma2(d_inner, b[k], sums[0][k]);
+        if (BIAS) sums[1][k] = add2(sums[1][k], d_inner);
+        x[k] = mul2(d_inner, in);                                   // gradient of the gate's logit
+        x[k] = fma2(mul2(x[k], g[k]), pair(-1.f), x[k]);
+        s2 = add2(s2, x[k]);
+        dn[k] = mul2(d_inner, weight[k]);
+        s0 = fma2(dn[k], b[k], s0);
+        if (CENTER) s1 = add2(s1, dn[k]);
       }
       if (gated && p.d_gate) X::store(x, p.d_gate, row, c, t, lanes, active);
-      if (p.param[0] || p.gate_row) {
-        red.sum(s);
-        if (p.gate_row && p.d_gate && t == 0 && active) ((typename Row<T>::Bits*)p.d_gate)[row] = Row<T>::put(s[2]);
+      float s[3] = {both(s0), both(s2), CENTER ? both(s1) : 0.f};
+      if (CENTER) {
+        if (p.param[0] || p.gate_row) red.sum(s);
+      } else if (p.gate_row) {
+        float u[2] = {s[0], s[1]};
+        red.sum(u);
+        s[0] = u[0]; s[1] = u[1];
+      } else if (p.param[0]) {
+        float u[1] = {s[0]};
+        red.sum(u);
+        s[0] = u[0];
       }
+      if (p.gate_row && p.d_gate && t == 0 && active) ((typename Row<T>::Bits*)p.d_gate)[row] = Row<T>::put(s[1]);
       if (p.param[0]) {
-        s[0] *= per_c;
-        s[1] = CENTER ? s[1] * per_c : 0.f;
+        const float2 along = pair(-ib * s[0] * per_c), across = pair(CENTER ? -ib * s[2] * per_c : 0.f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) dn[e] = ib * (dn[e] - s[1] - b[e] * s[0]);
+        for (int k = 0; k < P; ++k) {
+          dn[k] = fma2(dn[k], pair(ib), mul2(b[k], along));
+          if (CENTER) dn[k] = add2(dn[k], across);
+        }
       }
       if (p.d_block) X::store(dn, p.d_block, row, c, t, lanes, active);
     }
@@ -437,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) backward_kern
     if (rows > 1) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < E; ++e) columns[e * kBlock + threadIdx.x] = sums[s][e];
+      for (int e = 0; e < E; ++e) columns[e * kBlock + threadIdx.x] = e % 2 ? sums[s][e / 2].y : sums[s][e / 2].x;
       __syncthreads();
       for (int i = threadIdx.x; i < lanes * E; i += blockDim.x) {
         const int e = i / lanes, tt = i - e * lanes;
@@ -452,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) backward_kern
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int at = X::column(e / VEC, t, lanes) + e % VEC;
-        if (at < c) to[at] = sums[s][e];
+        if (at < c) to[at] = e % 2 ? sums[s][e / 2].y : sums[s][e / 2].x;
       }
     }
   }
