@@ -21,7 +21,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kVec = 8;                       // values a thread takes at a time: 16 bytes of a 16-bit type, 32 of float
 constexpr int kBatch = 128;                   // ranges of a launch: their table is the kernel's argument (4 KB at most)
-constexpr int kBlocksPerSm = 8;
+constexpr int kBlocksPerSm = 6;
 
 struct Ranges {
   const void* src[kBatch];
@@ -36,9 +36,10 @@ static_assert(sizeof(Ranges) <= 4000, "kernel arguments are limited");
 struct Piece {                                // one chunk of a range
   const void* src;
   void* dst;
-  int64_t begin, end;
+  int n;
   int src_dtype, dst_dtype;
 };
+__device__ __forceinline__ int bytes_of(int dtype) { return dtype == SPH_F32 ? 4 : 2; }
 __device__ __forceinline__ Piece piece_of(const Ranges& r, int chunk) {
   int lo = 0, hi = r.count - 1;
   while (lo < hi) {
@@ -46,77 +47,129 @@ __device__ __forceinline__ Piece piece_of(const Ranges& r, int chunk) {
     if (r.first[mid] <= chunk) lo = mid; else hi = mid - 1;
   }
   Piece p;
-  p.src = r.src[lo];
-  p.dst = r.dst[lo];
-  p.begin = (int64_t)(chunk - r.first[lo]) * r.chunk;
-  p.end = min(r.n[lo], p.begin + r.chunk);
+  const int64_t begin = (int64_t)(chunk - r.first[lo]) * r.chunk;
   p.src_dtype = r.dtypes[lo] & 15;
   p.dst_dtype = r.dtypes[lo] >> 4;
+  p.src = (const char*)r.src[lo] + begin * bytes_of(p.src_dtype);
+  p.dst = (char*)r.dst[lo] + begin * bytes_of(p.dst_dtype);
+  p.n = (int)min(r.n[lo] - begin, (int64_t)r.chunk);
   return p;
 }
 
-__device__ __forceinline__ float widen(unsigned short bits, int dtype) {
-  return dtype == SPH_F16 ? __half2float(__ushort_as_half(bits)) : __uint_as_float((unsigned)bits << 16);
-}
-__device__ __forceinline__ unsigned short narrow(float v, int dtype) {
-  return dtype == SPH_F16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
-}
+__device__ __forceinline__ bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// Values i .. i+7 of a range (0 behind its end).  Plain loads: src may be dst.
-__device__ __forceinline__ void load8(float (&v)[kVec], const void* src, int dtype, int64_t i, int64_t end) {
-  const bool whole = i + kVec <= end;
-  if (dtype == SPH_F32) {
-    const float* s = (const float*)src + i;
-    if (whole && ((uintptr_t)s & 15) == 0) {
-      const float4 a = *(const float4*)s, b = *(const float4*)(s + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
+// 8 values of a type, as they lie in memory.  Plain loads: src may be dst.
+template <int DTYPE>
+struct Eight {
+  static constexpr int kWords = DTYPE == SPH_F32 ? 8 : 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void fetch(const void* src, int i) {                // 16-byte aligned
+    const uint4* s = (const uint4*)((const char*)src + (size_t)i * (DTYPE == SPH_F32 ? 4 : 2));
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) v[j] = i + j < end ? s[j] : 0.f;
-    }
-  } else {
-    const unsigned short* s = (const unsigned short*)src + i;
-    if (whole && ((uintptr_t)s & 15) == 0) {
-      const uint4 a = *(const uint4*)s;
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = widen((unsigned short)(w[j] & 0xffffu), dtype);
-        v[2 * j + 1] = widen((unsigned short)(w[j] >> 16), dtype);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) v[j] = i + j < end ? widen(s[j], dtype) : 0.f;
+    for (int j = 0; j < kWords / 4; ++j) {
+      const uint4 a = s[j];
+      w[4 * j] = a.x; w[4 * j + 1] = a.y; w[4 * j + 2] = a.z; w[4 * j + 3] = a.w;
     }
   }
+  __device__ __forceinline__ void fetch_some(const void* src, int i, int n) {    // any alignment, 0 from n on
+    if (DTYPE == SPH_F32) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) w[j % kWords] = i + j < n ? ((const uint32_t*)src)[i + j] : 0u;
+    } else {
+      const unsigned short* s = (const unsigned short*)src + i;
+#pragma unroll
+      for (int j = 0; j < kVec / 2; ++j)
+        w[j] = (i + 2 * j < n ? (uint32_t)s[2 * j] : 0u) | (i + 2 * j + 1 < n ? (uint32_t)s[2 * j + 1] << 16 : 0u);
+    }
+  }
+  __device__ __forceinline__ void values(float (&v)[kVec]) const {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      if (DTYPE == SPH_F32) {
+        v[j] = __uint_as_float(w[j % kWords]);
+      } else if (DTYPE == SPH_BF16) {
+        v[j] = __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+      } else {
+        const float2 f = __half22float2(*(const __half2*)&w[j / 2]);
+        v[j] = j & 1 ? f.y : f.x;
+      }
+    }
+  }
+};
+
+// f(values, place of the first) for every 8 values of a piece that are this thread's, kAhead times as many asked for at once.
+constexpr int kAhead = 4;
+template <int DTYPE, typename F>
+__device__ __forceinline__ void each(const Piece& p, F f) {
+  constexpr int step = kThreads * kVec;
+  int i = (int)threadIdx.x * kVec;
+  float v[kVec];
+  if (aligned(p.src)) {
+    const int last = p.n - kVec;              // the last place of 8 values
+    for (; i + (kAhead - 1) * step <= last; i += kAhead * step) {
+      Eight<DTYPE> r[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) r[a].fetch(p.src, i + a * step);
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        r[a].values(v);
+        f(v, i + a * step);
+      }
+    }
+#pragma unroll 1
+    for (; i <= last; i += step) {
+      Eight<DTYPE> r;
+      r.fetch(p.src, i);
+      r.values(v);
+      f(v, i);
+    }
+  }
+#pragma unroll 1
+  for (; i < p.n; i += step) {
+    Eight<DTYPE> r;
+    r.fetch_some(p.src, i, p.n);
+    r.values(v);
+    f(v, i);
+  }
+}
+template <typename F>
+__device__ __forceinline__ void each(const Piece& p, F f) {
+  if (p.src_dtype == SPH_F32) each<SPH_F32>(p, f);
+  else if (p.src_dtype == SPH_F16) each<SPH_F16>(p, f);
+  else each<SPH_BF16>(p, f);
 }
 
-__device__ __forceinline__ void store8(const float (&v)[kVec], void* dst, int dtype, int64_t i, int64_t end) {
-  const bool whole = i + kVec <= end;
-  if (dtype == SPH_F32) {
-    float* d = (float*)dst + i;
-    if (whole && ((uintptr_t)d & 15) == 0) {
+__device__ __forceinline__ uint32_t narrow(float a, float b, int dtype) {
+  if (dtype == SPH_F16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *(const uint32_t*)&h;
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *(const uint32_t*)&h;
+}
+// Values i .. i+7 of a piece, those that there are.
+__device__ __forceinline__ void store8(const float (&v)[kVec], const Piece& p, int i, bool dst_aligned) {
+  if (p.dst_dtype == SPH_F32) {
+    float* d = (float*)p.dst + i;
+    if (dst_aligned && i + kVec <= p.n) {
       *(float4*)d = make_float4(v[0], v[1], v[2], v[3]);
       *(float4*)(d + 4) = make_float4(v[4], v[5], v[6], v[7]);
     } else {
 #pragma unroll
       for (int j = 0; j < kVec; ++j)
-        if (i + j < end) d[j] = v[j];
+        if (i + j < p.n) d[j] = v[j];
     }
   } else {
-    unsigned short* d = (unsigned short*)dst + i;
-    unsigned short h[kVec];
+    unsigned short* d = (unsigned short*)p.dst + i;
+    uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) h[j] = narrow(v[j], dtype);
-    if (whole && ((uintptr_t)d & 15) == 0) {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = (uint32_t)h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
+    for (int j = 0; j < 4; ++j) w[j] = narrow(v[2 * j], v[2 * j + 1], p.dst_dtype);
+    if (dst_aligned && i + kVec <= p.n) {
       *(uint4*)d = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
 #pragma unroll
       for (int j = 0; j < kVec; ++j)
-        if (i + j < end) d[j] = h[j];
+        if (i + j < p.n) d[j] = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
     }
   }
 }
@@ -140,15 +193,12 @@ __device__ double block_join(double v) {
 }
 
 template <bool MAX>
-__global__ void __launch_bounds__(kThreads) norm_partials_kernel(const __grid_constant__ Ranges r, double* partial) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) norm_partials_kernel(const __grid_constant__ Ranges r, double* partial) {
   after_previous();
   double sum = 0.0;
   for (int c = blockIdx.x; c < r.chunks; c += gridDim.x) {
     const Piece p = piece_of(r, c);
-    int64_t i = p.begin + (int64_t)threadIdx.x * kVec;
-    for (; i < p.end; i += (int64_t)kThreads * kVec) {
-      float v[kVec];
-      load8(v, p.src, p.src_dtype, i, p.end);
+    each(p, [&](float (&v)[kVec], int) {
       if (MAX) {
         unsigned top = 0u;                    // as integers |NaN| is above infinity
 #pragma unroll
@@ -165,7 +215,7 @@ __global__ void __launch_bounds__(kThreads) norm_partials_kernel(const __grid_co
           for (int j = 0; j < kVec; ++j) sum = fma((double)v[j], (double)v[j], sum);
         }
       }
-    }
+    });
   }
   sum = block_join<MAX>(sum);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
@@ -187,7 +237,7 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* partial, i
 }
 
 template <bool MAX>
-__global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ Ranges r, const double* partial, int n, float max_norm,
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) clip_kernel(const __grid_constant__ Ranges r, const double* partial, int n, float max_norm,
                                                         float* norm) {
   after_previous();
   const float total = total_norm<MAX>(partial, n);
@@ -197,14 +247,12 @@ __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ 
   for (int c = r.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
     const Piece p = piece_of(r, c);
     if (by == 1.f && p.src == p.dst) continue;
-    int64_t i = p.begin + (int64_t)threadIdx.x * kVec;
-    for (; i < p.end; i += (int64_t)kThreads * kVec) {
-      float v[kVec];
-      load8(v, p.src, p.src_dtype, i, p.end);
+    const bool dst_aligned = aligned(p.dst);
+    each(p, [&](float (&v)[kVec], int i) {
 #pragma unroll
       for (int j = 0; j < kVec; ++j) v[j] *= by;
-      store8(v, p.dst, p.dst_dtype, i, p.end);
-    }
+      store8(v, p, i, dst_aligned);
+    });
   }
 }
 
@@ -233,10 +281,11 @@ int64_t take(const sph_clip_tensor* t, int32_t count, int32_t* at, bool with_dst
     }
     total += x.n;
   }
-  // chunks that give every block a few of them, so that none is left with much more than the others
+  // chunks that give every block some of them, so that none is left with much more than the others
   constexpr int64_t unit = kThreads * kVec;
-  const int64_t per_block = total / ((int64_t)sms * kBlocksPerSm * 4);
-  r->chunk = (int32_t)std::min<int64_t>(16 * unit, std::max<int64_t>(unit, div_up64(per_block, unit) * unit));
+  const int64_t per_block = total / ((int64_t)sms * kBlocksPerSm * 6);
+  const int64_t whole = per_block >= kAhead * unit ? kAhead * unit : unit;
+  r->chunk = (int32_t)std::min<int64_t>(64 * unit, std::max<int64_t>(unit, div_up64(per_block, whole) * whole));
   int64_t chunks = 0;
   for (int k = 0; k < r->count; ++k) {
     r->first[k] = (int32_t)chunks;

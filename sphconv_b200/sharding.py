@@ -146,7 +146,6 @@ def _largest(norm_type: float) -> bool:
     return norm_type == math.inf
 
 
-@torch.no_grad()
 def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
     """sqrt(sum g^2) over every value of every tensor (norm_type 2), or max |g| (inf; NaN if any is): a float32 scalar on their
     device, nothing is read back.  float32, float16 and bfloat16 tensors, mixed; sums are held in 64 bits, in a fixed order."""
@@ -156,12 +155,12 @@ def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Te
         return _capi.host().grad_clip(grads, None, None, largest)
     if not grads:
         return torch.zeros(())
-    if largest:
-        return torch.stack([g.abs().max().float() if g.numel() else torch.zeros(()) for g in grads]).max()
-    return torch.stack([g.double().square().sum() for g in grads]).sum().sqrt().float()
+    with torch.no_grad():
+        if largest:
+            return torch.stack([g.abs().max().float() if g.numel() else torch.zeros(()) for g in grads]).max()
+        return torch.stack([g.double().square().sum() for g in grads]).sum().sqrt().float()
 
 
-@torch.no_grad()
 def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None,
                    norm_type: float = 2.0) -> torch.Tensor:
     """Every gradient times min(1, max_norm / (norm + 1e-6)), in place or into `out` (tensors of the same shapes, of any of the
@@ -179,9 +178,10 @@ def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, out: Optional
     if len({g.data_ptr() for g in grads if g.numel()}) < sum(g.numel() > 0 for g in grads):
         raise RuntimeError("a gradient is in the list twice")
     norm = grad_norm(grads, norm_type)
-    by = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
-    for g, o in zip(grads, grads if out is None else out):
-        o.copy_(g.float() * by)
+    with torch.no_grad():
+        by = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
+        for g, o in zip(grads, grads if out is None else out):
+            o.copy_(g.float() * by)
     return norm
 
 
