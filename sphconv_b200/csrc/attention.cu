@@ -22,6 +22,7 @@ namespace attn {
 constexpr int kTile = 64;
 constexpr int kThreads = 256;
 constexpr int kScorePitch = kTile + 4;
+constexpr int kMostParts = 64;                // of a walk: two lanes of a warp have them all
 
 template <typename T> __device__ __forceinline__ float to_float(T v);
 template <> __device__ __forceinline__ float to_float(float v) { return v; }
@@ -387,37 +388,64 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const T* d_out, const T
   }
 }
 
-// Parts of the forward pass: out = sum of 2^(lse_i - lse) part_i with lse = log2 of the sum of 2^lse_i; a warp a row.
-template <typename T>
+// Parts of the forward pass: out = sum of 2^(lse_i - lse) part_i with lse = log2 of the sum of 2^lse_i.  WARPS warps a row, that share the
+// parts; of a warp, lanes the parts' lse first, then the channels.
+template <typename T, int WARPS>
 __global__ void __launch_bounds__(kThreads) join_forward_kernel(const float* part, const float* part_lse, int splits, int64_t rows, int d,
                                                                 T* out, float* lse) {
+  constexpr int kRows = kThreads / 32 / WARPS;              // of a block
+  __shared__ float s_v[kThreads / 32][SPH_ATTENTION_MAX_CHANNELS];
   after_previous();
-  const int lane = threadIdx.x & 31;
-  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * (kThreads / 32)) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
+    const int64_t r = r0 + warp / WARPS;
+    const bool mine = r < rows;
+    float l[2];                                             // of parts lane and lane + 32; +inf: one without keys
     float top = -INFINITY;
     bool some = false;
-    for (int s = 0; s < splits; ++s) {
-      const float l = part_lse[(int64_t)s * rows + r];
-      if (l == INFINITY) continue;                                    // +inf: a part without keys
-      some = true;
-      top = l != l ? l : fmaxf(top, l);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int s = lane + 32 * i;
+      l[i] = mine && s < splits ? part_lse[(int64_t)s * rows + r] : INFINITY;
+      some |= l[i] != INFINITY;
+      top = fmaxf(top, l[i] == INFINITY ? -INFINITY : l[i]);          // NaN is left to the sum
     }
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    some = __any_sync(0xffffffffu, some);
     const float base = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
-    for (int s = 0; s < splits; ++s) {
-      const float l = part_lse[(int64_t)s * rows + r];
-      if (l != INFINITY) sum += exp2f(l - base);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] = l[i] == INFINITY ? 0.f : exp2f(l[i] - base);   // weights from here on
+      sum += l[i];
     }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float inv = some ? 1.f / sum : 0.f;
-    for (int c = lane; c < d; c += 32) {
-      float v = 0.f;
-      for (int s = 0; s < splits; ++s) {
-        const float l = part_lse[(int64_t)s * rows + r];
-        if (l != INFINITY) v = fmaf(exp2f(l - base) * inv, part[((int64_t)s * rows + r) * d + c], v);
-      }
-      out[r * d + c] = from_float<T>(v);
+    float v[SPH_ATTENTION_MAX_CHANNELS / 32] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = warp % WARPS; s < splits; s += WARPS) {
+      const float f = __shfl_sync(0xffffffffu, s < 32 ? l[0] : l[1], s & 31) * inv;
+      if (!mine || f == 0.f) continue;                      // a part without keys is not looked at
+#pragma unroll
+      for (int i = 0; i < SPH_ATTENTION_MAX_CHANNELS / 32; ++i)
+        if (lane + 32 * i < d) v[i] = fmaf(f, part[((int64_t)s * rows + r) * d + lane + 32 * i], v[i]);
     }
-    if (lane == 0 && lse) lse[r] = some ? base + log2f(sum) : INFINITY;
+    if (WARPS > 1) {
+#pragma unroll
+      for (int i = 0; i < SPH_ATTENTION_MAX_CHANNELS / 32; ++i) s_v[warp][lane + 32 * i] = v[i];
+      __syncthreads();
+      if (warp % WARPS == 0) {
+#pragma unroll
+        for (int i = 0; i < SPH_ATTENTION_MAX_CHANNELS / 32; ++i)
+          for (int x = 1; x < WARPS; ++x) v[i] += s_v[warp + x][lane + 32 * i];
+      }
+      __syncthreads();
+    }
+    if (mine && warp % WARPS == 0) {
+#pragma unroll
+      for (int i = 0; i < SPH_ATTENTION_MAX_CHANNELS / 32; ++i)
+        if (lane + 32 * i < d) out[r * d + lane + 32 * i] = from_float<T>(v[i]);
+      if (lane == 0 && lse) lse[r] = some ? base + log2f(sum) : INFINITY;
+    }
   }
 }
 
@@ -433,6 +461,9 @@ __global__ void __launch_bounds__(kThreads) join_sum_kernel(const float* part, i
 }
 
 int attention_forward_tc(const Params& p, bool bf16, int blocks, cudaStream_t st);      // attention_tc.cu
+// attention_decode.cu
+int attention_decode_rows(int dtype, int64_t rows);
+int attention_decode(const Params& p, int dtype, int rows, int blocks, cudaStream_t st);
 // attention_tc_bwd.cu
 int attention_backward_tc(const Params& p, bool bf16, bool keys, int blocks, cudaStream_t st);
 
@@ -449,20 +480,23 @@ int padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 int forward_smem(int dp) { return (3 * kTile * (dp + 4) + kTile * kScorePitch) * 4; }
 int backward_smem(int dp, bool keys) { return (4 * kTile * (dp + 4) + (keys ? 2 : 1) * kTile * kScorePitch) * 4; }
 
-// Parts that the walk of `blocks` blocks over `tiles` tiles each is split into, where `slots` blocks run at a time: what takes the
-// fewest rounds of tiles, with kStart tiles' time for a block to start and end, and that of writing and reading parts of `values`.
-int splits_for(int64_t blocks, int64_t slots, int64_t tiles, int64_t values) {
-  constexpr int64_t kStart = 8, kMost = 64, kValues = 500000;      // values of a part in a tile's time, 0.7 us
+// Parts that the walk of `blocks` blocks over `tiles` tiles each is split into, where `slots` blocks run at a time.  What it costs: the
+// tiles there are and the start of every block (`start` tiles' time), spread over the slots; half a part's time at the end, when some slots
+// have run out of work (scans differ in length: few large parts end far apart); and writing and reading parts of `values`, of which
+// `rate` are a tile's time.
+int splits_for(int64_t blocks, int64_t slots, int64_t tiles, int64_t values, double start, double rate) {
   int best = 1;
-  int64_t least = INT64_MAX;
-  for (int64_t s = 1; s <= std::min(kMost, std::max<int64_t>(1, tiles / 2)); ++s) {
-    const int64_t cost = div_up64(blocks * s, slots) * (div_up64(tiles, s) + kStart) + (s > 1 ? 4 + s * values / kValues : 0);
+  double least = 1e300;
+  for (int64_t s = 1; s <= std::min<int64_t>(kMostParts, std::max<int64_t>(1, tiles / 2)); ++s) {
+    const double part = (double)tiles / s + start;
+    const double cost = std::max(1.0, (double)(blocks * s) / slots) * part + 0.5 * part + (s > 1 ? start + s * (double)values / rate : 0.0);
     if (cost < least) { least = cost; best = (int)s; }
   }
   return best;
 }
 
 struct Plan {
+  int decode;                                // rows of a block of the decoding kernel; 0: another one runs forward
   int fwd_splits, dq_splits, dkv_splits;
   int fwd_blocks, dq_blocks, dkv_blocks;     // without the splits
 };
@@ -471,25 +505,31 @@ Plan plan_of(const sph_attention& a, const Params& params, int sms) {
   const int64_t room = 227 * 1024;
   auto per_sm = [&](int smem) { return std::min<int64_t>(room / (smem + 1024), 4); };
   Plan p;
-  const int64_t q_tiles = most_tiles(a.n_q * group, kTile, a.B), k_tiles = most_tiles(a.n_k, kTile, a.B);
-  p.fwd_blocks = p.dq_blocks = (int)(q_tiles * a.k_heads);
-  p.dkv_blocks = (int)(k_tiles * a.k_heads);
-  // tiles that there really are, if scans are of like length
   const int64_t B = std::max(a.B, 1);
+  const int64_t q_rows = a.n_q * group, q_values = a.n_q * a.q_heads * a.channels, k_values = 2 * a.n_k * a.k_heads * a.channels;
+  // tiles that there really are, if scans are of like length, and how many a block walks over
   auto real = [&](int64_t rows, int64_t size) { return std::max<int64_t>(1, div_up64(rows, size * B)) * B * a.k_heads; };
   auto walk = [&](int64_t rows, int64_t size) { return div_up64(rows, B * size); };
-  const int64_t q_rows = a.n_q * group, q_values = a.n_q * a.q_heads * a.channels, k_values = 2 * a.n_k * a.k_heads * a.channels;
-  if (on_tensor_cores(a, params)) {
+  if (on_tensor_cores(a, params)) {          // 0.7 us a tile; a block starts in 5 us, one that takes several tiles of rows in 2
+    constexpr double kRate = 500000;
     p.fwd_blocks = p.dq_blocks = most_tiles(q_rows, kTcTile, a.B) * a.k_heads;
     p.dkv_blocks = most_tiles(a.n_k, kTcTile, a.B) * a.k_heads;
-    p.fwd_splits = splits_for(real(q_rows, kTcTile), 2 * sms, walk(a.n_k, kTcStep), q_values);
-    p.dq_splits = splits_for(real(q_rows, kTcTile), sms, walk(a.n_k, kTcStep), q_values);
-    p.dkv_splits = splits_for(real(a.n_k, kTcTile), sms, walk(q_rows, kTcStep), k_values);
-    return p;
+    p.fwd_splits = splits_for(real(q_rows, kTcTile), 2 * sms, walk(a.n_k, kTcStep), q_values, 8, kRate);
+    p.dq_splits = splits_for(real(q_rows, kTcTile), sms, walk(a.n_k, kTcStep), q_values, 4, kRate);
+    p.dkv_splits = splits_for(real(a.n_k, kTcTile), sms, walk(q_rows, kTcStep), k_values, 4, kRate);
+  } else {                                   // 4 us a tile
+    constexpr double kRate = 3000000;
+    p.fwd_blocks = p.dq_blocks = most_tiles(q_rows, kTile, a.B) * a.k_heads;
+    p.dkv_blocks = most_tiles(a.n_k, kTile, a.B) * a.k_heads;
+    p.fwd_splits = splits_for(real(q_rows, kTile), sms * per_sm(forward_smem(dp)), walk(a.n_k, kTile), q_values, 1, kRate);
+    p.dq_splits = splits_for(real(q_rows, kTile), sms * per_sm(backward_smem(dp, false)), walk(a.n_k, kTile), q_values, 1, kRate);
+    p.dkv_splits = splits_for(real(a.n_k, kTile), sms * per_sm(backward_smem(dp, true)), walk(q_rows, kTile), k_values, 1, kRate);
   }
-  p.fwd_splits = splits_for(real(q_rows, kTile), sms * per_sm(forward_smem(dp)), walk(a.n_k, kTile), q_values);
-  p.dq_splits = splits_for(real(q_rows, kTile), sms * per_sm(backward_smem(dp, false)), walk(a.n_k, kTile), q_values);
-  p.dkv_splits = splits_for(real(a.n_k, kTile), sms * per_sm(backward_smem(dp, true)), walk(q_rows, kTile), k_values);
+  p.decode = params.vec ? attention_decode_rows(a.dtype, div_up64(q_rows, B)) : 0;
+  if (p.decode) {                            // steps of 64 keys
+    p.fwd_blocks = most_tiles(q_rows, p.decode, a.B) * a.k_heads;
+    p.fwd_splits = splits_for(real(q_rows, p.decode), 2 * sms, walk(a.n_k, 64), q_values, 1.5, 500000);
+  }
   return p;
 }
 
@@ -526,10 +566,15 @@ int run_forward(Params p, const Plan& plan, bool tensor_cores, void* scratch, cu
     p.part = (float*)scratch;
     p.part_lse = p.part + rows * p.d * p.splits;
   }
-  const int rc = tensor_cores ? attention_forward_tc(p, std::is_same<T, __nv_bfloat16>::value, plan.fwd_blocks * p.splits, st)
-                              : forward<T>(p, plan.fwd_blocks * p.splits, st);
+  constexpr int dtype = std::is_same<T, float>::value ? SPH_F32 : std::is_same<T, __half>::value ? SPH_F16 : SPH_BF16;
+  const int rc = plan.decode  ? attention_decode(p, dtype, plan.decode, plan.fwd_blocks * p.splits, st)
+                 : tensor_cores ? attention_forward_tc(p, std::is_same<T, __nv_bfloat16>::value, plan.fwd_blocks * p.splits, st)
+                                : forward<T>(p, plan.fwd_blocks * p.splits, st);
   if (rc != SPH_OK || p.splits == 1) return rc;
-  launch(join_forward_kernel<T>, grid_for(rows, kThreads / 32), kThreads, 0, st, p.part, p.part_lse, p.splits, rows, p.d, (T*)p.out, p.lse);
+  // a few rows leave most of the GPU to the parts of a row
+  constexpr int kWarps = kThreads / 32;
+  if (rows <= 148 * 4) launch(join_forward_kernel<T, kWarps>, grid_for(rows, 1), kThreads, 0, st, p.part, p.part_lse, p.splits, rows, p.d, (T*)p.out, p.lse);
+  else launch(join_forward_kernel<T, 1>, grid_for(rows, kWarps), kThreads, 0, st, p.part, p.part_lse, p.splits, rows, p.d, (T*)p.out, p.lse);
   SPH_LAUNCH_CHECK();
   return SPH_OK;
 }
@@ -588,8 +633,8 @@ int fill(const sph_attention* a, const char* who, Params* p) {
     set_error("%s: %d channels a head, at most %d are supported", who, a->channels, SPH_ATTENTION_MAX_CHANNELS);
     return SPH_ERR_LIMIT;
   }
-  // tiles and the rows of a scan (queries times heads) are numbered in 31 bits
-  const int64_t most = (int64_t)1 << 30;
+  // tiles, times their parts, and the rows of a scan (queries times heads) are numbered in 31 bits
+  const int64_t most = (int64_t)1 << 29;
   if (a->n_k > most || a->n_q * (a->q_heads / a->k_heads) > most || (a->n_q * a->q_heads / kTile + (a->B + 2ll) * a->k_heads) * 64 > most ||
       (a->n_k * a->k_heads / kTile + (a->B + 2ll) * a->k_heads) * 64 > most) {
     set_error("%s: too many rows", who);

@@ -93,6 +93,12 @@ __device__ __forceinline__ int2 split_rows(int n, int split, int splits, int siz
   return make_int2(first, min(n, first + per));
 }
 
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 inline int most_tiles(int64_t rows, int64_t size, int B) { return (int)(rows / size) + B + 2; }
 
 }  // namespace attn
