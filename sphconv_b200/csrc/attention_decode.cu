@@ -5,10 +5,10 @@
 // its own softmax - maximum, sum and O - over the keys it saw; they are joined at the end, over the warp, the block and, where the keys are
 // split over blocks, in a second launch.  The maximum follows only when a score is more than 2^8 above it.
 //
-// Per key and row 16 bytes a lane are 4 to 8 multiplications for S and as many for O, two an instruction: with up to 4 rows of 16-bit keys,
-// or 8 of float32, they fit beside the loads.  The sum over a key's lanes leaves each lane the scores of its share of the rows, whose
-// powers it takes alone and hands round.  One query over 87 k rows of 8 scans (4 rows of 64 channels a key head, bf16): 61 us with
-// the tensor cores' tiles of 128 rows, of which 4 are used, DECODE_US us here.
+// The sum over a key's lanes leaves each lane the scores of its share of the rows, whose powers it takes alone and hands round.
+// One query over 87 k rows of 8 scans, 8 key heads of 64 channels, bf16: 235 us, 6.1 TB/s.  With 4 rows a key head the instructions take
+// longer than the loads (2 key heads: 95 us, on the tensor cores, whose tiles of 128 rows then have 4, 84; 128 channels 170 and 139),
+// so 16-bit keys come here for one row only; float32, whose other kernel has tiles of 64 rows on the CUDA cores, for up to 8.
 #include <algorithm>
 
 #include "attention.cuh"
@@ -298,16 +298,11 @@ int start(const Params& p, int blocks, cudaStream_t st) {
 }  // namespace
 
 // Most query rows of a block, for `rows` of a scan and key head on average; 0: too many for this kernel.
-int attention_decode_rows(int dtype, int64_t rows) {
-  if (rows <= 1) return 1;
-  if (dtype == SPH_F32) return rows <= 8 ? 8 : 0;
-  return rows <= 4 ? 4 : 0;
-}
+int attention_decode_rows(int dtype, int64_t rows) { return rows <= 1 ? 1 : dtype == SPH_F32 && rows <= 8 ? 8 : 0; }
 
 int attention_decode(const Params& p, int dtype, int rows, int blocks, cudaStream_t st) {
   if (dtype == SPH_F32) return rows == 1 ? start<float, 1>(p, blocks, st) : start<float, 8>(p, blocks, st);
-  if (dtype == SPH_F16) return rows == 1 ? start<__half, 1>(p, blocks, st) : start<__half, 4>(p, blocks, st);
-  return rows == 1 ? start<__nv_bfloat16, 1>(p, blocks, st) : start<__nv_bfloat16, 4>(p, blocks, st);
+  return dtype == SPH_F16 ? start<__half, 1>(p, blocks, st) : start<__nv_bfloat16, 1>(p, blocks, st);
 }
 
 }  // namespace attn

@@ -137,19 +137,21 @@ __device__ __forceinline__ void load_rows(uint32_t to, int t, int n, int d, cons
   }
 }
 
-// 16 accumulator values times `by` to 16-bit or float32 memory that is 16-byte aligned in steps of 8 (16-bit) or 4 values.
+// 16 accumulator values times `by` to 16-bit or float32 memory that is 16-byte aligned in steps of 8 (16-bit) or 4 values; all 16 of a
+// 16-bit type in one store where the address is a multiple of 32.
 template <bool BF16>
 __device__ __forceinline__ void store16(const uint32_t (&v)[16], float by, void* to, int n) {       // n: of them, a multiple of 8
-  uint4* dst = (uint4*)to;
+  uint32_t w[8];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (8 * i >= n) break;
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      w[j] = pack2<BF16>(__uint_as_float(v[8 * i + 2 * j]) * by, __uint_as_float(v[8 * i + 2 * j + 1]) * by);
-    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int j = 0; j < 8; ++j) w[j] = pack2<BF16>(__uint_as_float(v[2 * j]) * by, __uint_as_float(v[2 * j + 1]) * by);
+  if (n >= 16 && ((uintptr_t)to & 31) == 0) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+    return;
   }
+  ((uint4*)to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  if (n >= 16) ((uint4*)to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 __device__ __forceinline__ void store16_float(const uint32_t (&v)[16], float by, float* to, int n) {
   float4* dst = (float4*)to;

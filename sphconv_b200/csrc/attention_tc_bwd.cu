@@ -28,7 +28,7 @@ namespace attn {
 namespace {
 
 constexpr int kC = 64;                        // columns of a tile
-constexpr int kRowWarps = 8, kScoreWarp = 8, kGradWarp = 10, kColumnWarp = 12, kRowLoadWarp = 13;
+constexpr int kRowWarps = 8, kScoreWarp = 8, kGradWarp = 10, kColumnWarp = 12;
 constexpr int kThreadsTc = 14 * 32;
 constexpr float kShiftP = 12.f;               // fp16: P times 2^12
 constexpr float kMostDs = 49152.f, kAimDs = 512.f;    // fp16: dS is scaled to the latter when it would pass the former
@@ -187,11 +187,34 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
     const int r = quarter * 32 + lane;
     constexpr float kShift = BF16 ? 0.f : kShiftP;
     float *stat_lse = s_stat[warp][0], *stat_delta = s_stat[warp][1];
-#pragma unroll 1
-    for (int index = blockIdx.x; index < items && !dead; index += gridDim.x) {
-      const Item it = find_item<KEYS>(p, index);
-      if (it.w.scan < 0) continue;
+    float next[4];                            // -lse and -delta of the columns of this warp's next tile: lane and lane + 32
+    auto fetch = [&](const Item& it, int j) {
       const Rows at{p, it};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = it.first + j * kC + 32 * i + lane;
+        const bool some = j < it.tiles && c < it.last;
+        const int64_t q = some ? at.query(c) : 0;
+        next[i] = some ? kShift - p.lse[q] : -INFINITY;
+        next[2 + i] = some ? -p.delta[q] : 0.f;
+      }
+    };
+    // tiles alternate between the halves from the start on: the first one of this warp in a tile of rows that g tiles lie in front of
+    auto first_tile = [&](int before) { return (before ^ half) & 1; };
+    Item it = find_item<KEYS>(p, blockIdx.x), following;
+    if (KEYS) fetch(it, first_tile(0));
+#pragma unroll 1
+    for (int index = blockIdx.x; index < items && !dead; index += gridDim.x, it = following) {
+      const Rows at{p, it};
+      // what follows is looked for while this one is worked on
+      auto look_ahead = [&]() {
+        following = find_item<KEYS>(p, index + gridDim.x);
+        if (KEYS) fetch(following, first_tile(g + it.tiles));
+      };
+      if (it.w.scan < 0) {
+        look_ahead();
+        continue;
+      }
       const bool any_row = quarter * 32 < it.rows, mine = r < it.rows;
       const bool row_is = mine && (!KEYS || at.is_key(it.row0 + r));  // a key, or a query
       float lse = -INFINITY, delta = 0.f;     // minus the row's; -infinity: P = 0
@@ -201,20 +224,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
         delta = -p.delta[q];
       }
       const float row_lse[4] = {lse, lse, lse, lse}, row_delta[4] = {delta, delta, delta, delta};
-      float next[4];                          // the columns' of this warp's next tile: lane and lane + 32
-      auto fetch = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int c = it.first + j * kC + 32 * i + lane;
-          const bool some = j < it.tiles && c < it.last;
-          const int64_t q = some ? at.query(c) : 0;
-          next[i] = some ? kShift - p.lse[q] : -INFINITY;
-          next[2 + i] = some ? -p.delta[q] : 0.f;
-        }
-      };
-      // this warp's first tile: tiles alternate between the halves from the start on
-      const int j0 = (g ^ half) & 1;
-      if (KEYS) fetch(j0);
+      const int j0 = first_tile(g);
       float& row_f = s_f[n & 1][r];
 #pragma unroll 1
       for (int j = j0; j < it.tiles; j += 2) {
@@ -228,7 +238,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
           stat_lse[lane] = next[0]; stat_lse[lane + 32] = next[1];
           stat_delta[lane] = next[2]; stat_delta[lane + 32] = next[3];
           __syncwarp();
-          fetch(j + 2);
+          fetch(it, j + 2);
         }
         if (!warp_wait(smem_u32(&s_s_full[b]), phase, abort_flag)) { dead = true; break; }
         const uint32_t at_s = lanes + S::s_at(b), at_dp = lanes + S::dp_at(b);
@@ -310,6 +320,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
         if (one) mbar_arrive(smem_u32(&s_p_full[b]));
       }
       // ---- results: KEYS: the first half has dV, the second dK; else each has half of dQ
+      look_ahead();
       if (!dead && it.tiles > 0) dead = !warp_wait(smem_u32(&s_all), (uint32_t)n & 1u, abort_flag);
       if (!dead && any_row) {
         tc_fence_after();
