@@ -106,9 +106,20 @@ struct Row {
   __device__ __forceinline__ int64_t out(const Params& p) const { return q * p.hq + h; }
 };
 
-// The query rows of a tile to shared memory; the warp's arrival included.
-template <int THREADS>
-__device__ __forceinline__ void load_queries(uint32_t to, int t, int rows, const Params& p, const Work& w, int head, uint32_t bar, bool one) {
+// The query rows of a tile to shared memory; the warp's arrival included.  Behind the last of them TMA may bring anything: it is a matter
+// of its own row's, which is not stored.
+template <int DP, int THREADS>
+__device__ __forceinline__ void load_queries(uint32_t to, int t, bool first, bool one, int rows, const Params& p, const TileMap& m, const Work& w,
+                                             int head, uint32_t bar) {
+  if (m.usable) {
+    if (one && first) {
+      mbar_arrive_expect_tx(bar, DP * kM * 2u);
+      tma_tile<DP>(to, kM * 128u, m, head * p.group, w.q0 + w.tile * (kM / p.group), bar);
+    } else if (one) {
+      mbar_arrive(bar);
+    }
+    return;
+  }
   load_rows<kM, THREADS>(to, t, rows, p.d, pieces_of(p.d), p.q, [&](int r) { return Row(p, w, head, r).query(p); }, [](int) { return true; });
   cp_async_arrive(bar);
   __syncwarp();
@@ -199,7 +210,8 @@ struct Shape {
 
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kThreadsTc, 2)
-forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ TileMap k_map, const __grid_constant__ TileMap v_map) {
+forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ TileMap q_map, const __grid_constant__ TileMap k_map,
+                  const __grid_constant__ TileMap v_map) {
   using S = Shape<DP>;
   constexpr int kStages = S::kStages;
   constexpr uint32_t kTileBytes = S::kTileBytes, kColS = S::kColS, kColO = S::kColO;
@@ -376,7 +388,7 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
       load_keys<DP, kLoaders>(k_at + st * kTileBytes, t, first, one, p, k_map, p.k, p.k_row, p.k_head, w, keys, part.head, j,
                                smem_u32(&s_k_full[st]));
       if (!S::kQInTmem && j == 0)
-        load_queries<kLoaders>(q_at, t, rows, p, w, part.head, smem_u32(&s_q_full), one);    // behind the first keys
+        load_queries<DP, kLoaders>(q_at, t, first, one, rows, p, q_map, w, part.head, smem_u32(&s_q_full));      // behind the first keys
       if (!warp_wait(smem_u32(&s_v_empty[st]), phase, abort_flag)) break;
       load_keys<DP, kLoaders>(v_at + st * kTileBytes, t, first, one, p, v_map, p.v, p.v_row, p.v_head, w, keys, part.head, j,
                                smem_u32(&s_v_full[st]));
@@ -397,11 +409,12 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
 
 template <int DP, bool BF16>
 int start(const Params& p, int blocks, cudaStream_t st) {
-  TileMap k_map, v_map;
+  TileMap q_map, k_map, v_map;
+  make_tile_map(&q_map, p.q, p.n_q, p.hq, p.d, p.q_row, p.q_head, kM, p.group);
   make_tile_map(&k_map, p.k, p.n_k, p.hkv, p.d, p.k_row, p.k_head, kN, 1);
   make_tile_map(&v_map, p.v, p.n_k, p.hkv, p.d, p.v_row, p.v_head, kN, 1);
   SPH_CUDA(allow_smem(forward_tc_kernel<DP, BF16>, Shape<DP>::kSmem));
-  launch(forward_tc_kernel<DP, BF16>, blocks, kThreadsTc, Shape<DP>::kSmem, st, p, k_map, v_map);
+  launch(forward_tc_kernel<DP, BF16>, blocks, kThreadsTc, Shape<DP>::kSmem, st, p, q_map, k_map, v_map);
   SPH_LAUNCH_CHECK();
   return SPH_OK;
 }

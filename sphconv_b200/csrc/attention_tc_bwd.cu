@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
   constexpr int PL = S::kPlaces, ST = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t s_r_full[2], s_r_empty[2], s_c_full[ST], s_c_empty[ST], s_s_full[PL], s_p_full[PL], s_done[PL];
-  __shared__ __align__(8) uint64_t s_all, s_free, s_turn[4][2];
+  __shared__ __align__(8) uint64_t s_all, s_free, s_some, s_turn[4][2];
   __shared__ __align__(16) float s_stat[kRowWarps][2][kC];  // of a warp's tile: -lse, -delta of the columns
   __shared__ float s_f[2][kM];                // fp16: dS of a row is held times this, of this tile of rows and the last; 0: not known yet
   __shared__ uint32_t s_tmem;
@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
     }
     mbar_init(smem_u32(&s_all), kGrads);
     mbar_init(smem_u32(&s_free), kRowWarps);
+    mbar_init(smem_u32(&s_some), 1);
     mbar_init_fence();
   }
   if (warp == kScoreWarp) {
@@ -434,6 +435,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
     // ======================= columns =======================
     const Pieces pc = pieces_of(p.d);
     const bool fit = KEYS ? m.q.usable && m.d_out.usable : m.k.usable && m.v.usable && p.mask == nullptr;
+    uint32_t ends = 0;                        // tiles with rows missing so far
 #pragma unroll 1
     for (int index = blockIdx.x; index < items && !dead; index += gridDim.x) {
       const Item it = find_item<KEYS>(p, index);
@@ -448,6 +450,24 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
             mbar_arrive_expect_tx(bar, 2 * S::kColBytes);
             tma_rows<DP, KEYS, 1>(to1, to2, m, p, it, first, bar);
           }
+          continue;
+        }
+        if (fit) {                            // the scan's last rows: what TMA brought behind them may be anything, and has to be zeros
+          const uint32_t some = smem_u32(&s_some);
+          if (one) {
+            mbar_arrive_expect_tx(some, 2 * S::kColBytes);
+            tma_rows<DP, KEYS, 1>(to1, to2, m, p, it, first, some);
+          }
+          __syncwarp();
+          if (!warp_wait(some, ends++ & 1u, abort_flag)) { dead = true; break; }
+          const int pieces = (kC - cols) * 8; // of a block of 64 channels: rows are 128 bytes there, in their order
+#pragma unroll
+          for (int x = 0; x < 2 * (DP / 64); ++x)
+            for (int i = lane; i < pieces; i += 32)
+              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(to1 + x * (kC * 128u) + (uint32_t)(cols * 128 + i * 16)), "r"(0) : "memory");
+          fence_proxy_async();
+          __syncwarp();
+          if (one) mbar_arrive(bar);
           continue;
         }
         if (KEYS) {
