@@ -22,6 +22,7 @@ namespace attn {
 constexpr int kTile = 64;
 constexpr int kThreads = 256;
 constexpr int kScorePitch = kTile + 4;
+constexpr int kTcTile = 128, kTcStep = 64;    // rows of a tile and of a step of its walk in the tensor-core kernels
 constexpr int kMostParts = 64;                // of a walk: two lanes of a warp have them all
 
 template <typename T> __device__ __forceinline__ float to_float(T v);
@@ -134,24 +135,11 @@ __device__ __forceinline__ void store_row(const float (&acc)[DP / 16], float by,
     }
 }
 
-// Work of a block: items of tiles, key heads, parts.
-struct Place {
-  int item, head, split;
-};
-__device__ __forceinline__ Place place_of(const Params& p) {
-  Place r;
-  r.split = blockIdx.x % p.splits;
-  const int i = blockIdx.x / p.splits;
-  r.head = i % p.hkv;
-  r.item = i / p.hkv;
-  return r;
-}
-
 template <bool QUERIES>
-__device__ __forceinline__ Work block_work(const Params& p, int item) {
+__device__ __forceinline__ Work block_work(const Params& p) {
   __shared__ Work s_work;
   if (threadIdx.x < 32) {
-    const Work w = find_work<QUERIES>(p, item, kTile);
+    const Work w = find_work<QUERIES>(p, blockIdx.x / p.hkv, kTile, kTile);
     if (threadIdx.x == 0) s_work = w;
   }
   __syncthreads();
@@ -178,14 +166,14 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   __shared__ uint8_t s_key[kTile];
   after_previous();
   check_scans(p);
-  const Place at = place_of(p);
-  const Work w = block_work<true>(p, at.item);
+  const int key_head = blockIdx.x % p.hkv;
+  const Work w = block_work<true>(p);
   if (w.scan < 0) return;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int rows = min(kTile, w.nq * p.group - w.tile * kTile);       // of the tile
   auto query = [&](int r, int* head) {
     const int i = w.tile * kTile + r;
-    *head = at.head * p.group + i % p.group;
+    *head = key_head * p.group + i % p.group;
     return w.q0 + i / p.group;
   };
   load_tile<T, DP>(s_q, p.d, p.vec, [&](int r) -> const T* {
@@ -193,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
     const int64_t q = query(min(r, rows - 1), &h);
     return r < rows ? (const T*)p.q + q * p.q_row + h * p.q_head : nullptr;
   });
-  const int2 keys = split_rows(w.nk, at.split, p.splits, kTile);
+  const int2 keys = make_int2(w.first, w.last);
   float o[4][DP / 16], top[4], sum[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -210,10 +198,10 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
     }
     __syncthreads();
     load_tile<T, DP>(s_k, p.d, p.vec, [&](int r) -> const T* {
-      return s_key[r] ? (const T*)p.k + (int64_t)(w.k0 + k0 + r) * p.k_row + at.head * p.k_head : nullptr;
+      return s_key[r] ? (const T*)p.k + (int64_t)(w.k0 + k0 + r) * p.k_row + key_head * p.k_head : nullptr;
     });
     load_tile<T, DP>(s_v, p.d, p.vec, [&](int r) -> const T* {
-      return s_key[r] ? (const T*)p.v + (int64_t)(w.k0 + k0 + r) * p.v_row + at.head * p.v_head : nullptr;
+      return s_key[r] ? (const T*)p.v + (int64_t)(w.k0 + k0 + r) * p.v_row + key_head * p.v_head : nullptr;
     });
     __syncthreads();
     float s[4][4];
@@ -256,9 +244,11 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
     const int64_t q = query(r, &h);
     const bool none = sum[i] == 0.f;
     const float by = none ? 0.f : 1.f / sum[i], lse = none ? INFINITY : top[i] + log2f(sum[i]);
-    if (p.splits > 1) {
-      store_row<float, DP>(o[i], by, p.part + (((int64_t)at.split * p.n_q + q) * p.hq + h) * p.d, p.d, tx);
-      if (tx == 0) p.part_lse[((int64_t)at.split * p.n_q + q) * p.hq + h] = lse;
+    if (p.parts > 1) {
+      const int64_t at = ((int64_t)w.part * p.n_q + q) * p.hq + h;
+      store_row<float, DP>(o[i], by, p.part + at * p.d, p.d, tx);
+      if (tx == 0) p.part_lse[at] = lse;
+      if (tx == 0 && w.part == 0) p.part_count[at] = w.parts;
     } else {
       store_row<T, DP>(o[i], by, (T*)p.out + (q * p.hq + h) * p.d, p.d, tx);
       if (tx == 0 && p.lse) p.lse[q * p.hq + h] = lse;
@@ -277,13 +267,13 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
   __shared__ float s_lse[kTile], s_delta[kTile];
   __shared__ uint8_t s_key[kTile];
   after_previous();
-  const Place at = place_of(p);
-  const Work w = block_work<!KEYS>(p, at.item);
+  const int key_head = blockIdx.x % p.hkv;
+  const Work w = block_work<!KEYS>(p);
   if (w.scan < 0) return;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int all = w.nq * p.group;
   auto query = [&](int i, int* head) {                                // row i of the scan's queries
-    *head = at.head * p.group + i % p.group;
+    *head = key_head * p.group + i % p.group;
     return (int64_t)w.q0 + i / p.group;
   };
   auto load_queries = [&](float* q_to, float* d_to, int first, int n) {
@@ -316,16 +306,16 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
       s_key[threadIdx.x] = (int)threadIdx.x < n && (p.mask == nullptr || p.mask[w.k0 + first + threadIdx.x] != 0);
     __syncthreads();
     load_tile<T, DP>(k_to, p.d, p.vec, [&](int r) -> const T* {
-      return s_key[r] ? (const T*)p.k + (int64_t)(w.k0 + first + r) * p.k_row + at.head * p.k_head : nullptr;
+      return s_key[r] ? (const T*)p.k + (int64_t)(w.k0 + first + r) * p.k_row + key_head * p.k_head : nullptr;
     });
     load_tile<T, DP>(v_to, p.d, p.vec, [&](int r) -> const T* {
-      return s_key[r] ? (const T*)p.v + (int64_t)(w.k0 + first + r) * p.v_row + at.head * p.v_head : nullptr;
+      return s_key[r] ? (const T*)p.v + (int64_t)(w.k0 + first + r) * p.v_row + key_head * p.v_head : nullptr;
     });
   };
   const int row0 = w.tile * kTile, rows = min(kTile, (KEYS ? w.nk : all) - row0);
   if (KEYS) load_keys(s_r1, s_r2, row0, rows);
   else load_queries(s_r1, s_r2, row0, rows);
-  const int2 span = split_rows(KEYS ? all : w.nk, at.split, p.splits, kTile);
+  const int2 span = make_int2(w.first, w.last);
   float a1[4][DP / 16], a2[4][DP / 16];                               // dV ; dK or dQ
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -358,14 +348,15 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
     if (r >= rows) continue;
     int64_t at_row;                                                   // of [rows][heads]
     if (KEYS) {
-      at_row = (int64_t)(w.k0 + row0 + r) * p.hkv + at.head;
+      at_row = (int64_t)(w.k0 + row0 + r) * p.hkv + key_head;
     } else {
       int h;
       const int64_t q = query(row0 + r, &h);
       at_row = q * p.hq + h;
     }
-    if (p.splits > 1) {
-      at_row += (int64_t)at.split * (KEYS ? (int64_t)p.n_k * p.hkv : (int64_t)p.n_q * p.hq);
+    if (p.parts > 1) {
+      if (tx == 0 && w.part == 0) p.part_count[at_row] = w.parts;
+      at_row += (int64_t)w.part * (KEYS ? (int64_t)p.n_k * p.hkv : (int64_t)p.n_q * p.hq);
       store_row<float, DP>(a2[i], p.scale, p.part + at_row * p.d, p.d, tx);
       if (KEYS) store_row<float, DP>(a1[i], 1.f, p.part2 + at_row * p.d, p.d, tx);
     } else {
@@ -375,11 +366,21 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
   }
 }
 
-// delta of every row of every query head: a warp each
+// delta of every row of every query head, a warp each; the first two warps plan what the tensor-core kernels do, for dQ and for dK and dV.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) delta_kernel(const T* d_out, const T* out, float* delta, int64_t rows, int d) {
+__global__ void __launch_bounds__(kThreads) delta_kernel(const T* d_out, const T* out, float* delta, int64_t rows, int d,
+                                                         const __grid_constant__ Params dq, const __grid_constant__ Params dkv) {
   after_previous();
   const int lane = threadIdx.x & 31;
+  if (blockIdx.x == 0 && threadIdx.x < 64) {
+    const Params& p = threadIdx.x < 32 ? dq : dkv;
+    auto leave = [&](const ScanPlan& x, int s0) {
+      if (s0 + lane < p.B + 2) const_cast<ScanPlan*>(p.plan)[s0 + lane] = x;
+      return false;
+    };
+    if (threadIdx.x < 32) plan_scans<true>(p, kTcTile, kTcStep, leave);
+    else plan_scans<false>(p, kTcTile, kTcStep, leave);
+  }
   for (int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * (kThreads / 32)) {
     float s = 0.f;
     for (int c = lane; c < d; c += 32) s = fmaf(to_float(d_out[r * d + c]), to_float(out[r * d + c]), s);
@@ -391,8 +392,8 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const T* d_out, const T
 // Parts of the forward pass: out = sum of 2^(lse_i - lse) part_i with lse = log2 of the sum of 2^lse_i.  WARPS warps a row, that share the
 // parts; of a warp, lanes the parts' lse first, then the channels.
 template <typename T, int WARPS>
-__global__ void __launch_bounds__(kThreads) join_forward_kernel(const float* part, const float* part_lse, int splits, int64_t rows, int d,
-                                                                T* out, float* lse) {
+__global__ void __launch_bounds__(kThreads) join_forward_kernel(const float* part, const float* part_lse, const int* count, int most,
+                                                                int64_t rows, int d, T* out, float* lse) {
   constexpr int kRows = kThreads / 32 / WARPS;              // of a block
   __shared__ float s_v[kThreads / 32][SPH_ATTENTION_MAX_CHANNELS];
   after_previous();
@@ -400,6 +401,7 @@ __global__ void __launch_bounds__(kThreads) join_forward_kernel(const float* par
   for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
     const int64_t r = r0 + warp / WARPS;
     const bool mine = r < rows;
+    const int splits = mine ? min(max(count[r], 0), most) : 0;        // unordered scans may have left it unwritten
     float l[2];                                             // of parts lane and lane + 32; +inf: one without keys
     float top = -INFINITY;
     bool some = false;
@@ -422,9 +424,9 @@ __global__ void __launch_bounds__(kThreads) join_forward_kernel(const float* par
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float inv = some ? 1.f / sum : 0.f;
     float v[SPH_ATTENTION_MAX_CHANNELS / 32] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = warp % WARPS; s < splits; s += WARPS) {
+    for (int s = warp % WARPS; s < splits; s += WARPS) {    // a warp has one row
       const float f = __shfl_sync(0xffffffffu, s < 32 ? l[0] : l[1], s & 31) * inv;
-      if (!mine || f == 0.f) continue;                      // a part without keys is not looked at
+      if (f == 0.f) continue;                               // a part without keys is not looked at
 #pragma unroll
       for (int i = 0; i < SPH_ATTENTION_MAX_CHANNELS / 32; ++i)
         if (lane + 32 * i < d) v[i] = fmaf(f, part[((int64_t)s * rows + r) * d + lane + 32 * i], v[i]);
@@ -451,11 +453,12 @@ __global__ void __launch_bounds__(kThreads) join_forward_kernel(const float* par
 
 // Parts of a gradient, added in their order.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) join_sum_kernel(const float* part, int splits, int64_t n, T* to) {
+__global__ void __launch_bounds__(kThreads) join_sum_kernel(const float* part, const int* count, int most, int64_t n, int d, T* to) {
   after_previous();
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+    const int parts = min(max(count[i / d], 0), most);
     float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += part[(int64_t)s * n + i];
+    for (int s = 0; s < parts; ++s) v += part[(int64_t)s * n + i];
     to[i] = from_float<T>(v);
   }
 }
@@ -474,31 +477,34 @@ namespace {
 bool on_tensor_cores(const sph_attention& a, const Params& p) {
   return (a.dtype == SPH_F16 || a.dtype == SPH_BF16) && p.vec && p.scale > 0.f;
 }
-constexpr int kTcTile = 128, kTcStep = 64;
 
 int padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 int forward_smem(int dp) { return (3 * kTile * (dp + 4) + kTile * kScorePitch) * 4; }
 int backward_smem(int dp, bool keys) { return (4 * kTile * (dp + 4) + (keys ? 2 : 1) * kTile * kScorePitch) * 4; }
 
-// Parts that the walk of `blocks` blocks over `tiles` tiles each is split into, where `slots` blocks run at a time.  What it costs: the
-// tiles there are and the start of every block (`start` tiles' time), spread over the slots; half a part's time at the end, when some slots
-// have run out of work (scans differ in length: few large parts end far apart); and writing and reading parts of `values`, of which
-// `rate` are a tile's time.
+// Parts that the walk of `blocks` blocks over `tiles` tiles each is split into on average, where `slots` blocks run at a time.  What it
+// costs, in tiles' time: the rounds of parts that there are, as whole ones and as they would be if every slot went on at once, taken by
+// half (the device makes the parts of scans of different length equally long, but not their number a multiple of the slots), `start` for a
+// block to start; and writing and reading parts of `values`, of which `rate` are a tile's time.
 int splits_for(int64_t blocks, int64_t slots, int64_t tiles, int64_t values, double start, double rate) {
   int best = 1;
   double least = 1e300;
   for (int64_t s = 1; s <= std::min<int64_t>(kMostParts, std::max<int64_t>(1, tiles / 2)); ++s) {
     const double part = (double)tiles / s + start;
-    const double cost = std::max(1.0, (double)(blocks * s) / slots) * part + 0.5 * part + (s > 1 ? start + s * (double)values / rate : 0.0);
+    const double rounds = 0.5 * (double)div_up64(blocks * s, slots) + 0.5 * (std::max(1.0, (double)(blocks * s) / slots) + 0.25);
+    const double cost = rounds * part + (s > 1 ? start + s * (double)values / rate : 0.0);
     if (cost < least) { least = cost; best = (int)s; }
   }
   return best;
 }
 
+// Of a direction: parts of a tile's walk, at most, and blocks.
+struct Split {
+  int parts, aim, items;                     // items: what a head's part of the grid has room for
+};
 struct Plan {
   int decode;                                // rows of a block of the decoding kernel; 0: another one runs forward
-  int fwd_splits, dq_splits, dkv_splits;
-  int fwd_blocks, dq_blocks, dkv_blocks;     // without the splits
+  Split fwd, dq, dkv;
 };
 Plan plan_of(const sph_attention& a, const Params& params, int sms) {
   const int group = a.q_heads / a.k_heads, dp = padded(a.channels);
@@ -507,29 +513,27 @@ Plan plan_of(const sph_attention& a, const Params& params, int sms) {
   Plan p;
   const int64_t B = std::max(a.B, 1);
   const int64_t q_rows = a.n_q * group, q_values = a.n_q * a.q_heads * a.channels, k_values = 2 * a.n_k * a.k_heads * a.channels;
-  // tiles that there really are, if scans are of like length, and how many a block walks over
-  auto real = [&](int64_t rows, int64_t size) { return std::max<int64_t>(1, div_up64(rows, size * B)) * B * a.k_heads; };
-  auto walk = [&](int64_t rows, int64_t size) { return div_up64(rows, B * size); };
+  // rows in tiles of `size` (a key head's), that walk over `walk` rows in steps of `step`
+  auto split = [&](int64_t rows, int64_t size, int64_t walk, int64_t step, int64_t slots, int64_t values, double start, double rate) {
+    const int64_t tiles = std::max<int64_t>(1, div_up64(rows, size * B)) * B;             // if scans are of like length
+    const int n = splits_for(tiles * a.k_heads, slots, div_up64(walk, B * step), values, start, rate);
+    const int64_t most = most_tiles(rows, size, a.B);
+    // of scans that are longer than the others a tile has more parts
+    return n == 1 ? Split{1, 1, (int)most} : Split{std::min(4 * n, kMostParts), (int)(tiles * n), (int)(most + tiles * n)};
+  };
   if (on_tensor_cores(a, params)) {          // 0.7 us a tile; a block starts in 5 us, one that takes several tiles of rows in 2
     constexpr double kRate = 500000;
-    p.fwd_blocks = p.dq_blocks = most_tiles(q_rows, kTcTile, a.B) * a.k_heads;
-    p.dkv_blocks = most_tiles(a.n_k, kTcTile, a.B) * a.k_heads;
-    p.fwd_splits = splits_for(real(q_rows, kTcTile), 2 * sms, walk(a.n_k, kTcStep), q_values, 8, kRate);
-    p.dq_splits = splits_for(real(q_rows, kTcTile), sms, walk(a.n_k, kTcStep), q_values, 4, kRate);
-    p.dkv_splits = splits_for(real(a.n_k, kTcTile), sms, walk(q_rows, kTcStep), k_values, 4, kRate);
+    p.fwd = split(q_rows, kTcTile, a.n_k, kTcStep, 2 * sms, q_values, 8, kRate);
+    p.dq = split(q_rows, kTcTile, a.n_k, kTcStep, sms, q_values, 4, kRate);
+    p.dkv = split(a.n_k, kTcTile, q_rows, kTcStep, sms, k_values, 4, kRate);
   } else {                                   // 4 us a tile
     constexpr double kRate = 3000000;
-    p.fwd_blocks = p.dq_blocks = most_tiles(q_rows, kTile, a.B) * a.k_heads;
-    p.dkv_blocks = most_tiles(a.n_k, kTile, a.B) * a.k_heads;
-    p.fwd_splits = splits_for(real(q_rows, kTile), sms * per_sm(forward_smem(dp)), walk(a.n_k, kTile), q_values, 1, kRate);
-    p.dq_splits = splits_for(real(q_rows, kTile), sms * per_sm(backward_smem(dp, false)), walk(a.n_k, kTile), q_values, 1, kRate);
-    p.dkv_splits = splits_for(real(a.n_k, kTile), sms * per_sm(backward_smem(dp, true)), walk(q_rows, kTile), k_values, 1, kRate);
+    p.fwd = split(q_rows, kTile, a.n_k, kTile, sms * per_sm(forward_smem(dp)), q_values, 1, kRate);
+    p.dq = split(q_rows, kTile, a.n_k, kTile, sms * per_sm(backward_smem(dp, false)), q_values, 1, kRate);
+    p.dkv = split(a.n_k, kTile, q_rows, kTile, sms * per_sm(backward_smem(dp, true)), k_values, 1, kRate);
   }
   p.decode = params.vec ? attention_decode_rows(a.dtype, div_up64(q_rows, B)) : 0;
-  if (p.decode) {                            // steps of 64 keys
-    p.fwd_blocks = most_tiles(q_rows, p.decode, a.B) * a.k_heads;
-    p.fwd_splits = splits_for(real(q_rows, p.decode), 2 * sms, walk(a.n_k, 64), q_values, 1.5, 500000);
-  }
+  if (p.decode) p.fwd = split(q_rows, p.decode, a.n_k, 64, 2 * sms, q_values, 1.5, 500000);
   return p;
 }
 
@@ -561,20 +565,26 @@ unsigned grid_for(int64_t items, int64_t per_block) { return (unsigned)std::min<
 template <typename T>
 int run_forward(Params p, const Plan& plan, bool tensor_cores, void* scratch, cudaStream_t st) {
   const int64_t rows = (int64_t)p.n_q * p.hq;
-  p.splits = plan.fwd_splits;
-  if (p.splits > 1) {
+  p.parts = plan.fwd.parts;
+  p.aim = plan.fwd.aim;
+  if (p.parts > 1) {
     p.part = (float*)scratch;
-    p.part_lse = p.part + rows * p.d * p.splits;
+    p.part_lse = p.part + rows * p.d * p.parts;
+    p.part_count = (int*)(p.part_lse + rows * p.parts);
   }
   constexpr int dtype = std::is_same<T, float>::value ? SPH_F32 : std::is_same<T, __half>::value ? SPH_F16 : SPH_BF16;
-  const int rc = plan.decode  ? attention_decode(p, dtype, plan.decode, plan.fwd_blocks * p.splits, st)
-                 : tensor_cores ? attention_forward_tc(p, std::is_same<T, __nv_bfloat16>::value, plan.fwd_blocks * p.splits, st)
-                                : forward<T>(p, plan.fwd_blocks * p.splits, st);
-  if (rc != SPH_OK || p.splits == 1) return rc;
+  const int blocks = plan.fwd.items * p.hkv;
+  const int rc = plan.decode    ? attention_decode(p, dtype, plan.decode, blocks, st)
+                 : tensor_cores ? attention_forward_tc(p, dtype == SPH_BF16, blocks, st)
+                                : forward<T>(p, blocks, st);
+  if (rc != SPH_OK || p.parts == 1) return rc;
   // a few rows leave most of the GPU to the parts of a row
   constexpr int kWarps = kThreads / 32;
-  if (rows <= 148 * 4) launch(join_forward_kernel<T, kWarps>, grid_for(rows, 1), kThreads, 0, st, p.part, p.part_lse, p.splits, rows, p.d, (T*)p.out, p.lse);
-  else launch(join_forward_kernel<T, 1>, grid_for(rows, kWarps), kThreads, 0, st, p.part, p.part_lse, p.splits, rows, p.d, (T*)p.out, p.lse);
+  auto join = [&](auto* kernel, unsigned grid) {
+    launch(kernel, grid, kThreads, 0, st, p.part, p.part_lse, p.part_count, p.parts, rows, p.d, (T*)p.out, p.lse);
+  };
+  if (rows <= 148 * 4) join(join_forward_kernel<T, kWarps>, grid_for(rows, 1));
+  else join(join_forward_kernel<T, 1>, grid_for(rows, kWarps));
   SPH_LAUNCH_CHECK();
   return SPH_OK;
 }
@@ -584,36 +594,33 @@ int run_backward(Params p, const Plan& plan, bool tensor_cores, const void* out,
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   const int64_t rows = (int64_t)p.n_q * p.hq, k_values = (int64_t)p.n_k * p.hkv * p.d;
   float* delta = (float*)scratch;
-  float* part = delta + (rows + 3) / 4 * 4;
   p.delta = delta;
-  if (rows) {
-    launch(delta_kernel<T>, grid_for(rows, kThreads / 32), kThreads, 0, st, (const T*)p.d_out, (const T*)out, delta, rows, p.d);
+  ScanPlan* plans = (ScanPlan*)(delta + (rows + 3) / 4 * 4);
+  p.part_count = (int*)(plans + 2 * (p.B + 2));
+  p.part = (float*)p.part_count + (std::max(rows, (int64_t)p.n_k * p.hkv) + 3) / 4 * 4;
+  Params dq = p, dkv = p;
+  dq.parts = plan.dq.parts; dq.aim = plan.dq.aim; dq.plan = plans;
+  dkv.parts = plan.dkv.parts; dkv.aim = plan.dkv.aim; dkv.plan = plans + p.B + 2;
+  dkv.part2 = dkv.part + k_values * dkv.parts;
+  launch(delta_kernel<T>, std::max(1u, grid_for(rows, kThreads / 32)), kThreads, 0, st, (const T*)p.d_out, (const T*)out, delta, rows, p.d, dq, dkv);
+  SPH_LAUNCH_CHECK();
+  auto join = [&](const float* part, int parts, int64_t n, void* to) {
+    launch(join_sum_kernel<T>, grid_for(n, kThreads), kThreads, 0, st, part, p.part_count, parts, n, p.d, (T*)to);
     SPH_LAUNCH_CHECK();
-  }
+    return SPH_OK;
+  };
   if (p.dq && rows) {
-    p.splits = plan.dq_splits;
-    p.part = part;
-    const int rc = tensor_cores ? attention_backward_tc(p, bf16, false, plan.dq_blocks * p.splits, st)
-                                : backward<T, false>(p, plan.dq_blocks * p.splits, st);
+    const int blocks = plan.dq.items * p.hkv;
+    int rc = tensor_cores ? attention_backward_tc(dq, bf16, false, blocks, st) : backward<T, false>(dq, blocks, st);
+    if (rc == SPH_OK && dq.parts > 1) rc = join(dq.part, dq.parts, rows * p.d, p.dq);
     if (rc != SPH_OK) return rc;
-    if (p.splits > 1) {
-      launch(join_sum_kernel<T>, grid_for(rows * p.d, kThreads), kThreads, 0, st, part, p.splits, rows * p.d, (T*)p.dq);
-      SPH_LAUNCH_CHECK();
-    }
   }
   if ((p.dk || p.dv) && k_values) {
-    p.splits = plan.dkv_splits;
-    p.part = part;
-    p.part2 = part + k_values * p.splits;
-    const int rc = tensor_cores ? attention_backward_tc(p, bf16, true, plan.dkv_blocks * p.splits, st)
-                                : backward<T, true>(p, plan.dkv_blocks * p.splits, st);
+    const int blocks = plan.dkv.items * p.hkv;
+    int rc = tensor_cores ? attention_backward_tc(dkv, bf16, true, blocks, st) : backward<T, true>(dkv, blocks, st);
+    if (rc == SPH_OK && dkv.parts > 1) rc = join(dkv.part, dkv.parts, k_values, p.dk);
+    if (rc == SPH_OK && dkv.parts > 1) rc = join(dkv.part2, dkv.parts, k_values, p.dv);
     if (rc != SPH_OK) return rc;
-    if (p.splits > 1) {
-      launch(join_sum_kernel<T>, grid_for(k_values, kThreads), kThreads, 0, st, p.part, p.splits, k_values, (T*)p.dk);
-      SPH_LAUNCH_CHECK();
-      launch(join_sum_kernel<T>, grid_for(k_values, kThreads), kThreads, 0, st, p.part2, p.splits, k_values, (T*)p.dv);
-      SPH_LAUNCH_CHECK();
-    }
   }
   return SPH_OK;
 }
@@ -670,9 +677,9 @@ extern "C" int64_t sph_attention_scratch_bytes(const sph_attention* a, int backw
   if (sms <= 0) return SPH_ERR_CUDA;
   const Plan plan = plan_of(*a, p, sms);
   const int64_t rows = (int64_t)p.n_q * p.hq, k_values = (int64_t)p.n_k * p.hkv * p.d;
-  if (!backward) return plan.fwd_splits > 1 ? plan.fwd_splits * rows * (p.d + 1) * 4 : 0;
-  return ((rows + 3) / 4 * 4 + std::max(plan.dq_splits > 1 ? plan.dq_splits * rows * p.d : 0,
-                                         plan.dkv_splits > 1 ? 2 * plan.dkv_splits * k_values : 0)) * 4;
+  if (!backward) return plan.fwd.parts > 1 ? (plan.fwd.parts * rows * (p.d + 1) + rows) * 4 : 0;
+  return 2 * (p.B + 2) * (int64_t)sizeof(ScanPlan) + ((rows + 3) / 4 * 4 + (std::max(rows, (int64_t)p.n_k * p.hkv) + 3) / 4 * 4 +
+          std::max(plan.dq.parts > 1 ? plan.dq.parts * rows * p.d : 0, plan.dkv.parts > 1 ? 2 * plan.dkv.parts * k_values : 0)) * 4;
 }
 
 extern "C" int sph_attention_forward(const sph_attention* a, void* d_out, float* d_lse, void* d_scratch, int32_t* d_status, void* stream) {
@@ -685,7 +692,7 @@ extern "C" int sph_attention_forward(const sph_attention* a, void* d_out, float*
   const int sms = current_sm_count();
   if (sms <= 0) return SPH_ERR_CUDA;
   const Plan plan = plan_of(*a, p, sms);
-  SPH_CHECK_ARG(plan.fwd_splits == 1 || (d_scratch && (uintptr_t)d_scratch % 16 == 0), "the scratch must be 16-byte aligned");
+  SPH_CHECK_ARG(plan.fwd.parts == 1 || (d_scratch && (uintptr_t)d_scratch % 16 == 0), "the scratch must be 16-byte aligned");
   p.out = d_out;
   p.lse = d_lse;
   p.status = d_status;

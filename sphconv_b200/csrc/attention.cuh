@@ -3,9 +3,13 @@
 // Queries and keys are rows of B scans; scan b has the rows ptr[b] .. ptr[b+1]-1 of each, and what lies in front of the first or behind
 // the last scan is treated as two scans more that have nothing on the other side: such rows get zeros.  The lengths are on the device
 // only.  A grid has room for as many tiles as any lengths could need, and every block counts through the scans to find its own.
+// Where there are few tiles, what each walks over is split into parts: equally long ones, whatever the scans' lengths, as many as the grid
+// has room for.  Of a part's results the sums are float32 in a place of their own, and joined in the parts' order by another launch.
 //
 // Query heads that share a key head are rows of one tile: row r of a scan and key head is query r / group, head r % group.
 #pragma once
+
+#include <limits.h>
 
 #include "common.cuh"
 
@@ -26,18 +30,27 @@ struct Params {
   const void* d_out;                                        // [n_q][hq][d]
   const float* delta;                                       // [n_q][hq] sum of d_out * out
   void *dq, *dk, *dv;                                       // as q, [n_k][hkv][d]
-  float *part, *part2;                                      // with splits > 1: [splits][rows][heads][d], and of dv
-  float* part_lse;                                          // forward: [splits][n_q][hq]
-  int splits;
+  int parts, aim;                                           // most parts of a tile's walk; how many all tiles are to have about, a head
+  float *part, *part2;                                      // with parts > 1: [parts][rows][heads][d], and of dv
+  float* part_lse;                                          // forward: [parts][n_q][hq]
+  int* part_count;                                          // [rows][heads]
+  const struct ScanPlan* plan;                              // [B + 2], where another kernel has left it
   int vec;                                                  // rows can be read in pieces of 16 bytes
   int* status;
 };
 
-// One tile of queries or keys.
+// A scan's rows and how they are divided: its tiles' parts are numbers upto - tiles * parts .. upto - 1.
+struct __align__(16) ScanPlan {
+  int upto, parts, per, tiles;                              // per: rows of the walk that a part has
+  int q0, nq, k0, nk;
+};
+
+// A tile of queries or keys, and the part of the other side that it is to be walked over with.
 struct Work {
   int scan;                                                 // -1: nothing to do
   int tile;
   int q0, nq, k0, nk;                                       // rows of the scan
+  int part, parts, first, last;                             // keys, or rows of queries and heads
 };
 
 __device__ __forceinline__ int2 scan_rows(const int* ptr, int B, int n, int s) {
@@ -46,51 +59,106 @@ __device__ __forceinline__ int2 scan_rows(const int* ptr, int B, int n, int s) {
   return make_int2(begin, max(begin, end));
 }
 
-// Tile `item` of all scans' tiles of `size` rows (of queries: a row per head of the group); called by one whole warp.
-template <bool QUERIES>
-__device__ __forceinline__ Work find_work(const Params& p, int item, int size) {
+// Divides the scans' tiles of `size` rows (of queries: a row per head of the group), that are walked over in steps of `step`, into parts;
+// by one whole warp, found(plan, first) with 32 scans' plans in its lanes, until it says that this is enough.  A part has `chunk` steps: with
+// A steps of all tiles' walks and T tiles, chunk = ceil(A / aim) makes at most aim + T parts.
+template <bool QUERIES, typename Found>
+__device__ __forceinline__ void plan_scans(const Params& p, int size, int step, Found found) {
   const int lane = threadIdx.x & 31;
-  Work w;
-  w.scan = -1;
+  ScanPlan x;
+  int steps;
+  auto look = [&](int s) {
+    int2 q = make_int2(0, 0), k = make_int2(0, 0);
+    if (s < p.B + 2) {
+      q = scan_rows(p.q_ptr, p.B, p.n_q, s);
+      k = scan_rows(p.k_ptr, p.B, p.n_k, s);
+      if (s == 0 || s == p.B + 1) (QUERIES ? k : q) = make_int2(0, 0);
+    }
+    x.q0 = q.x; x.nq = q.y - q.x;
+    x.k0 = k.x; x.nk = k.y - k.x;
+    const int64_t rows = (int64_t)x.nq * p.group, keys = x.nk;
+    x.tiles = (int)(((QUERIES ? rows : keys) + size - 1) / size);
+    steps = (int)(((QUERIES ? keys : rows) + step - 1) / step);
+  };
+  int chunk = INT_MAX;
+  if (p.parts > 1) {
+    long long a = 0;
+    for (int s0 = 0; s0 < p.B + 2; s0 += 32) {
+      look(s0 + lane);
+      a += (long long)x.tiles * steps;
+    }
+    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    chunk = (int)min(max((a + p.aim - 1) / p.aim, 1ll), (long long)INT_MAX);
+  }
   int before = 0;
   for (int s0 = 0; s0 < p.B + 2; s0 += 32) {
-    const int s = s0 + lane;
-    int tiles = 0;
-    if (s < p.B + 2) {
-      const int2 r = QUERIES ? scan_rows(p.q_ptr, p.B, p.n_q, s) : scan_rows(p.k_ptr, p.B, p.n_k, s);
-      const int64_t rows = (int64_t)(r.y - r.x) * (QUERIES ? p.group : 1);
-      tiles = (int)((rows + size - 1) / size);
-    }
-    int upto = tiles;
+    look(s0 + lane);
+    const int mine = p.parts > 1 ? max(chunk, (steps + p.parts - 1) / p.parts) : INT_MAX;  // steps of a part
+    x.parts = steps == 0 || steps <= mine ? 1 : (steps - 1) / mine + 1;
+    x.per = x.parts > 1 ? mine * step : INT_MAX;
+    x.upto = x.tiles * x.parts;
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
+      const int v = __shfl_up_sync(0xffffffffu, x.upto, o);
+      if (lane >= o) x.upto += v;
     }
-    const unsigned here = __ballot_sync(0xffffffffu, before + upto > item);
-    if (here) {
-      const int l = __ffs((int)here) - 1;
-      w.scan = s0 + l;
-      w.tile = item - before - (__shfl_sync(0xffffffffu, upto, l) - __shfl_sync(0xffffffffu, tiles, l));
-      break;
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
+    x.upto += before;
+    if (found(x, s0)) break;
+    before = __shfl_sync(0xffffffffu, x.upto, 31);
   }
-  if (w.scan >= 0) {
-    const bool real = w.scan > 0 && w.scan <= p.B;
-    const int2 none = make_int2(0, 0);
-    const int2 q = real || QUERIES ? scan_rows(p.q_ptr, p.B, p.n_q, w.scan) : none;
-    const int2 k = real || !QUERIES ? scan_rows(p.k_ptr, p.B, p.n_k, w.scan) : none;
-    w.q0 = q.x; w.nq = q.y - q.x;
-    w.k0 = k.x; w.nk = k.y - k.x;
-  }
+}
+
+// Part `item` as its scan's plan has it.
+template <bool QUERIES>
+__device__ __forceinline__ Work work_of(const Params& p, const ScanPlan& x, int scan, int item) {
+  Work w;
+  w.scan = -1;
+  const int left = item - (x.upto - x.tiles * x.parts);
+  if (left < 0 || left >= x.tiles * x.parts) return w;      // scans that overlap may count up to anything
+  w.scan = scan;
+  w.parts = x.parts;
+  w.tile = x.parts > 1 ? left / x.parts : left;
+  w.part = left - w.tile * x.parts;
+  w.q0 = x.q0; w.nq = x.nq; w.k0 = x.k0; w.nk = x.nk;
+  const int64_t all = QUERIES ? x.nk : (int64_t)x.nq * p.group;
+  w.first = (int)min(all, (int64_t)x.per * w.part);
+  w.last = (int)min(all, (int64_t)x.per * (w.part + 1));
   return w;
 }
 
-// Part `split` of `splits` of n rows, in whole tiles of `size`: [first, last).
-__device__ __forceinline__ int2 split_rows(int n, int split, int splits, int size) {
-  const int per = ((n + size - 1) / size + splits - 1) / splits * size;
-  const int first = min((int64_t)n, (int64_t)per * split);
-  return make_int2(first, min(n, first + per));
+// Part `item` of all scans' tiles; by one whole warp.
+template <bool QUERIES>
+__device__ __forceinline__ Work find_work(const Params& p, int item, int size, int step) {
+  Work w;
+  w.scan = -1;
+  plan_scans<QUERIES>(p, size, step, [&](const ScanPlan& x, int s0) {
+    const unsigned here = __ballot_sync(0xffffffffu, x.upto > item);
+    if (here == 0) return false;
+    const int l = __ffs((int)here) - 1;
+    ScanPlan y;
+    y.upto = __shfl_sync(0xffffffffu, x.upto, l); y.parts = __shfl_sync(0xffffffffu, x.parts, l);
+    y.per = __shfl_sync(0xffffffffu, x.per, l); y.tiles = __shfl_sync(0xffffffffu, x.tiles, l);
+    y.q0 = __shfl_sync(0xffffffffu, x.q0, l); y.nq = __shfl_sync(0xffffffffu, x.nq, l);
+    y.k0 = __shfl_sync(0xffffffffu, x.k0, l); y.nk = __shfl_sync(0xffffffffu, x.nk, l);
+    w = work_of<QUERIES>(p, y, s0 + l, item);
+    return true;
+  });
+  return w;
+}
+// The same where another kernel has left the plan.
+template <bool QUERIES>
+__device__ __forceinline__ Work find_planned(const Params& p, int item) {
+  const int lane = threadIdx.x & 31;
+  Work w;
+  w.scan = -1;
+  for (int s0 = 0; s0 < p.B + 2; s0 += 32) {
+    const int s = s0 + lane;
+    const unsigned here = __ballot_sync(0xffffffffu, s < p.B + 2 && __ldg(&p.plan[s].upto) > item);
+    if (here == 0) continue;
+    const int l = s0 + __ffs((int)here) - 1;
+    const int4 a = __ldg((const int4*)(p.plan + l)), b = __ldg((const int4*)(p.plan + l) + 1);
+    return work_of<QUERIES>(p, ScanPlan{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, l, item);
+  }
+  return w;
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {

@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(kThreadsDecode, 2) decode_kernel(const __grid_
   constexpr int P = Key<T>::kPairs, E = 2 * P, KEYS = 32 / LANES;
   __shared__ Work s_work;
   __shared__ float s_m[kWarps][R], s_l[kWarps][R];
-  __shared__ float s_o[kWarps][R][LANES * E];
+  __shared__ __align__(16) float s_o[kWarps][R][LANES * E];           // written two at a time
   after_previous();
   if (blockIdx.x == 0 && p.status != nullptr) {             // scans that are not in order, or not within the rows
     bool bad = false;
@@ -81,10 +81,10 @@ __global__ void __launch_bounds__(kThreadsDecode, 2) decode_kernel(const __grid_
     }
     if (bad) atomicOr(p.status, SPH_STATUS_BAD_INDEX);
   }
-  const int split = blockIdx.x % p.splits, head = blockIdx.x / p.splits % p.hkv;
+  const int head = blockIdx.x % p.hkv;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (warp == 0) {
-    const Work w = find_work<true>(p, blockIdx.x / p.splits / p.hkv, R);
+    const Work w = find_work<true>(p, blockIdx.x / p.hkv, R, kStep);
     if (lane == 0) s_work = w;
   }
   __syncthreads();
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kThreadsDecode, 2) decode_kernel(const __grid_
   }
   // of value i % W of every lane that has row r
   auto of_row = [&](const float (&x)[W], int r) { return __shfl_sync(0xffffffffu, x[r % W], r / W * (LANES * W / R), LANES); };
-  const int2 keys = split_rows(w.nk, split, p.splits, kStep);
+  const int2 keys = make_int2(w.first, w.last);
   const T* k_at = (const T*)p.k + (int64_t)w.k0 * p.k_row + head * p.k_head;
   const T* v_at = (const T*)p.v + (int64_t)w.k0 * p.v_row + head * p.v_head;
   const int mine = warp * KEYS + lane / LANES;
@@ -262,15 +262,16 @@ __global__ void __launch_bounds__(kThreadsDecode, 2) decode_kernel(const __grid_
       v = fmaf(f, s_o[x][r][ch], v);
     }
     const bool none = sum == 0.f;
-    const int64_t at = out_row(r), part_at = (int64_t)split * p.n_q * p.hq + at;
+    const int64_t at = out_row(r), part_at = (int64_t)w.part * p.n_q * p.hq + at;
     if (ch < p.d) {
       const float result = none ? 0.f : v / sum;
-      if (p.splits > 1) p.part[part_at * p.d + ch] = result;
+      if (p.parts > 1) p.part[part_at * p.d + ch] = result;
       else ((T*)p.out)[at * p.d + ch] = Key<T>::put(result);
     }
     if (ch == 0) {
       const float lse = none ? INFINITY : top + log2f(sum);
-      if (p.splits > 1) p.part_lse[part_at] = lse;
+      if (p.parts > 1 && w.part == 0) p.part_count[at] = w.parts;
+      if (p.parts > 1) p.part_lse[part_at] = lse;
       else if (p.lse) p.lse[at] = lse;
     }
   }

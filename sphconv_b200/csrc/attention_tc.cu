@@ -83,16 +83,6 @@ __device__ __forceinline__ void report_scans(const Params& p) {
   if (bad) atomicOr(p.status, SPH_STATUS_BAD_INDEX);
 }
 
-// What of the work is a block's: a tile of queries of one key head against a part of the keys.
-struct Part {
-  int split, head, item;
-  __device__ __forceinline__ explicit Part(const Params& p) {
-    split = blockIdx.x % p.splits;
-    head = blockIdx.x / p.splits % p.hkv;
-    item = blockIdx.x / p.splits / p.hkv;
-  }
-};
-
 // Row r of a block's tile: of which query and head it is.
 struct Row {
   int64_t q;
@@ -174,9 +164,9 @@ __device__ __forceinline__ void issue_out(uint32_t to, uint32_t p_at, uint64_t v
 
 // A row's part of the result, from its accumulator at TMEM `at_o`.
 template <bool BF16>
-__device__ __forceinline__ void store_out(const Params& p, const Work& w, const Part& part, uint32_t at_o, int r, int rows, float top, float sum) {
+__device__ __forceinline__ void store_out(const Params& p, const Work& w, int head, uint32_t at_o, int r, int rows, float top, float sum) {
   const bool none = sum == 0.f, mine = r < rows;
-  const int64_t at = Row(p, w, part.head, min(r, rows - 1)).out(p), part_at = (int64_t)part.split * p.n_q * p.hq + at;
+  const int64_t at = Row(p, w, head, min(r, rows - 1)).out(p), part_at = (int64_t)w.part * p.n_q * p.hq + at;
   const float by = none ? 0.f : 1.f / sum, lse = none ? INFINITY : top + log2f(sum);
 #pragma unroll 1
   for (int c = 0; c < p.d; c += 16) {
@@ -188,10 +178,11 @@ __device__ __forceinline__ void store_out(const Params& p, const Work& w, const 
       for (int e = 0; e < 16; ++e) v[e] = 0u;
     }
     if (!mine) continue;
-    if (p.splits > 1) store16_float(v, by, p.part + part_at * p.d + c, p.d - c);
+    if (p.parts > 1) store16_float(v, by, p.part + part_at * p.d + c, p.d - c);
     else store16<BF16>(v, by, (uint16_t*)p.out + at * p.d + c, p.d - c);
   }
-  if (mine && p.splits > 1) p.part_lse[part_at] = lse;
+  if (mine && p.parts > 1 && w.part == 0) p.part_count[at] = w.parts;
+  if (mine && p.parts > 1) p.part_lse[part_at] = lse;
   else if (mine && p.lse) p.lse[at] = lse;
 }
 
@@ -224,7 +215,7 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = (int)uniform((uint32_t)tid >> 5);
-  const Part part(p);
+  const int head = blockIdx.x % p.hkv;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t q_at = base, k_at = base + S::kQBytes, v_at = k_at + kStages * kTileBytes;
   if (tid == 0) {
@@ -246,13 +237,13 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
   after_previous<false>();
   report_scans(p);
   if (warp == 0) {
-    const Work w = find_work<true>(p, part.item, kM);
+    const Work w = find_work<true>(p, blockIdx.x / p.hkv, kM, kN);
     if (lane == 0) s_work = w;
   }
   __syncthreads();
   const Work w = s_work;
   if (w.scan < 0) return;
-  const int2 keys = split_rows(w.nk, part.split, p.splits, kN);
+  const int2 keys = make_int2(w.first, w.last);
   const int tiles = (keys.y - keys.x + kN - 1) / kN;
   const int rows = min(kM, w.nq * p.group - w.tile * kM);
   if (warp == kScoreWarp) {
@@ -272,7 +263,7 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
     const bool one = elect_one();
     if (S::kQInTmem && tiles > 0) {
       const int r = warp * 32 + lane, pieces = p.d / 8;
-      const uint4* from = (const uint4*)Row(p, w, part.head, min(r, rows - 1)).query(p);
+      const uint4* from = (const uint4*)Row(p, w, head, min(r, rows - 1)).query(p);
       uint32_t v[32];
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
@@ -335,7 +326,7 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
     }
     if (!dead && (tiles == 0 || warp_wait(smem_u32(&s_o_done[(tiles - 1) & 1]), (uint32_t)((tiles - 1) >> 1) & 1u, abort_flag))) {
       tc_fence_after();
-      if (any_row) store_out<BF16>(p, w, part, lanes + kColO, warp * 32 + lane, rows, top, sum);
+      if (any_row) store_out<BF16>(p, w, head, lanes + kColO, warp * 32 + lane, rows, top, sum);
     }
   } else if (warp == kScoreWarp) {
     // ======================= MMAs of S =======================
@@ -385,12 +376,12 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
       const int st = j % kStages;
       const uint32_t phase = ((uint32_t)(j / kStages) & 1u) ^ 1u;
       if (!warp_wait(smem_u32(&s_k_empty[st]), phase, abort_flag)) break;
-      load_keys<DP, kLoaders>(k_at + st * kTileBytes, t, first, one, p, k_map, p.k, p.k_row, p.k_head, w, keys, part.head, j,
+      load_keys<DP, kLoaders>(k_at + st * kTileBytes, t, first, one, p, k_map, p.k, p.k_row, p.k_head, w, keys, head, j,
                                smem_u32(&s_k_full[st]));
       if (!S::kQInTmem && j == 0)
-        load_queries<DP, kLoaders>(q_at, t, first, one, rows, p, q_map, w, part.head, smem_u32(&s_q_full));      // behind the first keys
+        load_queries<DP, kLoaders>(q_at, t, first, one, rows, p, q_map, w, head, smem_u32(&s_q_full));      // behind the first keys
       if (!warp_wait(smem_u32(&s_v_empty[st]), phase, abort_flag)) break;
-      load_keys<DP, kLoaders>(v_at + st * kTileBytes, t, first, one, p, v_map, p.v, p.v_row, p.v_head, w, keys, part.head, j,
+      load_keys<DP, kLoaders>(v_at + st * kTileBytes, t, first, one, p, v_map, p.v, p.v_row, p.v_head, w, keys, head, j,
                                smem_u32(&s_v_full[st]));
     }
     cp_async_wait_all();

@@ -73,23 +73,18 @@ __device__ __forceinline__ void p_and_ds(uint32_t (&v)[16], uint32_t (&u)[16], f
 // One tile of rows against a part of the columns.
 struct Item {
   Work w;
-  int split, head, all, first, last, tiles, row0, rows;               // all: rows of queries; first, last: columns
+  int head, tiles, row0, rows;                // tiles: of columns
 };
 template <bool KEYS>
 __device__ __forceinline__ Item find_item(const Params& p, int index) {          // by whole warps
   Item i;
-  i.split = index % p.splits;
-  i.head = index / p.splits % p.hkv;
-  i.w = find_work<!KEYS>(p, index / p.splits / p.hkv, kM);
+  i.head = index % p.hkv;
+  i.w = find_planned<!KEYS>(p, index / p.hkv);
   i.tiles = i.rows = 0;
   if (i.w.scan < 0) return i;
-  i.all = i.w.nq * p.group;
-  const int2 span = split_rows(KEYS ? i.all : i.w.nk, i.split, p.splits, kC);
-  i.first = span.x;
-  i.last = span.y;
-  i.tiles = (span.y - span.x + kC - 1) / kC;
+  i.tiles = (i.w.last - i.w.first + kC - 1) / kC;
   i.row0 = i.w.tile * kM;
-  i.rows = min(kM, (KEYS ? i.w.nk : i.all) - i.row0);
+  i.rows = (int)min((int64_t)kM, (KEYS ? i.w.nk : (int64_t)i.w.nq * p.group) - i.row0);
   return i;
 }
 
@@ -193,8 +188,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
       const Rows at{p, it};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int c = it.first + j * kC + 32 * i + lane;
-        const bool some = j < it.tiles && c < it.last;
+        const int c = it.w.first + j * kC + 32 * i + lane;
+        const bool some = j < it.tiles && c < it.w.last;
         const int64_t q = some ? at.query(c) : 0;
         next[i] = some ? kShift - p.lse[q] : -INFINITY;
         next[2 + i] = some ? -p.delta[q] : 0.f;
@@ -229,7 +224,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
       float& row_f = s_f[n & 1][r];
 #pragma unroll 1
       for (int j = j0; j < it.tiles; j += 2) {
-        const int b = (g + j) % PL, k0 = it.first + j * kC, cols = min(kC, it.last - k0);
+        const int b = (g + j) % PL, k0 = it.w.first + j * kC, cols = min(kC, it.w.last - k0);
         const uint32_t phase = (uint32_t)((g + j) / PL) & 1u;
         const bool whole = KEYS || (cols == kC && p.mask == nullptr);
         uint2 bits = make_uint2(~0u, ~0u);
@@ -349,9 +344,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
             for (int e = 0; e < 16; ++e) v[e] = 0u;
           }
           if (!mine) continue;
-          if (p.splits > 1) store16_float(v, by, part + (it.split * of + to_row) * p.d + c, p.d - c);
+          if (p.parts > 1) store16_float(v, by, part + (it.w.part * of + to_row) * p.d + c, p.d - c);
           else store16<BF16>(v, by, (uint16_t*)to + to_row * p.d + c, p.d - c);
         }
+        if (mine && p.parts > 1 && it.w.part == 0 && half == 0) p.part_count[to_row] = it.w.parts;
         tc_fence_before();
       }
       __syncwarp();
@@ -381,7 +377,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
         for (int j = 0; j < it.tiles; ++j, ++g) {
           const int st = g % ST, b = g % PL;
           if (!warp_spin(smem_u32(&s_c_full[st]), (uint32_t)(g / ST) & 1u, abort_flag)) { dead = true; break; }
-          if (!columns_fit || it.last - it.first - j * kC < kC) fence_proxy_async();
+          if (!columns_fit || it.w.last - it.w.first - j * kC < kC) fence_proxy_async();
           if (g >= PL && !warp_spin(smem_u32(&s_done[b]), (uint32_t)((g - PL) / PL) & 1u, abort_flag)) { dead = true; break; }
           tc_fence_after();
           const uint64_t cols_desc = c_desc + (uint32_t)st * (2 * S::kColBytes / 16u);
@@ -415,7 +411,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
         for (int j = 0; j < it.tiles; ++j, ++g) {
           const int st = g % ST, b = g % PL;
           if (!warp_spin(smem_u32(&s_c_full[st]), (uint32_t)(g / ST) & 1u, abort_flag)) { dead = true; break; }
-          if (!columns_fit || it.last - it.first - j * kC < kC) fence_proxy_async();
+          if (!columns_fit || it.w.last - it.w.first - j * kC < kC) fence_proxy_async();
           if (!warp_spin(smem_u32(&s_p_full[b]), (uint32_t)(g / PL) & 1u, abort_flag)) { dead = true; break; }
           tc_fence_after();
           const uint64_t cols_desc = c_desc + (uint32_t)st * (2 * S::kColBytes / 16u);
@@ -442,7 +438,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
       const Rows at{p, it};
 #pragma unroll 1
       for (int j = 0; j < it.tiles; ++j, ++g) {
-        const int st = g % ST, first = it.first + j * kC, cols = min(kC, it.last - first);
+        const int st = g % ST, first = it.w.first + j * kC, cols = min(kC, it.w.last - first);
         const uint32_t to1 = c_at + st * 2 * S::kColBytes, to2 = to1 + S::kColBytes, bar = smem_u32(&s_c_full[st]);
         if (!warp_wait(smem_u32(&s_c_empty[st]), ((uint32_t)(g / ST) & 1u) ^ 1u, abort_flag)) { dead = true; break; }
         if (fit && cols == kC) {
