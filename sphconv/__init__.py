@@ -10,7 +10,7 @@ from sphconv_b200 import *  # noqa: F401,F403
 from sphconv_b200 import __all__  # noqa: F401
 
 for _name in ("tensor", "functional", "conv", "modules", "utils", "sphconv_cuda", "rangevoxel", "voxelize", "quant",
-              "sharding", "pipeline"):
+              "sharding", "pipeline", "attention", "norm", "decoder"):
     _mod = importlib.import_module("sphconv_b200." + _name)
     sys.modules[__name__ + "." + _name] = _mod
     globals()[_name] = _mod

@@ -11,7 +11,11 @@ from .sphconv_cuda import config
 from ._capi import check_status
 from .pipeline import ScanPipeline
 from .voxelize import VoxelGenerator
+from .attention import CrossAttention
+from .decoder import QueryDecoder
+from .norm import ResidualNorm, RowNorm
 from .rangevoxel import RangeVoxel, merge_rangevoxel_batch, xyz2RangeVoxel
 
 __all__ = ["ScanPipeline", "VoxelGenerator", "Conv3d", "SparseConv3d", "SubMConv3d", "Sequential", "SparseSequential", "SphModule",
-           "SparseConvTensor", "config", "check_status", "RangeVoxel", "xyz2RangeVoxel", "merge_rangevoxel_batch"]
+           "SparseConvTensor", "config", "check_status", "CrossAttention", "QueryDecoder", "ResidualNorm", "RowNorm",
+           "RangeVoxel", "xyz2RangeVoxel", "merge_rangevoxel_batch"]

@@ -1,9 +1,10 @@
 """Cross attention of a head's queries to the rows of a sparse tensor: with ``SparseConvTensor.dense()``, which feeds a dense head, the
 other way out of the encoder.  Rows stay as they are, ragged over the scans.  No reference counterpart."""
 import math
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
+from torch import nn
 
 from . import _capi as C
 
@@ -31,3 +32,38 @@ def scan_rows(x) -> torch.Tensor:
     """k_ptr of a SparseConvTensor: int32 [B+1], where the rows of every scan begin and end."""
     ends = x.z_ptr.reshape(x.B, -1)[:, -1]
     return torch.cat([ends.new_zeros(1), ends]).to(torch.int32)
+
+
+class CrossAttention(nn.Module):
+    """cross_attention between its linear projections: forward(queries [n, channels], rows [m, row_channels], q_ptr, k_ptr,
+    key_mask=None) -> [n, channels].
+
+    The rows' keys and values are one product, read in place.  What asks the same rows again (a decoder's next token) keeps them:
+    k, v = project(rows) once, then attend(queries, k, v, q_ptr, k_ptr) for each."""
+
+    def __init__(self, channels: int, row_channels: int, heads: int, key_heads: Optional[int] = None,
+                 head_channels: Optional[int] = None, bias: bool = False):
+        super().__init__()
+        self.heads, self.key_heads = heads, heads if key_heads is None else key_heads
+        if self.heads < 1 or self.key_heads < 1 or self.heads % self.key_heads:
+            raise ValueError("{} heads are not a multiple of {} key heads".format(heads, self.key_heads))
+        if head_channels is None and channels % heads:
+            raise ValueError("{} channels are not a multiple of {} heads".format(channels, heads))
+        self.head_channels = channels // heads if head_channels is None else head_channels
+        self.to_q = nn.Linear(channels, self.heads * self.head_channels, bias)
+        self.to_kv = nn.Linear(row_channels, 2 * self.key_heads * self.head_channels, bias)
+        self.to_out = nn.Linear(self.heads * self.head_channels, channels, bias)
+
+    def extra_repr(self):
+        return "heads={}, key_heads={}, head_channels={}".format(self.heads, self.key_heads, self.head_channels)
+
+    def project(self, rows: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values of rows [m, row_channels]: two views of one [m, 2, key heads, head channels]."""
+        return self.to_kv(rows).view(rows.shape[0], 2, self.key_heads, self.head_channels).unbind(1)
+
+    def attend(self, queries, k, v, q_ptr, k_ptr, key_mask=None):
+        q = self.to_q(queries).view(queries.shape[0], self.heads, self.head_channels)
+        return self.to_out(cross_attention(q, k, v, q_ptr, k_ptr, key_mask).flatten(1))
+
+    def forward(self, queries, rows, q_ptr, k_ptr, key_mask=None):
+        return self.attend(queries, *self.project(rows), q_ptr, k_ptr, key_mask)

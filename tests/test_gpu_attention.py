@@ -286,3 +286,83 @@ def test_refusals():
     leaf = q.clone().requires_grad_()
     with pytest.raises(RuntimeError, match="twice"):
         torch.autograd.grad(cross_attention(leaf, k, v, q_ptr, k_ptr).sum(), leaf, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("hq,hkv,d", [(6, 2, 128), (4, 4, 40), (5, 1, 64)])
+def test_many_scans_of_very_different_lengths(hq, hkv, d, dtype):
+    """More scans than a warp has lanes, one of them with most of the keys and one with most of the queries."""
+    lq = [(7 * i) % 5 for i in range(75)]
+    lk = [(11 * i) % 9 for i in range(75)]
+    lk[40], lk[74], lq[33], lq[50] = 5000, 700, 400, 130
+    got, want = both(inputs(lq, lk, hq, hkv, d, TYPES[dtype], seed=9, extra=(3, 2)), True)
+    check(got, want)
+    sphconv.check_status()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_one_scan_of_most_keys_and_few_rows_is_split(dtype):
+    """A walk in as many parts as there are, on either side."""
+    check(*both(inputs([3, 90], [20000, 5], 2, 2, 64, TYPES[dtype], seed=11), True))
+    check(*both(inputs([9000, 2], [30, 3], 2, 1, 64, TYPES[dtype], seed=12), True))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_keys_that_are_the_values_and_shared_heads(dtype):
+    """One tensor as keys and values, and one head expanded to all: their gradients are the sums."""
+    t = TYPES[dtype]
+    q, k, _, q_ptr, k_ptr, _ = inputs([70, 9], [200, 31], 4, 4, 32, t, seed=13)
+    d_out = torch.randn(q.shape, device=DEV).to(t)
+    rows = k.detach().requires_grad_()
+    got, = torch.autograd.grad(cross_attention(q, rows, rows, q_ptr, k_ptr), rows, d_out)
+    want = attention64(q, k, k, q_ptr, k_ptr, d_out=d_out)
+    # each is rounded by itself, and their sum once more
+    half = torch.finfo(t).eps / 2
+    total = want["d_k"][0] + want["d_v"][0]
+    check({"rows": got}, {"rows": (total, want["d_k"][1] + want["d_v"][1] + half * total.abs())})
+    one = k[:, :1].detach().requires_grad_()
+    k4 = one.expand(-1, 4, -1)
+    out = cross_attention(q, k4, k4, q_ptr, k_ptr)
+    k4 = k4.detach().contiguous()
+    want = attention64(q, k4, k4, q_ptr, k_ptr, d_out=d_out)
+    check({"out": out.detach()}, {"out": want["out"]})
+    got, = torch.autograd.grad(out, one, d_out)
+    parts = torch.cat([want["d_k"][0], want["d_v"][0]], 1)
+    total = parts.sum(1, keepdim=True)
+    # eight terms: their sums are rounded seven times at most, each time half a step of at most the terms' sizes together
+    bound = (want["d_k"][1] + want["d_v"][1]).sum(1, keepdim=True) + 8 * half * parts.abs().sum(1, keepdim=True)
+    check({"one": got}, {"one": (total, bound)})
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_rows_far_apart(dtype):
+    """Offsets past 2^31 elements."""
+    t, n, d, far = TYPES[dtype], 75, 64, 1 << 25
+    store = torch.zeros(n * far, dtype=t, device=DEV)
+    q, k, v, q_ptr, k_ptr, _ = inputs([40, 3], [50, 25], 2, 1, d, t, seed=14)
+    far_k = store.as_strided((n, 1, d), (far, d, 1))
+    far_v = store.as_strided((n, 1, d), (far, d, 1), 4 * d)
+    far_k.copy_(k)
+    far_v.copy_(v)
+    assert (n - 1) * far > 2 ** 31
+    check(*both((q, far_k, far_v, q_ptr, k_ptr, None), True))
+    for lengths in ([1, 1], [300, 0]):
+        q = torch.randn(sum(lengths), 2, d, device=DEV).to(t)
+        args = (q, far_k, far_v, ptr(lengths), k_ptr, None)
+        check(*both(args, False))
+
+
+def test_more_values_than_31_bits():
+    n = (1 << 23) + 1000                        # times 4 heads of 64 channels
+    kv = torch.randn(400, 2, 4, 64, device=DEV).bfloat16()
+    k, v = (torch.zeros(n, 4, 64, dtype=torch.bfloat16, device=DEV) for _ in "kv")
+    k[-400:], v[-400:] = kv[:, 0], kv[:, 1]
+    q = torch.randn(3, 4, 64, device=DEV).bfloat16()
+    d_out = torch.randn_like(q)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    k_ptr = torch.tensor([0, n - 400, n], dtype=torch.int32, device=DEV)
+    out = cross_attention(*leaves, ptr([0, 3]), k_ptr)
+    got = dict(zip(("d_q", "d_k", "d_v"), torch.autograd.grad(out, leaves, d_out)), out=out.detach())
+    assert not got["d_k"][:-400].any() and not got["d_v"][:-400].any()
+    got["d_k"], got["d_v"] = got["d_k"][-400:], got["d_v"][-400:]
+    check(got, attention64(q.detach(), kv[:, 0], kv[:, 1], ptr([3]), ptr([400]), d_out=d_out))
