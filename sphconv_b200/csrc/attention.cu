@@ -61,15 +61,16 @@ __device__ __forceinline__ void load_tile(float* to, int d, int vec, Row row) {
   }
 }
 
-// s[i][j] = a[4 ty + i] . b[tx + 16 j]
+// s[i][j] = a[4 ty + i] . b[tx + 16 j], even and odd channels apart: two to an operation
 template <int DP>
 __device__ __forceinline__ void scores(float (&s)[4][4], const float* a, const float* b, int d, int tx, int ty) {
   constexpr int PITCH = DP + 4;
+  float2 sum[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-#pragma unroll 4
+    for (int j = 0; j < 4; ++j) sum[i][j] = make_float2(0.f, 0.f);
+#pragma unroll 2
   for (int c = 0; c < d; c += 4) {            // zeros up to a multiple of 4
     float4 x[4], y[4];
 #pragma unroll
@@ -79,9 +80,15 @@ __device__ __forceinline__ void scores(float (&s)[4][4], const float* a, const f
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        s[i][j] = fmaf(x[i].x, y[j].x, fmaf(x[i].y, y[j].y, fmaf(x[i].z, y[j].z, fmaf(x[i].w, y[j].w, s[i][j]))));
+      for (int j = 0; j < 4; ++j) {
+        sum[i][j] = fma2(make_float2(x[i].x, x[i].y), make_float2(y[j].x, y[j].y), sum[i][j]);
+        sum[i][j] = fma2(make_float2(x[i].z, x[i].w), make_float2(y[j].z, y[j].w), sum[i][j]);
+      }
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] = sum[i][j].x + sum[i][j].y;
 }
 
 // A thread's channels of a row: pieces of W consecutive ones, piece j at 16 W j + W tx.
@@ -90,9 +97,9 @@ struct Columns {
   static constexpr int W = DP >= 64 ? 4 : 2, N = DP / 16 / W;
 };
 
-// acc[i] += sum over n of p[4 ty + i][n] * v[n]
+// acc[i] += sum over n of p[4 ty + i][n] * v[n], channels two to an operation
 template <int DP>
-__device__ __forceinline__ void accumulate(float (&acc)[4][DP / 16], const float* p, const float* v, int tx, int ty) {
+__device__ __forceinline__ void accumulate(float2 (&acc)[4][DP / 32], const float* p, const float* v, int tx, int ty) {
   constexpr int PITCH = DP + 4, W = Columns<DP>::W, N = Columns<DP>::N;
 #pragma unroll 2
   for (int n = 0; n < kTile; n += 4) {
@@ -106,32 +113,34 @@ __device__ __forceinline__ void accumulate(float (&acc)[4][DP / 16], const float
     for (int m = 0; m < 4; ++m)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        float y[W];
+        float2 y[W / 2];
         const float* from = v + (n + m) * PITCH + 16 * W * j + W * tx;
-        if (W == 4) {
+        if constexpr (W == 4) {
           const float4 f = *(const float4*)from;
-          y[0] = f.x; y[1] = f.y; y[2 % W] = f.z; y[3 % W] = f.w;
+          y[0] = make_float2(f.x, f.y);
+          y[1] = make_float2(f.z, f.w);
         } else {
-          const float2 f = *(const float2*)from;
-          y[0] = f.x; y[1] = f.y;
+          y[0] = *(const float2*)from;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int w = 0; w < W; ++w) acc[i][j * W + w] = fmaf(x[i][m], y[w], acc[i][j * W + w]);
+          for (int w = 0; w < W / 2; ++w)
+            acc[i][j * W / 2 + w] = fma2(make_float2(x[i][m], x[i][m]), y[w], acc[i][j * W / 2 + w]);
       }
   }
 }
 
 template <typename T, int DP>
-__device__ __forceinline__ void store_row(const float (&acc)[DP / 16], float by, T* to, int d, int tx) {
+__device__ __forceinline__ void store_row(const float2 (&acc)[DP / 32], float by, T* to, int d, int tx) {
   constexpr int W = Columns<DP>::W, N = Columns<DP>::N;
 #pragma unroll
   for (int j = 0; j < N; ++j)
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const int c = 16 * W * j + W * tx + w;
-      if (c < d) to[c] = from_float<T>(acc[j * W + w] * by);
+      const float2 pair = acc[(j * W + w) / 2];
+      if (c < d) to[c] = from_float<T>((w % 2 ? pair.y : pair.x) * by);
     }
 }
 
@@ -182,13 +191,14 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
     return r < rows ? (const T*)p.q + q * p.q_row + h * p.q_head : nullptr;
   });
   const int2 keys = make_int2(w.first, w.last);
-  float o[4][DP / 16], top[4], sum[4];
+  float2 o[4][DP / 32];
+  float top[4], sum[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     top[i] = -INFINITY;
     sum[i] = 0.f;
 #pragma unroll
-    for (int j = 0; j < DP / 16; ++j) o[i][j] = 0.f;
+    for (int j = 0; j < DP / 32; ++j) o[i][j] = make_float2(0.f, 0.f);
   }
   for (int k0 = keys.x; k0 < keys.y; k0 += kTile) {
     __syncthreads();
@@ -229,7 +239,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
       }
       sum[i] = sum[i] * by + add;                                     // of this thread's columns; joined at the end
 #pragma unroll
-      for (int j = 0; j < DP / 16; ++j) o[i][j] *= by;
+      for (int j = 0; j < DP / 32; ++j) o[i][j] = mul2(o[i][j], make_float2(by, by));
     }
     __syncwarp();                                                     // a row of P belongs to half a warp
     accumulate<DP>(o, s_p, s_v, tx, ty);
@@ -316,11 +326,11 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
   if (KEYS) load_keys(s_r1, s_r2, row0, rows);
   else load_queries(s_r1, s_r2, row0, rows);
   const int2 span = make_int2(w.first, w.last);
-  float a1[4][DP / 16], a2[4][DP / 16];                               // dV ; dK or dQ
+  float2 a1[4][DP / 32], a2[4][DP / 32];                              // dV ; dK or dQ
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < DP / 16; ++j) a1[i][j] = a2[i][j] = 0.f;
+    for (int j = 0; j < DP / 32; ++j) a1[i][j] = a2[i][j] = make_float2(0.f, 0.f);
   for (int c0 = span.x; c0 < span.y; c0 += kTile) {
     __syncthreads();
     if (KEYS) load_queries(s_c1, s_c2, c0, min(kTile, span.y - c0));
