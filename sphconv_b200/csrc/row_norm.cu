@@ -221,19 +221,20 @@ __device__ __forceinline__ void statistics(const typename X::Pairs& x, Reducer& 
   inv = rsqrtf(fmaf(s[0], per_c, eps));
 }
 
-// 16-bit rows round what is left of it to 8 or 11 bits: 2^-21 is enough
+// The quotient of a fast division is off by 2^-22 at most; 16-bit rows round what is left to 8 or 11 bits, and take a fast exponential too.
 template <typename T>
-__device__ __forceinline__ float sigmoid(float x) {
-  if (sizeof(T) == 2) return __fdividef(1.f, 1.f + __expf(-x));
-  return 1.f / (1.f + expf(-x));
-}
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + (sizeof(T) == 2 ? __expf(-x) : expf(-x))); }
 template <typename T>
 __device__ __forceinline__ float2 sigmoid(float2 x) { return make_float2(sigmoid<T>(x.x), sigmoid<T>(x.y)); }
 
-// BIAS: there may be biases.  THREADS: most threads of a block; a small one leaves room for three on an SM (rows of 64 bf16 channels 85 ->
-// FWD us), two backward, whose sums take the registers.
+// Blocks of an SM: what their registers have room for, backward with the sums over rows in them.  Each keeps a row on its way (rows of 64
+// bf16 channels, three blocks forward instead of two: 85 -> 75 us).
+constexpr int forward_blocks_per_sm(int threads) { return threads >= 512 ? 1 : 768 / threads; }
+constexpr int backward_blocks_per_sm(int threads) { return threads >= 512 ? 1 : 512 / threads; }
+
+// BIAS: there may be biases.  THREADS: most threads of a block.
 template <typename T, int VEC, int NV, bool CENTER, bool BIAS, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) forward_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(THREADS, forward_blocks_per_sm(THREADS)) forward_kernel(const __grid_constant__ Params p) {
   using X = Tile<T, VEC, NV>;
   constexpr int P = X::P;
   using Pairs = typename X::Pairs;
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) forward_kerne
 }
 
 template <typename T, int VEC, int NV, bool CENTER, bool BIAS, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) backward_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(THREADS, backward_blocks_per_sm(THREADS)) backward_kernel(const __grid_constant__ Params p) {
   using X = Tile<T, VEC, NV>;
   constexpr int E = X::E, P = X::P;
   using Pairs = typename X::Pairs;
@@ -502,11 +503,15 @@ struct Shape {
 bool shape_of(int c, int esize, bool whole, Shape* s) {
   const int full = 16 / esize;
   s->vec = whole ? full : 1;
-  // 8 values a thread; 16 where more than 512 threads would be needed
-  for (const int e : {8, 16}) {
+  // A piece of 16 bytes a thread, or four elements: what backward keeps of a row in registers, without spilling (float32 rows of 1024
+  // channels, eight values instead of four: backward 97 -> 116 us; bf16 rows of 333, 118 -> 312).  More a thread for rows that would need
+  // more than 512 threads, or 256 where the pieces of float32 rows still fit then (2048 channels: forward 74 -> 59 us).
+  for (const int e : {4, 8, 16}) {
+    if (e < s->vec) continue;
+    const int most = e == 4 && s->vec == 4 ? 256 : 512;
     s->nv = e / s->vec;
     s->lanes = 1;
-    while (s->lanes < 512 && s->lanes * e < c) s->lanes *= 2;
+    while (s->lanes < most && s->lanes * e < c) s->lanes *= 2;
     if (s->lanes * e >= c) {
       s->threads = s->lanes > 32 ? s->lanes : kBlock;
       return true;
@@ -519,7 +524,6 @@ int grid_of(const Shape& s, int64_t n, int sms, int per_sm) {
   const int64_t blocks = div_up64(n, s.threads / s.lanes);
   return (int)std::min<int64_t>(blocks, (int64_t)sms * per_sm);
 }
-int backward_blocks_per_sm(const Shape& s) { return std::max(1, 512 / s.threads); }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool params_aligned(const Params& p) {
@@ -572,15 +576,18 @@ void start(bool backward, bool center, int grid, const Shape& s, cudaStream_t st
 template <typename T>
 void start(bool backward, bool center, int grid, const Shape& s, cudaStream_t st, const Params& p) {
   constexpr int V = Row<T>::kVec;
-  const bool wide = s.vec * s.nv == 16, large = s.threads > kBlock;
+  const bool large = s.threads > kBlock;
   if (s.vec == 1) {
-    if (wide) start<T, 1, 16, 512>(backward, center, grid, s, st, p);
-    else if (large) start<T, 1, 8, 512>(backward, center, grid, s, st, p);
-    else start<T, 1, 8, kBlock>(backward, center, grid, s, st, p);
+    if (s.nv == 16) start<T, 1, 16, 512>(backward, center, grid, s, st, p);
+    else if (s.nv == 8) start<T, 1, 8, 512>(backward, center, grid, s, st, p);
+    else if (large) start<T, 1, 4, 512>(backward, center, grid, s, st, p);
+    else start<T, 1, 4, kBlock>(backward, center, grid, s, st, p);
   } else {
-    if (wide) start<T, V, 16 / V, 512>(backward, center, grid, s, st, p);
-    else if (large) start<T, V, 8 / V, 512>(backward, center, grid, s, st, p);
-    else start<T, V, 8 / V, kBlock>(backward, center, grid, s, st, p);
+    if (s.nv == 1 && !large) start<T, V, 1, kBlock>(backward, center, grid, s, st, p);
+    else if (s.nv == 2 && large) start<T, V, 2, 512>(backward, center, grid, s, st, p);
+    else if constexpr (V == 8) start<T, V, 1, 512>(backward, center, grid, s, st, p);
+    else if (s.nv == 2) start<T, V, 2, kBlock>(backward, center, grid, s, st, p);
+    else start<T, V, 4, 512>(backward, center, grid, s, st, p);
   }
 }
 int start(int dtype, bool backward, bool center, int grid, const Shape& s, cudaStream_t st, Params& p) {
@@ -614,16 +621,20 @@ extern "C" int sph_residual_norm(const sph_norm* a, void* d_out, void* d_normed,
                      (p.gate_row || aligned16(a->gate)) && aligned16(d_out) && aligned16(d_normed) && params_aligned(p);
   Shape s;
   if (!shape_of(a->c, e, whole, &s)) { set_error("%s: too many channels", __func__); return SPH_ERR_LIMIT; }
-  return start(a->dtype, false, a->center != 0, grid_of(s, a->n, sms, std::max(1, 768 / s.threads)), s, (cudaStream_t)stream, p);
+  return start(a->dtype, false, a->center != 0, grid_of(s, a->n, sms, forward_blocks_per_sm(s.threads)), s, (cudaStream_t)stream, p);
 }
 
 extern "C" int64_t sph_residual_norm_scratch_bytes(int64_t n, int32_t c) {
   if (n < 0 || c <= 0) { set_error("%s: bad sizes", __func__); return SPH_ERR_INVALID; }
   const int sms = current_sm_count();
   if (sms <= 0) return SPH_ERR_CUDA;
-  Shape s;                                    // how many threads a row has goes by its channels alone
-  if (!shape_of(c, 4, false, &s)) { set_error("%s: %d channels, at most %d are supported", __func__, c, SPH_NORM_MAX_CHANNELS); return SPH_ERR_LIMIT; }
-  return std::max<int64_t>(1, grid_of(s, n, sms, backward_blocks_per_sm(s))) * kSums * c * (int64_t)sizeof(float);
+  int64_t blocks = 1;                         // of either way to read a row
+  for (const int esize : {2, 4}) {
+    Shape s;
+    if (!shape_of(c, esize, esize == 2, &s)) { set_error("%s: %d channels, at most %d are supported", __func__, c, SPH_NORM_MAX_CHANNELS); return SPH_ERR_LIMIT; }
+    blocks = std::max<int64_t>(blocks, grid_of(s, n, sms, backward_blocks_per_sm(s.threads)));
+  }
+  return blocks * kSums * c * (int64_t)sizeof(float);
 }
 
 extern "C" int sph_residual_norm_backward(const sph_norm* a, const void* d_dout, const void* d_dnormed, const float* d_stats,
@@ -654,7 +665,7 @@ extern "C" int sph_residual_norm_backward(const sph_norm* a, const void* d_dout,
   q.partial = p.partial;
   q.c = a->c;
   if (a->n > 0) {
-    q.blocks = grid_of(s, a->n, sms, backward_blocks_per_sm(s));
+    q.blocks = grid_of(s, a->n, sms, backward_blocks_per_sm(s.threads));
     const int done = start(a->dtype, true, a->center != 0, q.blocks, s, (cudaStream_t)stream, p);
     if (done != SPH_OK) return done;
   }
