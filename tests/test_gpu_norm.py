@@ -103,6 +103,15 @@ def test_forward_and_gradients(n, c, dtype, given, center):
     wants = torch.autograd.grad([p[1] for p in pairs], [v64[k] for k in names], [p[2].double() for p in pairs])
     held = [x for x in reference(v64, 1e-5, center, fixed=True) if x is not None]
     parts = torch.autograd.grad(held[-len(pairs):], [v64[k] for k in names], [p[2].double() for p in pairs])
+    if v["gate"] is not None and v["gate"].shape != v["residual"].shape:
+        # A row's gate has the sum over channels of total_c j_c, where total is the gradient of `out`, which is the residual's, and j_c that
+        # of out_c in the logit.  total_c is off by what `close` allows a residual, of the size of the row's largest; the sum and j_c round
+        # to 2^-24 of |total_c j_c| a few times: altogether of the size of that largest value times the sum of |j_c|.
+        wide = dict(v64, gate=v64["gate"].detach().expand(n, c).contiguous().requires_grad_())
+        j, = torch.autograd.grad(reference(wide, 1e-5, center)[0].sum(), wide["gate"])
+        at = names.index("residual")
+        largest = torch.maximum(wants[at].abs(), parts[at].abs()).amax(-1, keepdim=True)
+        parts = [largest * j.abs().sum(-1, keepdim=True) if k == "gate" else x for k, x in zip(names, parts)]
     for k, got, want, part in zip(names, grads, wants, parts):
         assert got.dtype == v[k].dtype and got.shape == v[k].shape
         if k in ("block", "residual", "gate"):
@@ -227,3 +236,33 @@ def test_refusals():
     leaf = x.clone().requires_grad_()
     with pytest.raises(RuntimeError, match="twice"):
         torch.autograd.grad(row_norm(leaf, w).sum(), leaf, create_graph=True)
+
+
+@pytest.mark.parametrize("n,c,dtype,given,center", [
+    # as many values a thread and threads a row as there are kinds of either, with rows enough that blocks have several
+    (700, 1024, "fp32", ("block", "weight", "gate", "scale", "next_weight"), False),
+    (500, 2048, "fp32", ("block", "weight", "bias", "gate", "scale", "next_weight", "next_bias"), True),
+    (400, 4096, "fp32", ("block", "weight", "gate_row", "scale", "next_weight"), False),
+    (400, 8192, "fp32", ("block", "weight", "bias", "gate", "scale", "next_weight", "next_bias"), True),
+    (400, 8190, "bf16", ("block", "weight", "gate", "scale", "next_weight", "next_bias"), False),
+    (400, 4104, "bf16", ("block", "weight", "gate_row", "scale", "next_weight"), False),
+    (500, 1999, "fp16", ("block", "weight", "bias", "gate", "next_weight", "next_bias"), True),
+    (500, 2100, "bf16", ("block", "gate", "scale", "next_weight"), False),
+    (450, 3001, "fp32", ("block", "weight", "gate_row", "scale", "next_weight"), False),
+])
+def test_wide_rows(n, c, dtype, given, center):
+    test_forward_and_gradients(n, c, dtype, given, center)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_gates_at_their_ends(dtype):
+    """Logits whose exponential is zero or infinite: a gate of exactly one or zero, and gradients without NaN."""
+    t = TYPES[dtype]
+    end = 6e4 if t == torch.float16 else 3e38
+    gate = torch.tensor([[-end], [-200.0], [0.0], [200.0], [end]], device=DEV).to(t).expand(5, 40).contiguous().requires_grad_()
+    block, residual = torch.full((5, 40), 2.0, device=DEV).to(t).requires_grad_(), torch.ones(5, 40, device=DEV).to(t)
+    out, _ = residual_norm(block, residual, gate=gate)
+    assert torch.equal(out[:, 0].float(), torch.tensor([1.0, 1.0, 2.0, 3.0, 3.0], device=DEV))
+    d_block, d_gate = torch.autograd.grad(out.float().sum(), (block, gate))
+    assert torch.equal(d_block[:, 0].float(), torch.tensor([0.0, 0.0, 0.5, 1.0, 1.0], device=DEV))
+    assert torch.equal(d_gate[:, 0].float(), torch.tensor([0.0, 0.0, 0.5, 0.0, 0.0], device=DEV))
