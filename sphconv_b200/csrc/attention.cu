@@ -356,6 +356,10 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
   for (int i = 0; i < 4; ++i) {
     const int r = 4 * ty + i;
     if (r >= rows) continue;
+    if (KEYS ? !s_key[r] : s_lse[r] == INFINITY) {                    // no key, or a query without: zeros, whatever the other side holds
+#pragma unroll
+      for (int j = 0; j < DP / 32; ++j) a1[i][j] = a2[i][j] = make_float2(0.f, 0.f);
+    }
     int64_t at_row;                                                   // of [rows][heads]
     if (KEYS) {
       at_row = (int64_t)(w.k0 + row0 + r) * p.hkv + key_head;

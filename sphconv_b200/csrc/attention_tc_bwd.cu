@@ -217,13 +217,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
         continue;
       }
       const bool any_row = quarter * 32 < it.rows, mine = r < it.rows;
-      const bool row_is = mine && (!KEYS || at.is_key(it.row0 + r));  // a key, or a query
       float lse = -INFINITY, delta = 0.f;     // minus the row's; -infinity: P = 0
       if (!KEYS && mine) {
         const int64_t q = at.query(it.row0 + r);
         lse = kShift - p.lse[q];
         delta = -p.delta[q];
       }
+      // a key, or a query that has some: else its results are zeros, whatever the other side holds
+      const bool row_is = mine && (KEYS ? at.is_key(it.row0 + r) : lse != -INFINITY);
       const float row_lse[4] = {lse, lse, lse, lse}, row_delta[4] = {delta, delta, delta, delta};
       const int j0 = first_tile(g);
       float& row_f = s_f[n & 1][r];

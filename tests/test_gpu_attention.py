@@ -366,3 +366,44 @@ def test_more_values_than_31_bits():
     assert not got["d_k"][:-400].any() and not got["d_v"][:-400].any()
     got["d_k"], got["d_v"] = got["d_k"][-400:], got["d_v"][-400:]
     check(got, attention64(q.detach(), kv[:, 0], kv[:, 1], ptr([3]), ptr([400]), d_out=d_out))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("layout", ["apart", "odd"])
+def test_gradients_that_are_not_finite_where_nothing_is_read(dtype, layout):
+    """NaN on its way back to queries without keys stays away from everything: they have zeros, and so do their scan's keys."""
+    q, k, v, q_ptr, k_ptr, _ = inputs([40, 200, 7], [300, 129, 0], 2, 2, 64, TYPES[dtype], layout=layout)
+    mask = torch.ones(k.shape[0], dtype=torch.bool, device=DEV)
+    mask[300:] = False                                    # every key of the second scan
+    mask[7] = False
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = cross_attention(*leaves, q_ptr, k_ptr, mask)
+    d_out = torch.randn(out.shape, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).to(out.dtype)
+    want = attention64(q, k, v, q_ptr, k_ptr, mask, d_out=d_out)
+    d_out[40:] = float("nan")
+    d_out[100:120] = float("inf")
+    got = dict(zip(("d_q", "d_k", "d_v"), torch.autograd.grad(out, leaves, d_out)), out=out.detach())
+    check(got, want)
+    assert not got["d_q"][40:].any() and not got["d_k"][~mask].any() and not got["d_v"][~mask].any()
+    # and in a scan with keys, whose gradients it spoils, those of what is no key are zeros all the same
+    d_out[3] = float("nan")
+    _, d_k, d_v = torch.autograd.grad(cross_attention(*leaves, q_ptr, k_ptr, mask), leaves, d_out)
+    assert not d_k[~mask].any() and not d_v[~mask].any()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_one_query_row_for_all_and_a_head_for_each(dtype):
+    """Queries broadcast over rows and heads (strides of zero), and more query heads of a key head than a tile has rows."""
+    t = TYPES[dtype]
+    _, k, v, q_ptr, k_ptr, _ = inputs([90, 1, 60], [70, 200, 31], 2, 2, 64, t, seed=21)
+    one = torch.randn(1, 1, 64, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).to(t)
+    check(*both((one.expand(151, 2, 64), k, v, q_ptr, k_ptr, None), True))
+    q, k, v, q_ptr, k_ptr, _ = inputs([3, 0, 2], [70, 200, 31], 300, 1, 48, t, seed=22)
+    check(*both((q, k, v, q_ptr, k_ptr, None), True))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_a_thousand_scans(dtype):
+    lq, lk = [i % 3 for i in range(1000)], [i % 4 * 5 for i in range(1000)]
+    check(*both(inputs(lq, lk, 2, 1, 32, TYPES[dtype], seed=23), True))
+    check(*both(inputs([1] * 1000, lk, 2, 2, 64, TYPES[dtype], seed=24), False))
