@@ -155,18 +155,6 @@ __device__ __forceinline__ Work block_work(const Params& p) {
   return s_work;
 }
 
-// Scans that are not in order, or not within the rows, are reported.
-__device__ __forceinline__ void check_scans(const Params& p) {
-  if (blockIdx.x != 0 || p.status == nullptr) return;
-  bool bad = false;
-  for (int b = threadIdx.x; b <= p.B; b += blockDim.x) {
-    const int q = __ldg(p.q_ptr + b), k = __ldg(p.k_ptr + b);
-    bad |= q < 0 || q > p.n_q || k < 0 || k > p.n_k;
-    if (b < p.B) bad |= q > __ldg(p.q_ptr + b + 1) || k > __ldg(p.k_ptr + b + 1);
-  }
-  if (bad) atomicOr(p.status, SPH_STATUS_BAD_INDEX);
-}
-
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Params p) {
   constexpr int PITCH = DP + 4;
@@ -174,7 +162,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   float *s_q = smem, *s_k = s_q + kTile * PITCH, *s_v = s_k + kTile * PITCH, *s_p = s_v + kTile * PITCH;
   __shared__ uint8_t s_key[kTile];
   after_previous();
-  check_scans(p);
+  report_scans(p);
   const int key_head = blockIdx.x % p.hkv;
   const Work w = block_work<true>(p);
   if (w.scan < 0) return;
@@ -380,13 +368,14 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
   }
 }
 
-// delta of every row of every query head, a warp each; the first two warps plan what the tensor-core kernels do, for dQ and for dK and dV.
+// delta of every row of every query head, a warp each; with dq.plan the first two warps plan what the tensor-core kernels do, for dQ and
+// for dK and dV.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) delta_kernel(const T* d_out, const T* out, float* delta, int64_t rows, int d,
                                                          const __grid_constant__ Params dq, const __grid_constant__ Params dkv) {
   after_previous();
   const int lane = threadIdx.x & 31;
-  if (blockIdx.x == 0 && threadIdx.x < 64) {
+  if (dq.plan != nullptr && blockIdx.x == 0 && threadIdx.x < 64) {
     const Params& p = threadIdx.x < 32 ? dq : dkv;
     auto leave = [&](const ScanPlan& x, int s0) {
       if (s0 + lane < p.B + 2) const_cast<ScanPlan*>(p.plan)[s0 + lane] = x;
@@ -613,7 +602,7 @@ int run_backward(Params p, const Plan& plan, bool tensor_cores, const void* out,
   p.part_count = (int*)(plans + 2 * (p.B + 2));
   p.part = (float*)p.part_count + (std::max(rows, (int64_t)p.n_k * p.hkv) + 3) / 4 * 4;
   Params dq = p, dkv = p;
-  dq.parts = plan.dq.parts; dq.aim = plan.dq.aim; dq.plan = plans;
+  dq.parts = plan.dq.parts; dq.aim = plan.dq.aim; dq.plan = tensor_cores ? plans : nullptr;
   dkv.parts = plan.dkv.parts; dkv.aim = plan.dkv.aim; dkv.plan = plans + p.B + 2;
   dkv.part2 = dkv.part + k_values * dkv.parts;
   launch(delta_kernel<T>, std::max(1u, grid_for(rows, kThreads / 32)), kThreads, 0, st, (const T*)p.d_out, (const T*)out, delta, rows, p.d, dq, dkv);

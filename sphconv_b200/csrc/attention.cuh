@@ -39,6 +39,18 @@ struct Params {
   int* status;
 };
 
+// Scans that are not in order, or not within the rows, are reported by the first block.
+__device__ __forceinline__ void report_scans(const Params& p) {
+  if (blockIdx.x != 0 || p.status == nullptr) return;
+  bool bad = false;
+  for (int b = threadIdx.x; b <= p.B; b += blockDim.x) {
+    const int q = __ldg(p.q_ptr + b), k = __ldg(p.k_ptr + b);
+    bad |= q < 0 || q > p.n_q || k < 0 || k > p.n_k;
+    if (b < p.B) bad |= q > __ldg(p.q_ptr + b + 1) || k > __ldg(p.k_ptr + b + 1);
+  }
+  if (bad) atomicOr(p.status, SPH_STATUS_BAD_INDEX);
+}
+
 // A scan's rows and how they are divided: its tiles' parts are numbers upto - tiles * parts .. upto - 1.
 struct __align__(16) ScanPlan {
   int upto, parts, per, tiles;                              // per: rows of the walk that a part has

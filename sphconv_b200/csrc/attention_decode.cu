@@ -72,15 +72,7 @@ __global__ void __launch_bounds__(kThreadsDecode, 2) decode_kernel(const __grid_
   __shared__ float s_m[kWarps][R], s_l[kWarps][R];
   __shared__ __align__(16) float s_o[kWarps][R][LANES * E];           // written two at a time
   after_previous();
-  if (blockIdx.x == 0 && p.status != nullptr) {             // scans that are not in order, or not within the rows
-    bool bad = false;
-    for (int b = threadIdx.x; b <= p.B; b += kThreadsDecode) {
-      const int q = __ldg(p.q_ptr + b), k = __ldg(p.k_ptr + b);
-      bad |= q < 0 || q > p.n_q || k < 0 || k > p.n_k;
-      if (b < p.B) bad |= q > __ldg(p.q_ptr + b + 1) || k > __ldg(p.k_ptr + b + 1);
-    }
-    if (bad) atomicOr(p.status, SPH_STATUS_BAD_INDEX);
-  }
+  report_scans(p);
   const int head = blockIdx.x % p.hkv;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (warp == 0) {

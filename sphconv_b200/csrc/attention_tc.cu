@@ -79,18 +79,6 @@ __device__ __forceinline__ void scale_row(uint32_t at, int d, float by) {
   }
 }
 
-// Scans that are not in order, or not within the rows, are reported by the first block.
-__device__ __forceinline__ void report_scans(const Params& p) {
-  if (blockIdx.x != 0 || p.status == nullptr) return;
-  bool bad = false;
-  for (int b = threadIdx.x; b <= p.B; b += blockDim.x) {
-    const int q = __ldg(p.q_ptr + b), k = __ldg(p.k_ptr + b);
-    bad |= q < 0 || q > p.n_q || k < 0 || k > p.n_k;
-    if (b < p.B) bad |= q > __ldg(p.q_ptr + b + 1) || k > __ldg(p.k_ptr + b + 1);
-  }
-  if (bad) atomicOr(p.status, SPH_STATUS_BAD_INDEX);
-}
-
 // Row r of a block's tile: of which query and head it is.
 struct Row {
   int64_t q;

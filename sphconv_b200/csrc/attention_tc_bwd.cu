@@ -20,7 +20,7 @@
 // warps that have a row take turns at it.
 //
 // P and dS are rounded to the rows' type for their products, and delta comes from the rounded output: gradients of bf16 rows are off by 0.0024
-// to 0.0028 of their size (root mean square), where their own rounding makes 0.0017 (0.0024 with that of dS).
+// to 0.0030 of their size (root mean square), where their own rounding makes 0.0017 (0.0024 with that of dS).
 // 8 scans of 300 queries and 12000 keys, 8 heads of 64 bf16 channels: dQ 155 us, dK and dV 225 us, 565 TFLOP/s of the seven products
 // together; the tensor pipe is 26 and 34 % busy, issue 35 and 44 %.
 #include <algorithm>
