@@ -83,6 +83,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __half2 v = __floats2half2_rn(a, b);
   return *(const uint32_t*)&v;
 }
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*(const __half2*)&w);
+}
 
 // Rows of one head, or of the heads of a group, as TMA brings them to a tile: blocks of 64 channels, zeros behind the last one.
 struct TileMap {

@@ -6,7 +6,7 @@
 //   P = 2^(scale log2 e S - lse),  dS = P (dP - delta);  lse and delta belong to the query: to the column, or to the row.
 // Both products of a tile give S and dP in TMEM; a thread reads its row of both, writes P and dS over them in the rows' type, and these
 // are the A operands of the products behind them, whose B operands are the column tiles again, MN-major.  Nothing is transposed,
-// and the accumulators stay in TMEM to the end.  That the scores are made twice, once a direction, costs 7 products in place of 5; in
+// and the accumulators stay in TMEM to the end.  That the scores are made twice, once a direction, costs 7 products in place of 5 (9 with the second value of dS); in
 // return there are no atomics, and results are the same every time.
 //
 // A block has an SM, with all of its TMEM, and takes one tile of rows after the other: the first scores of the next one are made, and its
@@ -19,10 +19,12 @@
 // value down when that outgrows the type (the accumulator is scaled along).  Even and odd tiles add to one accumulator, so the two
 // warps that have a row take turns at it.
 //
-// P and dS are rounded to the rows' type for their products, and delta comes from the rounded output: gradients of bf16 rows are off by 0.0024
-// to 0.0030 of their size (root mean square), where their own rounding makes 0.0017 (0.0024 with that of dS).
-// 8 scans of 300 queries and 12000 keys, 8 heads of 64 bf16 channels: dQ 155 us, dK and dV 225 us, 565 TFLOP/s of the seven products
-// together; the tensor pipe is 26 and 34 % busy, issue 35 and 44 %.
+// A score's gradients cancel - dS sums to zero over a query's keys - so dS goes into its products as two values of the rows' type, itself and
+// what that lost, one product more for either gradient.  P for dV is rounded, and delta comes from the rounded output: with bf16 rows
+// dQ is off by 0.0017 to 0.0026 of its size (root mean square), dK by 0.0017 to 0.0019, dV by 0.0024, where their own rounding makes 0.0017.  With dS
+// rounded once dQ had 0.0024 to 0.0030 and dK 0.0023 to 0.0027, at 504 us in place of 550:
+// 8 scans of 300 queries and 12000 keys, 8 heads of 64 bf16 channels, forward and backward together 550 us; dQ 165, dK and dV 260.  No unit is full:
+// with dS rounded once the tensor pipe was 34 and 26 % busy, issue 35 and 44 %.
 #include <algorithm>
 
 #include "attention_tc.cuh"
@@ -300,7 +302,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
         }
         if (any_row) {
           tc_fence_after();
-          // in the order of columns: P and dS take half of the place of what they are made from
+          // in the order of columns: P and dS take half of the place of what they are made from, and what dS lost in rounding goes
+          // where S was (KEYS: to the second half, once that has been read)
+          uint32_t lost[kC / 16][8];
 #pragma unroll
           for (int c = 0; c < kC; c += 16) {
             uint32_t v[16], u[16], h[8], e[8];
@@ -311,9 +315,20 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
               float2 y = make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
               if (!BF16) y = mul2(y, make_float2(f, f));
               e[i] = pack2<BF16>(y.x, y.y);
+              y = fma2(unpack2<BF16>(e[i]), make_float2(-1.f, -1.f), y);
+              lost[c / 16][i] = pack2<BF16>(y.x, y.y);
             }
             if (KEYS) tmem_st8(at_s + c / 2, h);
             tmem_st8(at_dp + c / 2, e);
+            if (!KEYS) {
+              tmem_st8(at_s + c / 2, lost[c / 16]);
+            } else if (c == 32) {
+              tmem_st8(at_s + 32, lost[0]);
+              tmem_st8(at_s + 40, lost[1]);
+            } else if (c == 48) {
+              tmem_st8(at_s + 48, lost[2]);
+              tmem_st8(at_s + 56, lost[3]);
+            }
           }
           tmem_st_wait();
           tc_fence_before();
@@ -425,6 +440,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
           if (one) {
 #pragma unroll
             for (int s = 0; s < kC / 16; ++s) umma_f16_ta(to, from + 8 * s, cols_desc + (uint64_t)(s * (2048 / 16)), idesc, j || s ? 1u : 0u);
+            if (x) {
+#pragma unroll
+              for (int s = 0; s < kC / 16; ++s)
+                umma_f16_ta(to, tmem + S::s_at(b) + (KEYS ? 32u : 0u) + 8 * s, cols_desc + (uint64_t)(s * (2048 / 16)), idesc, 1u);
+            }
             umma_commit(smem_u32(&s_done[b]));
             umma_commit(smem_u32(&s_c_empty[st]));
             if (j == it.tiles - 1) umma_commit(smem_u32(&s_all));
