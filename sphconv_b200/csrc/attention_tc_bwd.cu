@@ -6,8 +6,8 @@
 //   P = 2^(scale log2 e S - lse),  dS = P (dP - delta);  lse and delta belong to the query: to the column, or to the row.
 // Both products of a tile give S and dP in TMEM; a thread reads its row of both, writes P and dS over them in the rows' type, and these
 // are the A operands of the products behind them, whose B operands are the column tiles again, MN-major.  Nothing is transposed,
-// and the accumulators stay in TMEM to the end.  That the scores are made twice, once a direction, costs 7 products in place of 5 (9 with the second value of dS); in
-// return there are no atomics, and results are the same every time.
+// and the accumulators stay in TMEM to the end.  That the scores are made twice, once a direction, costs 7 products in place of 5 (9 with
+// the second value of dS); in return there are no atomics, and results are the same every time.
 //
 // A block has an SM, with all of its TMEM, and takes one tile of rows after the other: the first scores of the next one are made, and its
 // rows brought, while the results of the last are stored.  Warps 0-3 and 4-7 take even and odd tiles of columns, a thread a row; warps 8
