@@ -14,8 +14,8 @@
 // Backward reads the block, the residual, the gate and the two gradients, makes `out` again in float32 (the rounded one would shift
 // the gradient of a 16-bit row's norm) and takes mean and 1/deviation of both norms from the forward pass (16 bytes a row).  The
 // threads of a persistent grid own columns, so the sums over rows - gradients of weights, biases and the scale - stay in registers
-// (in shared memory with 16 values a thread: 2048 float32 rows of 8192 channels 275 -> 187 us) until the end; each block leaves its sums in the scratch, and a second launch adds those up in a fixed order: no atomics, the same
-// bits every time.
+// (in shared memory with 16 values a thread: 2048 float32 rows of 8192 channels 275 -> 187 us) until the end; each block leaves its
+// sums in the scratch, and a second launch adds those up in a fixed order: no atomics, the same bits every time.
 #include <algorithm>
 
 #include "common.cuh"
@@ -650,10 +650,13 @@ extern "C" int64_t sph_residual_norm_scratch_bytes(int64_t n, int32_t c) {
   if (n < 0 || c <= 0) { set_error("%s: bad sizes", __func__); return SPH_ERR_INVALID; }
   const int sms = current_sm_count();
   if (sms <= 0) return SPH_ERR_CUDA;
-  int64_t blocks = 1;                         // of either way to read a row
-  for (const int esize : {2, 4}) {
+  int64_t blocks = 1;                         // of any way to read a row
+  for (const int way : {0, 1, 2}) {
     Shape s;
-    if (!shape_of(c, esize, esize == 2, &s)) { set_error("%s: %d channels, at most %d are supported", __func__, c, SPH_NORM_MAX_CHANNELS); return SPH_ERR_LIMIT; }
+    if (!shape_of(c, way == 0 ? 2 : 4, way != 2, &s)) {
+      set_error("%s: %d channels, at most %d are supported", __func__, c, SPH_NORM_MAX_CHANNELS);
+      return SPH_ERR_LIMIT;
+    }
     blocks = std::max<int64_t>(blocks, grid_of(s, n, sms, backward_blocks_per_sm(s.threads)));
   }
   return blocks * kSums * c * (int64_t)sizeof(float);
