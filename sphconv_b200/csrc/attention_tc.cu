@@ -7,9 +7,14 @@
 // A block has one tile of queries (heads that share a key head are rows of it) and walks a scan's keys, or a part of them; two blocks
 // share an SM.  Keys and values come by TMA where a tile has all of its rows, and row by row with cp.async, which fills in zeros, where
 // keys are missing (the scan's end, a mask).
-//   P is taken against the row's maximum in its first tile, without looking for another one: what shows that the maximum has grown
-// too far is the sum of P over a tile, above 2^12.  Only then it is searched, O is read, scaled and written again, and P made anew.
-// Any P is below 2^12 then, which is no matter to a floating-point type.
+//   bf16: P is taken against the row's maximum in its first tile, without looking for another one: what shows that the maximum has
+// grown too far is the sum of P over a tile, above 2^12.  Only then it is searched, O is read, scaled and written again, and P made anew.
+// Any P is below 2^12 then, and has all of its bits.
+//   float16 has no room for that: it loses bits below 2^-14, and all of them below 2^-25.  Keys far below a row's largest are little each, but tens of
+// thousands of them are not, and where their scores are alike so is what each loses (40000 equal ones 16 below one key: the result off by
+// 6 %).  So P is held times 2^15, against a maximum that is looked for in every tile and followed when a score is 2^0.9 above it: at most
+// 2^-40 of the largest value is lost a key.  200 queries, 8 scans of 87 k rows, 4 heads of 32: 285 us, 248 against the first tile's without the
+// factor, 264 with a factor of 2^12 and a maximum that may be 2^3.9 behind.
 //
 // Warps 0-3 do the softmax, a thread a row; warps 4 and 5 issue the MMAs of S and of O (one warp for both took 1100 cycles a tile, most of
 // them waits that were over); warps 6 and 7 load.  S has two places, so that the next scores are there when a row's softmax ends.
@@ -33,16 +38,20 @@ namespace attn {
 namespace {
 
 constexpr int kN = 64;                        // keys of a tile
-constexpr float kMostSum = 4096.f;            // of a row's P over a tile: above it the row's maximum is taken anew
+constexpr float kMostSum = 4096.f;            // bf16, of a row's P over a tile: above it the row's maximum is taken anew
+constexpr float kShiftP = 15.f;               // fp16: P times 2^15
+constexpr float kSlack = 0.9f;                // fp16: the row's maximum is taken anew when a score is 2^0.9 above it: 2^15.9 < 65504
 
-// P = 2^(scale s + minus) of N scores in the rows' type, and the sum of P before rounding.
+// P = 2^(scale s + minus) of N scores in the rows' type, and the sum of P before rounding; fp16: 2^(scale (s + minus) + 15), so that
+// the largest score has no rounding to add to its exponent.
 template <bool BF16, int N>
 __device__ __forceinline__ float row_exp(const uint32_t (&s)[N], uint32_t* h, float scale, float minus) {
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   const float2 scale2 = make_float2(scale, scale), minus2 = make_float2(minus, minus);
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
-    const float2 e = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, minus2);
+    const float2 x = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+    const float2 e = BF16 ? fma2(x, scale2, minus2) : fma2(add2(x, minus2), scale2, make_float2(kShiftP, kShiftP));
     const float2 y = make_float2(exp2_approx(e.x), exp2_approx(e.y));
     sum[i / 2 & 1] = add2(sum[i / 2 & 1], y);
     h[i / 2] = pack2<BF16>(y.x, y.y);
@@ -272,7 +281,7 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
       __syncwarp();
       if (one) mbar_arrive(smem_u32(&s_q_full));
     }
-    float top = -INFINITY, sum = 0.f;
+    float top = -INFINITY, sum = 0.f;         // top: what P is taken against, scaled (fp16: a score as it is)
     bool dead = false;
 #pragma unroll 1
     for (int j = 0; j < tiles; ++j) {
@@ -295,23 +304,31 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
           const float minus = top == -INFINITY ? 0.f : -top;
           return row_exp<BF16>(v[0], h, p.scale_log2, minus) + row_exp<BF16>(v[1], h + 16, p.scale_log2, minus);
         };
-        float add = exps();
-        const bool anew = top == -INFINITY || !(add <= kMostSum);
+        float add, most;
+        bool anew;
+        if (BF16) {
+          add = exps();
+          anew = top == -INFINITY || !(add <= kMostSum);
+        } else {
+          most = fmaxf(row_max(v[0]), row_max(v[1]));                 // scale > 0
+          anew = (most - top) * p.scale_log2 > kSlack;                // NaN where both are infinite: no
+        }
         if (__any_sync(0xffffffffu, anew)) {
           float by = 1.f;
-          const float most = fmaxf(row_max(v[0]), row_max(v[1])) * p.scale_log2;        // scale > 0
+          if (BF16) most = fmaxf(row_max(v[0]), row_max(v[1])) * p.scale_log2;
           if (anew && most > top) {
-            by = exp2_approx(top - most);
+            by = exp2_approx(BF16 ? top - most : (top - most) * p.scale_log2);
             top = most;
             sum *= by;
           }
-          add = exps();
+          if (BF16) add = exps();
           if (j > 0) {
             if (!warp_wait(smem_u32(&s_o_done[b ^ 1]), (uint32_t)((j - 1) >> 1) & 1u, abort_flag)) { dead = true; break; }
             tc_fence_after();
             scale_row(lanes + kColO, p.d, by);
           }
         }
+        if (!BF16) add = exps();
         sum += add;
         tmem_st32(lanes + kColS + kN * b, h);
         tmem_st_wait();
@@ -322,7 +339,7 @@ forward_tc_kernel(const __grid_constant__ Params p, const __grid_constant__ Tile
     }
     if (!dead && (tiles == 0 || warp_wait(smem_u32(&s_o_done[(tiles - 1) & 1]), (uint32_t)((tiles - 1) >> 1) & 1u, abort_flag))) {
       tc_fence_after();
-      if (any_row) store_out<BF16>(p, w, head, lanes + kColO, warp * 32 + lane, rows, top, sum);
+      if (any_row) store_out<BF16>(p, w, head, lanes + kColO, warp * 32 + lane, rows, BF16 ? top : fmaf(top, p.scale_log2, -kShiftP), sum);
     }
   } else if (warp == kScoreWarp) {
     // ======================= MMAs of S =======================

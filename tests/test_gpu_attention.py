@@ -407,3 +407,18 @@ def test_a_thousand_scans(dtype):
     lq, lk = [i % 3 for i in range(1000)], [i % 4 * 5 for i in range(1000)]
     check(*both(inputs(lq, lk, 2, 1, 32, TYPES[dtype], seed=23), True))
     check(*both(inputs([1] * 1000, lk, 2, 2, 64, TYPES[dtype], seed=24), False))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("d", [8, 64, 128])
+@pytest.mark.parametrize("at", [5, 20000, 39999])
+def test_one_key_above_a_long_flat_rest(d, at, dtype):
+    """What a key far below the largest one gets is little, but tens of thousands of them are not, and their values are all the same: what is
+    lost of them does not average out.  Query i has one key that is 10 + i above the others, whose scores are zero."""
+    t, n, rows = TYPES[dtype], 40000, 14
+    q, k = torch.zeros(rows, 1, d, device=DEV), torch.zeros(n, 1, d, device=DEV)
+    q[:, 0, 0] = 10.0 + torch.arange(rows, device=DEV)    # exact in every type, and so are the scores
+    k[at, 0, 0] = 1.0
+    v = torch.ones(n, 1, d, device=DEV)
+    v[at] = 0.0
+    check(*both((q.to(t), k.to(t), v.to(t), ptr([rows]), ptr([n]), None), True, scale=1.0))
