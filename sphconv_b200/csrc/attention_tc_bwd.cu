@@ -15,9 +15,9 @@
 // dS that lay there are complete, and with two or three places (TMEM's room) this chain of handshakes is what a tile takes.  Warps 12 and
 // 13 bring columns and rows, by TMA or, where rows are missing or strides unfit, row by row with cp.async, which fills in zeros.
 //
-// float16 has no room below 2^-24: P is held times 2^12, and dS times a power of two of its row's own, that follows the row's largest
-// value down when that outgrows the type (the accumulator is scaled along).  Even and odd tiles add to one accumulator, so the two
-// warps that have a row take turns at it.
+// float16 has no room below 2^-24: P is held times 2^15 (its largest is 1; what the rounding of a score in the millions may put on that is
+// cut off), and dS times a power of two of its row's own, that follows the row's largest value down when that outgrows the type (the
+// accumulator is scaled along).  Even and odd tiles add to one accumulator, so the two warps that have a row take turns at it.
 //
 // A score's gradients cancel - dS sums to zero over a query's keys - so dS goes into its products as two values of the rows' type, itself and
 // what that lost, one product more for either gradient.  P for dV is rounded, and delta comes from the rounded output: with bf16 rows
@@ -37,7 +37,7 @@ namespace {
 constexpr int kC = 64;                        // columns of a tile
 constexpr int kRowWarps = 8, kScoreWarp = 8, kGradWarp = 10, kColumnWarp = 12;
 constexpr int kThreadsTc = 14 * 32;
-constexpr float kShiftP = 12.f;               // fp16: P times 2^12
+constexpr float kShiftP = 15.f;               // fp16: P times 2^15
 constexpr float kMostDs = 49152.f, kAimDs = 512.f;    // fp16: dS is scaled to the latter when it would pass the former
 
 template <int DP, bool KEYS>
@@ -57,7 +57,7 @@ struct Maps {
 };
 
 // P and dS of 16 columns of a row from its S and dP: minus_lse and minus_delta are the row's (4 values alike) or 16 of the columns.
-// Times 2^12 both in fp16, which the lse has taken in.
+// Times 2^15 both in fp16, which the lse has taken in.
 __device__ __forceinline__ void p_and_ds(uint32_t (&v)[16], uint32_t (&u)[16], float scale, const float* minus_lse, const float* minus_delta,
                                          bool columns) {
   const float2 scale2 = make_float2(scale, scale);
@@ -75,6 +75,15 @@ __device__ __forceinline__ void p_and_ds(uint32_t (&v)[16], uint32_t (&u)[16], f
       u[i + k] = __float_as_uint(y.x); u[i + k + 1] = __float_as_uint(y.y);
     }
   }
+}
+
+// Two values of P; at most 65504 in fp16.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_p(float a, float b) {
+  if (BF16) return pack2<BF16>(a, b);
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
 }
 
 // One tile of rows against a part of the columns.
@@ -311,7 +320,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
             piece(c, v, u);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              if (KEYS) h[i] = pack2<BF16>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+              if (KEYS) h[i] = pack_p<BF16>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
               float2 y = make_float2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
               if (!BF16) y = mul2(y, make_float2(f, f));
               e[i] = pack2<BF16>(y.x, y.y);

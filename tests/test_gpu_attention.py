@@ -422,3 +422,25 @@ def test_one_key_above_a_long_flat_rest(d, at, dtype):
     v = torch.ones(n, 1, d, device=DEV)
     v[at] = 0.0
     check(*both((q.to(t), k.to(t), v.to(t), ptr([rows]), ptr([n]), None), True, scale=1.0))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("d", [8, 64, 128])
+def test_a_key_far_below_another_for_many_queries(d, dtype):
+    """The value of a key that tens of thousands of queries give the same little weight: what its gradient loses does not average out.  The
+    two keys of scan i are 14 + i apart, and the gradient is 40000 times e^-(14 + i).
+
+    Not of d_q and d_k: `out`, here e^-(14 + i) in all channels, is rounded in steps of 2^-24 in float16, delta is the sum of d of them, and
+    off by up to d 2^-25 where it is itself no more; the bounds take the rounding for one of half a step relative to `out`."""
+    t, n, scans = TYPES[dtype], 40000, 12
+    q, k = torch.zeros(scans * n, 1, d, device=DEV), torch.zeros(2 * scans, 1, d, device=DEV)
+    q[:, 0, 0] = 14.0 + torch.arange(scans, device=DEV).repeat_interleave(n)
+    k[::2, 0, 0] = 1.0
+    v = torch.ones(2 * scans, 1, d, device=DEV)
+    v[::2] = 0.0
+    q, k, v = (x.to(t).requires_grad_() for x in (q, k, v))
+    q_ptr, k_ptr = ptr([n] * scans), ptr([2] * scans)
+    out = cross_attention(q, k, v, q_ptr, k_ptr, scale=1.0)
+    d_out = torch.ones_like(out)
+    d_v, = torch.autograd.grad(out, v, d_out)
+    check({"out": out, "d_v": d_v}, attention64(q, k, v, q_ptr, k_ptr, scale=1.0, d_out=d_out))
