@@ -266,3 +266,23 @@ def test_gates_at_their_ends(dtype):
     d_block, d_gate = torch.autograd.grad(out.float().sum(), (block, gate))
     assert torch.equal(d_block[:, 0].float(), torch.tensor([0.0, 0.0, 0.5, 1.0, 1.0], device=DEV))
     assert torch.equal(d_gate[:, 0].float(), torch.tensor([0.0, 0.0, 0.5, 0.0, 0.0], device=DEV))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("c", [64, 2048])
+def test_layer_norm_of_rows_whose_values_are_all_alike(c, dtype):
+    """Sums of 2^k equal values are exact, and so is their mean: every deviation is zero, far from zero as near to it, and what it is
+    multiplied with, 1 / sqrt(eps), must not bring anything back."""
+    t = TYPES[dtype]
+    x = torch.tensor([0.0, 0.1, -3.3, 1000.1, 30011.0], device=DEV).to(t)[:, None].expand(5, c).contiguous().requires_grad_()
+    w, b = torch.full((c,), 1.5, device=DEV, requires_grad=True), torch.linspace(-1, 1, c, device=DEV, requires_grad=True)
+    y = row_norm(x, w, b, center=True)
+    assert torch.equal(y, b.detach().to(t).expand(5, c))
+    d_w, = torch.autograd.grad(y.float().square().sum(), w)
+    assert not d_w.any()
+    gate = torch.zeros(5, 1, device=DEV, dtype=t)
+    out, normed = residual_norm(x, x.detach(), w, b, gate=gate, next_weight=w, center=True)
+    want = (x.detach().float() + 0.5 * b.detach()).to(t)
+    assert torch.equal(out, want)
+    d_w, = torch.autograd.grad(out.float().sum(), w)
+    assert not d_w.any()
