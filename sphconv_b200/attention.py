@@ -21,7 +21,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_ptr: to
     belongs to no scan, get zeros, and so do their gradients.  scale: 1 / sqrt(channels) by default.
 
     Scores, softmax and sums are float32; 16-bit rows have their probabilities rounded to their type in front of the product with v.
-    Differentiable once, in q, k and v; results do not depend on the run.  Pointers out of order or out of range are
+    Differentiable once, backward, in q, k and v; results do not depend on the run.  Pointers out of order or out of range are
     reported by check_status()."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.dim() and q.shape[-1] else 1.0

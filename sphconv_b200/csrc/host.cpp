@@ -73,6 +73,19 @@ void require_cuda(const optional<Tensor>& t) {
   if (t) require_cuda(*t);
 }
 
+// No operator carries a forward-mode tangent on: refused, where the result would come without one, a derivative of zero.
+void no_tangent(const Tensor& t) {
+  if (t.defined() && t._fw_grad(0).defined()) fail("sphconv_b200 ops have no forward-mode derivatives");
+}
+template <typename... T>
+void no_tangents(const T&... tensors) {
+  auto one = [](const auto& t) {
+    if constexpr (std::is_same_v<std::decay_t<decltype(t)>, Tensor>) no_tangent(t);
+    else if (t) no_tangent(*t);
+  };
+  (one(tensors), ...);
+}
+
 void* ptr(const Tensor& t) { return t.data_ptr(); }
 void* ptr(const optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; }
 int32_t* ints(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
@@ -452,6 +465,7 @@ Tensor conv_gather(const Tensor& rows, const Tensor& weight, const optional<Tens
   require_cuda(nbr);
   require_cuda(scale);
   require_cuda(bias);
+  no_tangents(rows, weight, scale, bias);
   const int code = dtype_code(rows, "feature");
   if (weight.scalar_type() != rows.scalar_type())
     fail(std::string("feature (") + c10::toString(rows.scalar_type()) + ") and weight (" + c10::toString(weight.scalar_type()) +
@@ -701,6 +715,7 @@ struct NormLayer : public torch::autograd::Function<NormLayer> {
 py::tuple residual_norm(const optional<Tensor>& block, const Tensor& residual, const optional<Tensor>& gate,
                         const optional<Tensor>& weight, const optional<Tensor>& bias, const optional<Tensor>& scale,
                         const optional<Tensor>& next_weight, const optional<Tensor>& next_bias, double eps, bool center) {
+  no_tangents(block, residual, gate, weight, bias, scale, next_weight, next_bias);
   bool train = residual.requires_grad();
   for (const auto* t : {&block, &gate, &weight, &bias, &scale, &next_weight, &next_bias}) train |= *t && (*t)->requires_grad();
   Tensor out, normed;
@@ -818,6 +833,7 @@ struct AttentionLayer : public torch::autograd::Function<AttentionLayer> {
 
 Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_ptr, const Tensor& k_ptr,
                        const optional<Tensor>& mask, double scale) {
+  no_tangents(q, k, v);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return AttentionLayer::apply(q, k, v, q_ptr, k_ptr, mask, scale);
   return attention_forward(attention_inputs(q, k, v, q_ptr, k_ptr, mask, scale), false).first;

@@ -19,7 +19,7 @@ def row_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]
     (x - mean) / sqrt(var + eps) * weight + bias.
 
     x: contiguous float32, float16 or bfloat16 rows of at most 8192 channels.  weight, bias [C]: any of these types.  Statistics are
-    float32; the result has the dtype of x.  Differentiable once."""
+    float32; the result has the dtype of x.  Differentiable once, backward."""
     return C.host().residual_norm(None, x, None, None, None, None, weight, bias, eps, center)[1]
 
 
@@ -35,7 +35,7 @@ def residual_norm(block: torch.Tensor, residual: torch.Tensor, weight: Optional[
 
     norm is row_norm's.  block, residual: contiguous rows of one shape and dtype.  gate: logits of that dtype, the rows' shape or
     one value a row [..., 1].  weight, bias, scale, next_weight, next_bias [C]: float32, float16 or bfloat16.  All of them are
-    differentiable (once); gradients of the parameters are summed in float32 in a fixed order, without atomics."""
+    differentiable (once, backward); gradients of the parameters are summed in float32 in a fixed order, without atomics."""
     return C.host().residual_norm(block, residual, gate, weight, bias, scale, next_weight, next_bias, eps, center)
 
 
