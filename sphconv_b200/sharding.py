@@ -161,11 +161,47 @@ def grad_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Te
         return torch.stack([g.double().square().sum() for g in grads]).sum().sqrt().float()
 
 
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the values fill their memory, in any order of the dimensions."""
+    expected = 1
+    for stride, size in sorted((stride, size) for stride, size in zip(t.stride(), t.shape) if size != 1):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _check_clip(grads: Sequence[torch.Tensor], out: Sequence[torch.Tensor]) -> None:
+    """What clipping refuses, on the CPU as the native call does it for tensors on a GPU."""
+    spans = []                                       # (begin, end, written) of memory that is read or written
+    for g, o in zip(grads, out):
+        for t in (g, o):
+            if t.device != grads[0].device:
+                raise RuntimeError("gradients on several devices: take their norms apart")
+            if t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+                raise RuntimeError("gradients are float32, float16 or bfloat16")
+            if t.numel() and not _dense(t):
+                raise RuntimeError("sphconv_b200 ops need contiguous tensors")
+        if g.shape != o.shape or (g.stride() != o.stride() and not (g.is_contiguous() and o.is_contiguous())):
+            raise RuntimeError("a destination must have its gradient's shape and layout")
+        if not g.numel():
+            continue
+        spans.append((o.data_ptr(), o.data_ptr() + o.numel() * o.element_size(), True))
+        if o.data_ptr() != g.data_ptr() or o.dtype != g.dtype:
+            spans.append((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size(), False))
+    ends = {True: 0, False: 0}                       # of what is written, and of what is read, so far
+    for begin, end, written in sorted(spans):
+        if begin < ends[True] or (written and begin < ends[False]):
+            raise RuntimeError("a gradient is in the list twice, or overlaps another one or a destination")
+        ends[written] = max(ends[written], end)
+
+
 def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None,
                    norm_type: float = 2.0) -> torch.Tensor:
     """Every gradient times min(1, max_norm / (norm + 1e-6)), in place or into `out` (tensors of the same shapes, of any of the
-    dtypes: rounded once); returns the norm before clipping.  A norm that is not finite makes the gradients so, as in
-    torch.nn.utils.clip_grad_norm_.  A tensor that is listed twice, or that overlaps another one or a destination, is refused."""
+    dtypes: rounded once); returns the norm before clipping.  A norm that is NaN makes all gradients NaN; an infinite one makes them zero
+    and those that are infinite NaN, as torch.nn.utils.clip_grad_norm_ does.  Tensors are dense, on one device (the CPU too), float32,
+    float16 or bfloat16.  One that is listed twice, or that overlaps another one or a destination, is refused."""
     largest, grads = _largest(norm_type), list(grads)
     if not max_norm >= 0:
         raise ValueError("max_norm must not be negative")
@@ -175,12 +211,12 @@ def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, out: Optional
     if grads and grads[0].is_cuda:
         from . import _capi
         return _capi.host().grad_clip(grads, out, float(max_norm), largest)
-    if len({g.data_ptr() for g in grads if g.numel()}) < sum(g.numel() > 0 for g in grads):
-        raise RuntimeError("a gradient is in the list twice")
+    to = grads if out is None else out
+    _check_clip(grads, to)
     norm = grad_norm(grads, norm_type)
     with torch.no_grad():
         by = torch.clamp(max_norm / (norm + 1e-6), max=1.0)
-        for g, o in zip(grads, grads if out is None else out):
+        for g, o in zip(grads, to):
             o.copy_(g.float() * by)
     return norm
 

@@ -62,6 +62,30 @@ def test_cpu_refusals():
     assert clip_grad_norm_([torch.nn.Parameter(g)], 1.0).item() == 0.0 and grad_norm([]).item() == 0.0
 
 
+def test_cpu_refuses_what_the_gpu_refuses():
+    g = torch.ones(64)
+    other = torch.empty(32)
+    for grads, out in (([g, g], None), ([g[:40], g[30:]], None), ([g[:40], g[:8]], None),
+                       ([g[:32], g[32:]], [g[1:33], other]), ([g[:32], g[32:]], [other, other]),
+                       ([g[:32], g[32:]], [other, other[:32]]), ([g[32:], g[:32]], [g[:32], other]),
+                       ([g], [torch.empty(63)]), ([g[:4]], [torch.empty(1, 4)]), ([g[:1]], [torch.empty(4)]),
+                       ([g.view(8, 8)], [torch.empty(8, 8).t()]), ([g.double()], None), ([g], [torch.empty(64).double()]),
+                       ([g[::2]], None), ([g[:1].expand(4)], None), ([g.bfloat16()], [g.bfloat16().view(torch.float16).double()]),
+                       ([g[:32]], [g.view(torch.bfloat16)[:32]]), ([g, g.to("meta")], None)):
+        kept = g.clone()
+        with pytest.raises(RuntimeError):
+            clip_gradients(grads, 1.0, out=out)
+        assert torch.equal(g, kept)                           # nothing was written
+    assert grad_norm([g[:40], g[30:]]).item() == pytest.approx(math.sqrt(74))         # reading twice is fine
+    # and what is allowed: neighbours, reading a value for two destinations, an order of dimensions that both have, nothing at all
+    a, b = torch.ones(64), torch.ones(64)
+    clip_gradients([a[:32], a[32:]], 0.5)
+    clip_gradients([b[:32], b[:32]], 0.5, out=[other, torch.empty(32)])
+    clip_gradients([b.view(8, 8).t()], 0.5, out=[torch.empty(8, 8).t()])
+    clip_gradients([b[:0], b[:0], b[:1]], 0.5)
+    check([torch.ones(64)], [a], torch.tensor(8.0), 0.5)
+
+
 SIZES = {
     "one": [1], "odd": [1, 7, 8, 9, 2047, 2048, 2049, 0, 100003], "many": [((i * 7919) % 5000) + 1 for i in range(400)],
     "large": [40_000_001, 3],
