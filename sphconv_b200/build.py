@@ -50,14 +50,14 @@ def _host_command():
             ["-l" + n for n in ("c10", "c10_cuda", "torch", "torch_cpu", "torch_cuda", "torch_python", "cudart", "dl")])
 
 
-HOOKED = ["conv_tc.cu", "conv_tmem.cu"]
+HOOKED = ["conv_tc.cu", "conv_tmem.cu", "attention_tc_bwd.cu"]
 HOOKS_LIB = os.path.join(LIBDIR, "libsphconv_b200_hooks.so")
 
 
 def build_test_hooks(force=False):
-    """A second library for the test of the bounded waits only: the same sources, with HOOKED compiled with
-    -DSPH_TEST_HOOKS (a 10 ms wait limit and the entry point sph_test_withhold_arrival).  The shipped library holds
-    none of it.  Returns the path."""
+    """A second library for the tests of the bounded waits only: the same sources, with HOOKED compiled with
+    -DSPH_TEST_HOOKS (a 10 ms wait limit, and in the convolutions the entry point sph_test_withhold_arrival).  The shipped
+    library holds none of it.  Returns the path."""
     build(force=force)
     if not force and os.path.exists(HOOKS_LIB) and os.path.getmtime(HOOKS_LIB) >= os.path.getmtime(LIB):
         return HOOKS_LIB

@@ -127,6 +127,27 @@ __device__ __forceinline__ bool warp_spin(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity, abort_flag));
 }
 
+// A wait of a whole warp for as long as a walk may take, which scans of any length have: given up only where `walked`, the tiles that the
+// walk has come to, stays as it is for a healthy wait's limit.
+__device__ __noinline__ bool wait_for_walk(uint32_t bar, uint32_t parity, volatile int* abort_flag, const volatile int* walked) {
+  long long t0 = clock64();
+  int before = *walked;
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
+    const int now = *walked;
+    if (__any_sync(0xffffffffu, now != before)) {
+      before = now;
+      t0 = clock64();
+    } else if (__any_sync(0xffffffffu, clock64() - t0 > kWaitLimitCycles)) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+}
+
 // 64-row boxes of queries and dO (QUERIES), or of keys and values, from row `first` of the scan on, N of them each.
 template <int DP, bool QUERIES, int N>
 __device__ __forceinline__ void tma_rows(uint32_t to1, uint32_t to2, const Maps& m, const Params& p, const Item& i, int first, uint32_t bar) {
@@ -149,7 +170,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
   __shared__ __align__(16) float s_stat[kRowWarps][2][kC];  // of a warp's tile: -lse, -delta of the columns
   __shared__ float s_f[2][kM];                // fp16: dS of a row is held times this, of this tile of rows and the last; 0: not known yet
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort;
+  __shared__ int s_abort, s_walked;           // s_walked: tiles of columns so far
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = (int)uniform((uint32_t)tid >> 5);
@@ -157,7 +178,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
   const uint32_t r_at = base, c_at = base + 4 * S::kRowBytes;         // two operands a tile of rows, and a stage of columns
   constexpr int kGrads = KEYS ? 2 : 1;
   if (tid == 0) {
-    s_abort = 0;
+    s_abort = s_walked = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&s_r_full[i]), 1);
       mbar_init(smem_u32(&s_r_empty[i]), 2);
@@ -476,6 +497,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
         const int st = g % ST, first = it.w.first + j * kC, cols = min(kC, it.w.last - first);
         const uint32_t to1 = c_at + st * 2 * S::kColBytes, to2 = to1 + S::kColBytes, bar = smem_u32(&s_c_full[st]);
         if (!warp_wait(smem_u32(&s_c_empty[st]), ((uint32_t)(g / ST) & 1u) ^ 1u, abort_flag)) { dead = true; break; }
+        if (one) *(volatile int*)&s_walked = g;
         if (fit && cols == kC) {
           if (one) {
             mbar_arrive_expect_tx(bar, 2 * S::kColBytes);
@@ -524,7 +546,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) backward_tc_kernel(const __grid
       if (it.tiles == 0) continue;
       const Rows at{p, it};
       const uint32_t to1 = r_at + (n & 1) * 2 * S::kRowBytes, to2 = to1 + S::kRowBytes, bar = smem_u32(&s_r_full[n & 1]);
-      if (!warp_wait(smem_u32(&s_r_empty[n & 1]), ((uint32_t)(n >> 1) & 1u) ^ 1u, abort_flag)) break;
+      // the tile of rows two before this one keeps its place for all of its walk
+      if (!wait_for_walk(smem_u32(&s_r_empty[n & 1]), ((uint32_t)(n >> 1) & 1u) ^ 1u, abort_flag, &s_walked)) break;
       ++n;
       if (fit) {
         if (one) {

@@ -1,10 +1,14 @@
 """Cross attention of queries to the rows of their scan, against the formulas in 64 bits."""
+import ctypes
 import math
+import os
 
 import pytest
 import torch
 
 import sphconv_b200 as sphconv
+from sphconv_b200 import _capi as C
+from sphconv_b200 import build as sph_build
 from sphconv_b200.attention import cross_attention, scan_rows
 from attention_oracle import attention64, check
 
@@ -444,3 +448,41 @@ def test_a_key_far_below_another_for_many_queries(d, dtype):
     d_out = torch.ones_like(out)
     d_v, = torch.autograd.grad(out, v, d_out)
     check({"out": out, "d_v": d_v}, attention64(q, k, v, q_ptr, k_ptr, scale=1.0, d_out=d_out))
+
+
+def test_a_walk_longer_than_a_wait_may_take():
+    """A tile of rows keeps its place while all of its scan is walked over, and what waits for that place waits as long: 62500 steps of
+    about half a microsecond are three times the limit of a wait in the library for tests (10 ms), where this is no failure either.
+    Results are those of the shipped library, whose limit is 0.2 s.  300 tiles of keys give some of the blocks three of them; the scans without
+    rows make the walk look short to the host, so that it is not split into parts."""
+    if not os.path.exists(sph_build.HOOKS_LIB):
+        pytest.skip("test-hooks library not built (python -m sphconv_b200.build)")
+    B, heads, d, nq, nk = 6000, 64, 8, 62500, 38400
+    g = torch.Generator(device=DEV).manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()  # noqa: E731
+    q, k, v, d_out = r(nq, heads, d), torch.zeros(nk, 1, d, device=DEV).bfloat16(), r(nk, 1, d), r(nq, heads, d)
+    ends = [torch.zeros(B + 1, dtype=torch.int32, device=DEV) for _ in "qk"]
+    for e, n in zip(ends, (nq, nk)):
+        e[3001:] = n
+    lse = torch.full((nq, heads), math.log2(nk), device=DEV)            # scores of zero
+    out = v.float().mean(0).bfloat16().expand(nq, heads, d).contiguous()
+    args = C.Attention(B, heads, 1, d, C.SPH_BF16, 1.0, nq, nk, C.ptr(q), C.ptr(k), C.ptr(v), heads * d, d, d, d, d, d,
+                       C.ptr(ends[0]), C.ptr(ends[1]), None)
+    results = []
+    for lib in (C.lib(), ctypes.CDLL(sph_build.HOOKS_LIB)):
+        for name in ("sph_attention_scratch_bytes", "sph_attention_backward"):
+            getattr(lib, name).restype, getattr(lib, name).argtypes = C.SIGNATURES[name]
+        size = lib.sph_attention_scratch_bytes(ctypes.byref(args), 1)
+        assert size == 2 * (B + 2) * 32 + 2 * nq * heads * 4            # plans, delta and counts, and no parts
+        scratch = torch.empty(size, dtype=torch.uint8, device=DEV)
+        dk, dv, status = torch.full_like(k, 7.0), torch.full_like(v, 7.0), torch.zeros(1, dtype=torch.int32, device=DEV)
+        assert lib.sph_attention_backward(ctypes.byref(args), C.ptr(d_out), C.ptr(out), C.ptr(lse), C.ptr(scratch), None, C.ptr(dk),
+                                          C.ptr(dv), C.ptr(status), C.stream_ptr(torch.device(DEV))) == 0
+        torch.cuda.synchronize()
+        assert int(status.item()) == 0
+        results.append((dk, dv))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    # every key has a weight of 1 / nk, to 2^-9, from every query: the sum's terms are 4 million of about 1 / nk
+    want = d_out.double().sum((0, 1)) / nk
+    size = d_out.double().abs().sum((0, 1)) / nk
+    assert ((results[0][1].double()[:, 0] - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -9 + 2.0 ** -12) * size).all()
