@@ -20,7 +20,15 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_ptr: to
     key_mask: bool [m]; rows where it is False are no keys and may hold anything.  A query whose scan has no key, and a row that
     belongs to no scan, get zeros, and so do their gradients.  scale: 1 / sqrt(channels) by default.
 
-    Scores, softmax and sums are float32; 16-bit rows have their probabilities rounded to their type in front of the product with v.
+    Scores, softmax and sums are float32; 16-bit rows have their probabilities rounded to their type in front of the product with v, and
+    gradients take their part of `out` from the rounded one.
+
+    How fast: 16-bit rows run on the tensor cores where channels are a multiple of 8, rows and heads begin on 16-byte boundaries and the
+    scale is positive.  Others take the CUDA cores and many times as long (256 queries and 20 k keys a scan, 8 scans, 4 heads: 85 us with
+    64 channels, 2.8 ms with 60), so projections are better padded.  Where scans have a query row for each key head or less on average, it is
+    taken for a decoding step, which reads a scan's keys once for each of its query rows: queries that are all in one of many scans are
+    better asked by themselves (64 over 87 k keys: 1.6 ms beside 63 scans without any, 48 us alone).
+
     Differentiable once, backward, in q, k and v; results do not depend on the run.  Pointers out of order or out of range are
     reported by check_status()."""
     if scale is None:

@@ -524,9 +524,11 @@ struct Shape {
 bool shape_of(int c, int esize, bool whole, Shape* s) {
   const int full = 16 / esize;
   s->vec = whole ? full : 1;
-  // A piece of 16 bytes a thread, or four elements: what backward keeps of a row in registers, without spilling (float32 rows of 1024
-  // channels, eight values instead of four: backward 97 -> 116 us; bf16 rows of 333, 118 -> 312).  More a thread for rows that would need
-  // more than 512 threads, or 256 where the pieces of float32 rows still fit then (2048 channels: forward 74 -> 59 us).
+  // A piece of 16 bytes a thread, or four elements: what backward keeps of a row in registers (float32 rows of 1024 channels, eight values
+  // instead of four: backward 97 -> 116 us; bf16 rows of 333, 118 -> 312).  Four values, and eight of 16 bits in a root-mean-square norm
+  // without a bias, fit without spilling; eight of 16 bits with a bias or a mean spill 250 to 310 bytes a thread (16384 x 2048 rows, gated:
+  // backward 230 us, 120 without), eight of float32 260 to 490, sixteen of either 850 to 1420.  More a thread for rows that would need more
+  // than 512 threads, or 256 where the pieces of float32 rows still fit then (2048 channels: forward 74 -> 59 us).
   for (const int e : {4, 8, 16}) {
     if (e < s->vec) continue;
     const int most = e == 4 && s->vec == 4 ? 256 : 512;

@@ -35,7 +35,11 @@ class QueryDecoder(nn.Module):
     forward(x): the decoder's own `queries` for every scan -> [B, queries, channels].
     forward(x, rows, q_ptr): any number of queries a scan, rows [n, channels] with scan b's from q_ptr[b] to q_ptr[b+1] -> [n, channels].
     key_mask bool [NNZ]: rows of the tensor that are left out where False.
-    Step after step on the same scans (tokens of a sequence): memory(x) once, then decode(rows, q_ptr, memory) each time."""
+    Step after step on the same scans (tokens of a sequence): memory(x) once, then decode(rows, q_ptr, memory) each time.
+
+    Keys and values are made of x.feature alone: where a row lies in its scan is known to the head as far as the features say it, so a caller
+    that needs positions adds them to the features (an embedding of x.z_idx and of the column, say).  Queries of a scan do not see
+    one another."""
 
     def __init__(self, channels: int, row_channels: int, heads: int, layers: int, queries: int = 0, key_heads: Optional[int] = None,
                  hidden: Optional[int] = None, eps: float = 1e-6, center: bool = False, initial_scale: Optional[float] = None):
