@@ -21,7 +21,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_ptr: to
     belongs to no scan, get zeros, and so do their gradients.  scale: 1 / sqrt(channels) by default.
 
     Scores, softmax and sums are float32; 16-bit rows have their probabilities rounded to their type in front of the product with v, and
-    gradients take their part of `out` from the rounded one.
+    gradients take their part of `out` from the rounded one.  Scores of some millions and more have lost their differences to float32's
+    rounding, and the probabilities with them.
 
     How fast: 16-bit rows run on the tensor cores where channels are a multiple of 8, rows and heads begin on 16-byte boundaries and the
     scale is positive.  Others take the CUDA cores and many times as long (256 queries and 20 k keys a scan, 8 scans, 4 heads: 85 us with

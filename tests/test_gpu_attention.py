@@ -486,3 +486,18 @@ def test_a_walk_longer_than_a_wait_may_take():
     want = d_out.double().sum((0, 1)) / nk
     size = d_out.double().abs().sum((0, 1)) / nk
     assert ((results[0][1].double()[:, 0] - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -9 + 2.0 ** -12) * size).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_gradients_of_scores_that_are_no_numbers(dtype):
+    """A NaN in a query reaches what that query has a part in: its own result and gradient, and its scan's and key head's keys and values."""
+    q, k, v, q_ptr, k_ptr, _ = inputs([140, 9], [200, 31], 4, 2, 64, TYPES[dtype], seed=25)
+    q[3, 1, 5] = float("nan")                             # head 1 reads key head 0
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = cross_attention(*leaves, q_ptr, k_ptr)
+    d_q, d_k, d_v = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    here = torch.zeros(149, 4, dtype=torch.bool, device=DEV)
+    here[3, 1] = True
+    assert out[here].isnan().all() and torch.isfinite(out[~here]).all() and d_q[here].isnan().all() and torch.isfinite(d_q[~here]).all()
+    for g in (d_k, d_v):
+        assert g[:200, 0].isnan().all() and torch.isfinite(g[:200, 1]).all() and torch.isfinite(g[200:]).all()
